@@ -1,0 +1,536 @@
+"""A decode worker's step over a 4-bit KV cache, operator by operator, as
+measurable cases through the package's public entry points.
+
+Kinds of work (`case["kind"]`):
+  tables  block tables, lengths, slots and positions of a step, made on the GPU
+          from the requests' page lists and lengths (build_step_tables)
+  rope    the norms of each query and key head and the rotation of their
+          positions, with K and V written to their BF16 page slots
+          (qk_norm_rope_scatter)
+  write   new K/V rows written to MXFP4 pages and read back as BF16 rows, as a
+          prefill chunk does that attends to what decode will see
+          (scatter_kv_mxfp4, gather_kv_mxfp4)
+  gather  a cached prefix's MXFP4 pages read back as BF16 rows (gather_kv_mxfp4)
+  read    decode attention over MXFP4 pages, one query token per sequence
+          (paged_decode_mxfp4)
+
+An MXFP4 value is an E2M1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives)
+times the power of two that its group of 32 head dims shares (an E8M0 byte:
+2^(byte - 127)). A page holds 16 tokens; per KV head its planes are laid out
+  K       [4 quarters of the dims][16 tokens][dim/8 bytes]
+  V       [4 quads of tokens][16 columns of dim/16 dims][4 tokens][dim/32 bytes]
+  scales  [dim/32 groups][16 tokens], one byte each, for K and V alike
+with the even dim of a byte's two in its low four bits.
+
+Page geometries are those of this repository's workloads: 2 KV heads x 64, 2 x
+128 and 4 x 128 with 7, 6 and 7 query heads each; drawn cases take others too.
+"""
+import math
+import random
+import sys
+from pathlib import Path
+
+import numpy as np
+import torch
+
+own = False
+
+B = 16    # tokens of a page
+G = 32    # head dims that share a scale
+EPS = 1e-6
+# KV heads, head dim, query heads per KV head
+GEOMETRY = {"0.5b": (2, 64, 7), "1.5b": (2, 128, 6), "7b": (4, 128, 7)}
+PROMPTS = (41, 5040, 7040)  # prompt lengths of the mixed serving load
+
+
+def _geometry(name):
+    heads, dim, group = GEOMETRY[name]
+    return dict(heads=heads, dim=dim, group=group)
+
+
+def listed():
+    return [
+        # One user's decode step: a handful of integers, launch-bound.
+        dict(name="tables_1", kind="tables", batch=1, context=5040, chunk=1, prefills=0, padded=0),
+        # A full decode batch padded to the size its graph was captured for.
+        dict(name="tables_256", kind="tables", batch=256, context=7040, chunk=1, prefills=0, padded=37),
+        # Chunked prefill beside decoding requests, and a long table.
+        dict(name="tables_48_chunked", kind="tables", batch=48, context=32768, chunk=2041, prefills=6, padded=0),
+        # One user's decode step, one layer.
+        dict(name="rope_1.5b_1", kind="rope", tokens=1, **_geometry("1.5b"), rotary=128, f32=False, pairs=False, norm=True, padded=0),
+        # Prefill of the 5040-token prefix, one layer.
+        dict(name="rope_1.5b_5040", kind="rope", tokens=5040, **_geometry("1.5b"), rotary=128, f32=False, pairs=False, norm=True, padded=0),
+        # A ragged chunk of FP32 projections, half of the dims rotated, in pairs.
+        dict(name="rope_7b_8191_f32", kind="rope", tokens=8191, **_geometry("7b"), rotary=64, f32=True, pairs=True, norm=True, padded=9),
+        # A decode step's new tokens of 64 sequences, one layer.
+        dict(name="write_0.5b_64", kind="write", tokens=64, **_geometry("0.5b"), f32=False, padded=0),
+        # A prefill chunk, one layer.
+        dict(name="write_7b_8192", kind="write", tokens=8192, **_geometry("7b"), f32=False, padded=0),
+        # The cached prefix of a request that goes on, one layer.
+        dict(name="gather_1.5b_7040", kind="gather", tokens=7040, **_geometry("1.5b"), padded=0),
+        # One user's decode step over a 5040-token context, one layer.
+        dict(name="read_0.5b_1x5040", kind="read", batch=1, context=5040, **_geometry("0.5b"), mixed=False),
+        # A full decode batch of equal long contexts, one layer.
+        dict(name="read_1.5b_64x5040", kind="read", batch=64, context=5040, **_geometry("1.5b"), mixed=False),
+        # A continuous batch of contexts of every length up to 32768 tokens, one layer.
+        dict(name="read_7b_64_mixed", kind="read", batch=64, context=32768, **_geometry("7b"), mixed=True),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    """One more case: any kind, head layout and option, sizes over their logarithm."""
+    kind = rng.choice(["tables", "rope", "rope", "write", "gather", "read", "read", "read"])
+    if kind == "tables":
+        batch = _log_int(rng, 1, 512)
+        prefills = min(batch, rng.choice([0, 0, 1, 4, 8]))
+        chunk = _log_int(rng, 2, 8192 // max(1, prefills)) if prefills else 1
+        return dict(kind=kind, batch=batch, context=_log_int(rng, 16, min(32768, (1 << 23) // batch)), chunk=chunk,
+                    prefills=prefills, padded=rng.choice([0, rng.randint(1, 64)]))
+    layout = dict(heads=rng.choice([1, 2, 2, 3, 4, 4, 8]), dim=rng.choice([64, 128]), group=rng.randint(1, 8))
+    if kind == "read":
+        batch = _log_int(rng, 1, 192)
+        most = 1.4e8 / (layout["heads"] * (layout["dim"] + layout["dim"] // 16)) / batch  # at most 140 MB of pages
+        return dict(kind=kind, batch=batch, context=_log_int(rng, 16, max(64, min(32768, int(most)))), **layout, mixed=rng.random() < 0.6)
+    padded = rng.choice([0, rng.randint(1, 24)])
+    if kind == "rope":
+        tokens = _log_int(rng, 1, 8192 * 36 // (layout["heads"] * (layout["group"] + 2)) // (2 if layout["dim"] == 128 else 1))
+        return dict(kind=kind, tokens=min(tokens, 16384), **layout, rotary=rng.choice([layout["dim"], layout["dim"], layout["dim"] // 2, 16, 48]),
+                    f32=rng.random() < 0.3, pairs=rng.random() < 0.4, norm=rng.random() < 0.8, padded=padded)
+    tokens = _log_int(rng, 1, min(16384, 8192 * 4 * 128 // (layout["heads"] * layout["dim"])))
+    c = dict(kind=kind, tokens=tokens, **layout, padded=padded)
+    return dict(c, f32=rng.random() < 0.3) if kind == "write" else c
+
+
+# ------------------------------------------------------------------ inputs
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _int(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _lengths(case, seed=0):
+    """Context lengths of a batch: all equal, or spread up to the longest (the
+    same lengths for every seed, in an order of its own)."""
+    n, most = case["batch"], case["context"]
+    if not case.get("mixed", True):
+        return [most] * n
+    r = random.Random(n * 100003 + most)
+    lens = [min(most, r.choice(PROMPTS) + r.randint(0, 256) if r.random() < 0.5 else _log_int(r, min(16, most), most)) for _ in range(n)]
+    lens[0] = most
+    random.Random(seed).shuffle(lens)
+    return lens
+
+
+def _requests(case, seed=0):
+    """(context length, new tokens of it) of each request of a step."""
+    lens = sorted(_lengths(case), reverse=True)
+    some = set(random.Random(len(lens)).sample(range(len(lens)), case["prefills"]))
+    all_ = [(n, min(case["chunk"], n) if i in some else 1) for i, n in enumerate(lens)]
+    random.Random(seed).shuffle(all_)
+    return all_
+
+
+def _slots(tokens, padded, gen):
+    """Slots of `tokens` tokens in shuffled pages, the last of them mid-page and
+    `padded` empty rows behind; and the blocks of a pool that holds them."""
+    need = -(-tokens // B)
+    blocks = need + 8
+    perm = torch.randperm(blocks, generator=gen, device="cuda")[:need]
+    slots = (perm[:, None] * B + torch.arange(B, device="cuda")).reshape(-1)[:tokens]
+    return torch.cat([slots, torch.full((padded,), -1, device="cuda")]).to(torch.int32), blocks
+
+
+def _prepare_tables(case, seed):
+    lens, new = zip(*_requests(case, seed))
+    counts = np.array([-(-n // B) for n in lens], np.int64)
+    starts = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    pages = torch.randperm(int(starts[-1]) + 64, generator=_gen(seed), device="cuda")[: int(starts[-1])].to(torch.int32)
+    most, tokens = int(counts.max()), sum(new) + case["padded"]
+    empty = lambda *n: torch.zeros(n, dtype=torch.int32, device="cuda")  # noqa: E731
+    return dict(pages=pages, page_starts=torch.from_numpy(starts).cuda(), cached=_int([a - b for a, b in zip(lens, new)]), new=_int(new),
+                tables=empty(len(lens), most), seq_lens=empty(len(lens)), token_starts=empty(len(lens) + 1), slots=empty(tokens),
+                positions=empty(tokens))
+
+
+def _prepare_rope(case, seed):
+    gen, n, heads, dim = _gen(seed), case["tokens"] + case["padded"], case["heads"], case["dim"]
+    q_heads = heads * case["group"]
+    dtype = torch.float32 if case["f32"] else torch.bfloat16
+    width = (q_heads + 2 * heads) * dim
+    qkv = torch.randn((n, width), generator=gen, device="cuda") * 1.5
+    qkv[:, : (q_heads + heads) * dim] *= torch.rand(width - heads * dim, generator=gen, device="cuda") * 3 + 0.2  # channels of unlike size
+    most = case["tokens"] + 4096
+    first = int(torch.randint(0, 4096, (1,), generator=gen, device="cuda"))
+    positions = torch.arange(first, first + n, device="cuda", dtype=torch.int32)
+    positions[case["tokens"]:] = -1
+    rot = case["rotary"]
+    angle = torch.arange(most, device="cuda", dtype=torch.float64)[:, None] * 1e6 ** (-torch.arange(0, rot, 2, device="cuda", dtype=torch.float64) / rot)
+    weight = lambda: (torch.randn(dim, generator=gen, device="cuda") * 0.2 + 1).to(dtype) if case["norm"] else None  # noqa: E731
+    slots, blocks = _slots(case["tokens"], case["padded"], gen)
+    # one block more than the pool has: the plain form writes rows without a slot there
+    pool = lambda: torch.zeros((blocks + 1) * B, heads, dim, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    return dict(qkv=qkv.to(dtype), positions=positions, cos_sin=torch.cat([angle.cos(), angle.sin()], 1).float(), q_weight=weight(), k_weight=weight(),
+                slots=slots, keys=pool(), values=pool(), q_out=torch.zeros((n, q_heads, dim), dtype=torch.bfloat16, device="cuda"), rows=blocks * B)
+
+
+def _quantise(x):
+    """E2M1 codes, two a byte, and E8M0 bytes of rows x[..., dim]: a group's
+    power of two is that of its largest value less 2 (the largest code, 6, has
+    exponent 2); values round to the nearest code, ties to the even one."""
+    x = x.float().unflatten(-1, (-1, G))
+    top = x.abs().amax(-1)
+    scale = (torch.frexp(top).exponent - 1 - 2 + 127).clamp(0, 254)
+    scale = torch.where(top > 0, scale, torch.zeros_like(scale))
+    a = torch.ldexp(x.abs(), 127 - scale[..., None])
+    code = sum((a > t).to(torch.uint8) for t in (0.25, 1.25, 2.5, 5.0)) + sum((a >= t).to(torch.uint8) for t in (0.75, 1.75, 3.5))
+    code = (code | (x < 0).to(torch.uint8) << 3).flatten(-2)
+    return code[..., 0::2] | code[..., 1::2] << 4, scale.to(torch.uint8)
+
+
+def _values(codes, scale):
+    """The FP32 values that codes [..., dim/2] and scales [..., dim/32] stand for."""
+    lut = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], device=codes.device)
+    lut = torch.cat([lut, -lut])
+    v = lut[torch.stack([codes & 15, codes >> 4], -1).flatten(-2).int()]
+    return torch.ldexp(v.unflatten(-1, (-1, G)), scale[..., None].int() - 127).flatten(-2)
+
+
+def _views(s):
+    """The pools by block, head and place: see the layout above."""
+    heads, dim = s["heads"], s["dim"]
+    return (s["k_pool"].view(-1, heads, 4, B, dim // 8), s["v_pool"].view(-1, heads, 4, 16, 4, dim // 32),
+            s["k_scales"].view(-1, heads, dim // G, B), s["v_scales"].view(-1, heads, dim // G, B))
+
+
+def _put_rows(s, slots, keys, values):
+    """Plain form of the writer: K and V rows [n][heads][dim] into their slots."""
+    k, v, ks, vs = _views(s)
+    block, at = torch.div(slots, B, rounding_mode="floor").long(), (slots % B).long()
+    codes, scale = _quantise(keys)
+    k[block, :, :, at] = codes.unflatten(-1, (4, -1))
+    ks[block, :, :, at] = scale
+    codes, scale = _quantise(values)
+    v[block, :, at // 4, :, at % 4] = codes.unflatten(-1, (16, -1))
+    vs[block, :, :, at] = scale
+
+
+def _get_rows(s, slots):
+    """Plain form of the gather: FP32 K and V rows [n][heads][dim] of the slots."""
+    k, v, ks, vs = _views(s)
+    block, at = torch.div(slots, B, rounding_mode="floor").long(), (slots % B).long()
+    return (_values(k[block, :, :, at].flatten(-2), ks[block, :, :, at]),
+            _values(v[block, :, at // 4, :, at % 4].flatten(-2), vs[block, :, :, at]))
+
+
+def _pages(case, blocks, spare):
+    """Empty MXFP4 pools of one layer, `blocks` pages and `spare` more."""
+    heads, dim = case["heads"], case["dim"]
+    empty = lambda n: torch.zeros((blocks + spare) * n, dtype=torch.uint8, device="cuda")  # noqa: E731
+    half = B * heads * dim // 2
+    return dict(heads=heads, dim=dim, blocks=blocks, k_pool=empty(half), v_pool=empty(half), k_scales=empty(half // 16), v_scales=empty(half // 16))
+
+
+def _fill(s, gen):
+    """Quantised N(0, 1) rows in every slot."""
+    step = max(1, (1 << 25) // (B * s["heads"] * s["dim"]))
+    for first in range(0, s["blocks"], step):
+        at = torch.arange(first * B, min(first + step, s["blocks"]) * B, device="cuda")
+        rows = torch.randn((2, len(at), s["heads"], s["dim"]), generator=gen, device="cuda")
+        _put_rows(s, at, rows[0], rows[1])
+
+
+def _prepare_write(case, seed):
+    gen, n = _gen(seed), case["tokens"] + case["padded"]
+    slots, blocks = _slots(case["tokens"], case["padded"], gen)
+    s = dict(_pages(case, blocks, 1), slots=slots)
+    if case["kind"] == "write":
+        dtype = torch.float32 if case["f32"] else torch.bfloat16
+        s["rows_in"] = (torch.randn((2, n, case["heads"], case["dim"]), generator=gen, device="cuda") * 1.5).to(dtype)
+    else:
+        _fill(s, gen)
+    s["rows_out"] = torch.zeros((2, n, case["heads"], case["dim"]), dtype=torch.bfloat16, device="cuda")
+    return s
+
+
+def _prepare_read(case, seed):
+    gen, lens = _gen(seed), _lengths(case, seed)
+    heads, dim, q_heads = case["heads"], case["dim"], case["heads"] * case["group"]
+    counts = [-(-n // B) for n in lens]
+    most, pages = max(counts), sum(counts) + 16
+    s = _pages(case, pages, 0)
+    _fill(s, gen)
+    ids = torch.randperm(pages, generator=gen, device="cuda").to(torch.int32)
+    width = torch.arange(most, device="cuda")
+    starts = _int(np.concatenate([[0], np.cumsum(counts)[:-1]]).tolist())
+    live = width < _int(counts)[:, None]
+    s["tables"] = torch.where(live, ids[(starts[:, None] + width).clamp(max=pages - 1)], torch.full_like(live, -1, dtype=torch.int32)).contiguous()
+    s["q"] = (torch.randn((len(lens), q_heads, dim), generator=gen, device="cuda") * 2).to(torch.bfloat16)
+    s["out"] = torch.zeros_like(s["q"])
+    s["seq_lens"], s["most"] = _int(lens), most
+    # partial results: a part per four pages of every sequence, at most 64 MB
+    s["workspace"] = torch.empty(min(len(lens) * q_heads * (dim + 2) * 4 * -(-most // 4), max(64 << 20, len(lens) * q_heads * (dim + 2) * 4)),
+                                 dtype=torch.uint8, device="cuda")
+    return s
+
+
+def prepare(case, seed):
+    kind = case["kind"]
+    s = _prepare_tables(case, seed) if kind == "tables" else _prepare_rope(case, seed) if kind == "rope" else \
+        _prepare_read(case, seed) if kind == "read" else _prepare_write(case, seed)
+    s["case"] = case
+    return s
+
+
+# ------------------------------------------------------------------ plain forms
+def _plain_tables(s):
+    new, counts = s["new"], s["page_starts"].diff()
+    ends = new.cumsum(0, dtype=torch.int32)
+    s["token_starts"][1:] = ends
+    s["seq_lens"].copy_(s["cached"] + new)
+    last = len(s["pages"]) - 1
+    j = torch.arange(s["tables"].shape[1], device="cuda")
+    s["tables"].copy_(torch.where(j < counts[:, None], s["pages"][(s["page_starts"][:-1, None] + j).clamp(max=last)], -1))
+    t = torch.arange(len(s["slots"]), device="cuda", dtype=torch.int32)
+    b = torch.searchsorted(ends, t, right=True)
+    live, b = b < len(new), b.clamp(max=len(new) - 1)
+    at = s["cached"][b] + t - s["token_starts"][b]
+    page = s["pages"][(s["page_starts"][b] + torch.div(at, B, rounding_mode="floor")).clamp(0, last)]
+    s["positions"].copy_(torch.where(live, at, -1))
+    s["slots"].copy_(torch.where(live, page * B + at % B, -1))
+
+
+def _plain_head(x, weight, cos, sin, case):
+    """Norm and rotation of x[n][heads][dim] in FP32."""
+    if case["norm"]:
+        x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + EPS) * weight.float()
+    rot = case["rotary"]
+    cos, sin = cos[:, None], sin[:, None]
+    if case["pairs"]:
+        a, b = x[..., 0:rot:2], x[..., 1:rot:2]
+        turned = torch.stack([a * cos - b * sin, b * cos + a * sin], -1).flatten(-2)
+    else:
+        a, b = x[..., : rot // 2], x[..., rot // 2:rot]
+        turned = torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+    return torch.cat([turned, x[..., rot:]], -1)
+
+
+def _plain_rope(s):
+    case = s["case"]
+    heads, dim, rot = case["heads"], case["dim"], case["rotary"]
+    rows = s["qkv"].float().unflatten(-1, (-1, dim))
+    q, k, v = rows.split([heads * case["group"], heads, heads], 1)
+    cos, sin = s["cos_sin"][s["positions"].clamp(min=0)].split(rot // 2, 1)
+    live = (s["positions"] >= 0)[:, None, None]
+    s["q_out"].copy_(torch.where(live, _plain_head(q, s["q_weight"], cos, sin, case), s["q_out"].float()))
+    at = torch.where(s["slots"] >= 0, s["slots"], s["rows"]).long()
+    s["keys"][at] = _plain_head(k, s["k_weight"], cos, sin, case).to(torch.bfloat16)
+    s["values"][at] = v.to(torch.bfloat16)
+
+
+def _plain_rows(s):
+    spare = torch.where(s["slots"] >= 0, s["slots"], s["blocks"] * B)
+    if "rows_in" in s:
+        _put_rows(s, spare, s["rows_in"][0], s["rows_in"][1])
+    rows = torch.stack(_get_rows(s, spare))
+    s["rows_out"].copy_(torch.where((s["slots"] >= 0)[:, None, None], rows, s["rows_out"].float()))
+
+
+def _plain_read(s):
+    case = s["case"]
+    heads, dim, group = case["heads"], case["dim"], case["group"]
+    batch, most = s["tables"].shape
+    slots = (s["tables"].clamp(min=0)[:, :, None] * B + torch.arange(B, device="cuda")).reshape(-1)
+    k, v = (x.view(batch, most * B, heads, dim).transpose(1, 2).contiguous() for x in _get_rows(s, slots))
+    q = s["q"].float().view(batch, heads, group, dim) / math.sqrt(dim)
+    scores = torch.matmul(q, k.transpose(2, 3).contiguous())
+    live = (torch.arange(most * B, device="cuda") < s["seq_lens"][:, None])[:, None, None]
+    scores = torch.where(live, scores, -math.inf)
+    p = torch.exp(scores - scores.amax(-1, keepdim=True))
+    s["out"].copy_((torch.matmul(p, v) / p.sum(-1, keepdim=True)).view(batch, heads * group, dim))
+
+
+# ------------------------------------------------------------------ the calls
+def _package():
+    path = str(Path(__file__).resolve().parent.parent / "paged-batch-engine_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import pbe_handoff
+    return pbe_handoff
+
+
+def _own_tables(s):
+    P = _package()
+    P.build_step_tables(s["pages"].data_ptr(), len(s["pages"]), s["page_starts"].data_ptr(), s["cached"].data_ptr(), s["new"].data_ptr(), len(s["new"]), B,
+                        s["tables"].data_ptr(), s["tables"].shape[1], s["seq_lens"].data_ptr(), s["token_starts"].data_ptr(), s["slots"].data_ptr(),
+                        s["positions"].data_ptr(), len(s["slots"]), stream=torch.cuda.current_stream().cuda_stream)
+
+
+def _own_rope(s):
+    P, case = _package(), s["case"]
+    heads, dim = case["heads"], case["dim"]
+    q_heads, qkv = heads * case["group"], s["qkv"]
+    width, at, e = qkv.shape[1], qkv.data_ptr(), qkv.element_size()
+    used = s["rows"] * heads * dim * 2
+    P.qk_norm_rope_scatter(at, width, at + q_heads * dim * e, width, at + (q_heads + heads) * dim * e, width,
+                           P.PBE_IN_F32 if case["f32"] else P.PBE_IN_BF16, qkv.shape[0], q_heads, heads, dim,
+                           s["q_weight"].data_ptr() if case["norm"] else 0, s["k_weight"].data_ptr() if case["norm"] else 0, EPS,
+                           s["positions"].data_ptr(), s["cos_sin"].data_ptr(), s["cos_sin"].shape[0], case["rotary"],
+                           P.PBE_ROPE_PAIRS if case["pairs"] else P.PBE_ROPE_HALVES, s["slots"].data_ptr(), B, P.PBE_KV_BF16, s["q_out"].data_ptr(),
+                           s["keys"].data_ptr(), used, s["values"].data_ptr(), used, stream=torch.cuda.current_stream().cuda_stream)
+
+
+def _own_rows(s):
+    P, stream = _package(), torch.cuda.current_stream().cuda_stream
+    heads, dim, n = s["heads"], s["dim"], len(s["slots"])
+    half = B * heads * dim // 2 * s["blocks"]
+    pools = (s["k_pool"].data_ptr(), half, s["v_pool"].data_ptr(), half, s["k_scales"].data_ptr(), half // 16, s["v_scales"].data_ptr(), half // 16)
+    if "rows_in" in s:
+        rows = s["rows_in"]
+        P.scatter_kv_mxfp4(rows[0].data_ptr(), rows[1].data_ptr(), P.PBE_IN_F32 if rows.dtype == torch.float32 else P.PBE_IN_BF16, n,
+                           s["slots"].data_ptr(), heads, dim, *pools, stream=stream)
+    P.gather_kv_mxfp4(*pools, s["slots"].data_ptr(), n, heads, dim, s["rows_out"][0].data_ptr(), s["rows_out"][1].data_ptr(), stream=stream)
+
+
+def _own_read(s):
+    P, case = _package(), s["case"]
+    P.paged_decode_mxfp4(s["k_pool"].data_ptr(), s["v_pool"].data_ptr(), s["k_pool"].numel(), s["k_scales"].data_ptr(), s["v_scales"].data_ptr(),
+                         s["k_scales"].numel(), case["heads"], case["dim"], s["q"].data_ptr(), s["out"].data_ptr(), case["batch"],
+                         case["heads"] * case["group"], s["tables"].data_ptr(), s["seq_lens"].data_ptr(), s["most"], 0, s["workspace"].data_ptr(),
+                         s["workspace"].numel(), stream=torch.cuda.current_stream().cuda_stream)
+
+
+def run(state):
+    s, kind = state, state["case"]["kind"]
+    if kind == "tables":
+        _own_tables(s) if own else _plain_tables(s)
+        return {k: s[k] for k in ("tables", "seq_lens", "token_starts", "slots", "positions")}
+    if kind == "rope":
+        _own_rope(s) if own else _plain_rope(s)
+        return {"q": s["q_out"], "keys": s["keys"][: s["rows"]], "values": s["values"][: s["rows"]]}
+    if kind == "read":
+        _own_read(s) if own else _plain_read(s)
+        return {"out": s["out"]}
+    _own_rows(s) if own else _plain_rows(s)
+    return {"rows": s["rows_out"]}
+
+
+def work(case):
+    kind = case["kind"]
+    if kind == "tables":
+        counts = [-(-n // B) for n in _lengths(case)]
+        tokens = sum(new for _, new in _requests(case))
+        return {"bytes": 4 * (sum(counts) + len(counts) * max(counts) + 5 * len(counts) + 2 + 2 * (tokens + case["padded"])), "flops": 0}
+    heads, dim, q_heads = case["heads"], case["dim"], case["heads"] * case["group"]
+    if kind == "read":
+        total = sum(_lengths(case))
+        pages = sum(-(-n // B) for n in _lengths(case))
+        return {"bytes": total * 2 * heads * (dim // 2 + dim // G) + 4 * pages + 4 * case["batch"] * (1 + q_heads * dim), "flops": 4 * total * q_heads * dim}
+    n = case["tokens"]
+    if kind == "rope":
+        e = 4 if case["f32"] else 2
+        # a row's positions, slot and line of the table, its inputs and its outputs
+        return {"bytes": n * (8 + 4 * case["rotary"] + (q_heads + 2 * heads) * dim * (e + 2)), "flops": n * (q_heads + heads) * dim * 7}
+    row = 2 * heads * dim
+    page = 2 * heads * (dim // 2 + dim // G)
+    if kind == "gather":
+        return {"bytes": n * (4 + page + 2 * row), "flops": 0}
+    return {"bytes": n * (8 + (4 if case["f32"] else 2) * row + 2 * page + 2 * row), "flops": 0}
+
+
+# ------------------------------------------------------------------ in 64 bits
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def _nearest(row):
+    """Groups of 32 doubles as MXFP4 holds them, from the definition."""
+    x = row.unflatten(-1, (-1, G))
+    top = x.abs().amax(-1, keepdim=True)
+    e = torch.floor(torch.log2(torch.where(top > 0, top, torch.ones_like(top))))
+    e = torch.where(2.0 ** e > top, e - 1, e)          # log2 of a value just below a power of two may round up to it
+    unit = 2.0 ** (e - 2).clamp(min=-127.0)
+    y = x.abs() / unit
+    codes = torch.tensor(_E2M1, dtype=torch.float64, device=row.device)
+    far = (y[..., None] - codes).abs()
+    far[..., 0::2] -= 1e-12                            # ties go to the even code; no other distances are as near
+    return (codes[far.argmin(-1)] * x.sign() * unit).flatten(-2)
+
+
+def _decoded(s, pool, scales, block, at, value):
+    """Rows of the given blocks and tokens in 64 bits, byte by byte of the layout."""
+    heads, dim = s["heads"], s["dim"]
+    d, h = torch.arange(dim, device="cuda"), torch.arange(heads, device="cuda")[:, None]
+    if value:
+        byte = (at // 4)[:, None, None] * (2 * dim) + (d // (dim // 16)) * (dim // 8) + (at % 4)[:, None, None] * (dim // 32) + d % (dim // 16) // 2
+    else:
+        byte = (d // (dim // 4)) * (2 * dim) + at[:, None, None] * (dim // 8) + d % (dim // 4) // 2
+    raw = pool[(block[:, None, None] * heads + h) * (8 * dim) + byte]
+    code = torch.where(d % 2 == 1, raw >> 4, raw & 15).long()
+    table = torch.tensor(_E2M1 + tuple(-v for v in _E2M1), dtype=torch.float64, device="cuda")
+    exponent = scales[(block[:, None, None] * heads + h) * (dim // 2) + (d // G) * B + at[:, None, None]]
+    return table[code] * 2.0 ** (exponent.double() - 127)
+
+
+def _exact_rope(case, seed):
+    s = _prepare_rope(case, seed)
+    heads, dim, rot, n = case["heads"], case["dim"], case["rotary"], case["tokens"]
+    q_heads = heads * case["group"]
+    rows = s["qkv"][:n].double().view(n, q_heads + 2 * heads, dim)
+    turn = s["cos_sin"].double()[s["positions"][:n].long()]
+    turn = torch.complex(turn[:, : rot // 2], turn[:, rot // 2:])[:, None]
+    out = []
+    for x, w in ((rows[:, :q_heads], s["q_weight"]), (rows[:, q_heads:-heads], s["k_weight"])):
+        x = x.clone()
+        if case["norm"]:
+            x = x / torch.sqrt((x * x).sum(-1, keepdim=True) / dim + EPS) * w.double()
+        lo, hi = (slice(0, rot, 2), slice(1, rot, 2)) if case["pairs"] else (slice(0, rot // 2), slice(rot // 2, rot))
+        z = torch.complex(x[..., lo], x[..., hi]) * turn
+        x[..., lo], x[..., hi] = z.real, z.imag
+        out.append(x)
+    q = torch.zeros(s["q_out"].shape, dtype=torch.float64, device="cuda")
+    q[:n] = out[0]
+    pools = []
+    for x in (out[1], rows[:, -heads:]):
+        pool = torch.zeros((s["rows"], heads, dim), dtype=torch.float64, device="cuda")
+        pool[s["slots"][:n].long()] = x
+        pools.append(pool)
+    return {"q": q, "keys": pools[0], "values": pools[1]}
+
+
+def exact(case, seed):
+    kind = case["kind"]
+    if kind == "tables":
+        return None  # whole numbers
+    if kind == "rope":
+        return _exact_rope(case, seed)
+    if kind == "read":
+        s = _prepare_read(case, seed)
+        heads, dim, group = case["heads"], case["dim"], case["group"]
+        out = torch.empty(s["out"].shape, dtype=torch.float64, device="cuda")
+        for b, n in enumerate(s["seq_lens"].tolist()):
+            t = torch.arange(n, device="cuda")
+            block = s["tables"][b].long()[t // B]
+            k, v = (_decoded(s, s[p], s[c], block, t % B, p == "v_pool").transpose(0, 1).contiguous()
+                    for p, c in (("k_pool", "k_scales"), ("v_pool", "v_scales")))
+            q = s["q"][b].double().view(heads, group, dim)
+            p = torch.softmax(torch.bmm(q, k.transpose(1, 2).contiguous()) / math.sqrt(dim), -1)
+            out[b] = torch.bmm(p, v).reshape(heads * group, dim)
+        return {"out": out}
+    s = _prepare_write(case, seed)
+    n = case["tokens"]
+    rows = torch.zeros(s["rows_out"].shape, dtype=torch.float64, device="cuda")
+    if kind == "write":
+        for first in range(0, n, 1024):  # the distances to all codes take eight times the rows
+            rows[:, first:min(n, first + 1024)] = _nearest(s["rows_in"][:, first:min(n, first + 1024)].double())
+    else:
+        slots = s["slots"][:n].long()
+        rows[0, :n] = _decoded(s, s["k_pool"], s["k_scales"], slots // B, slots % B, False)
+        rows[1, :n] = _decoded(s, s["v_pool"], s["v_scales"], slots // B, slots % B, True)
+    return {"rows": rows}
