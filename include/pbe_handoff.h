@@ -467,6 +467,63 @@ int pbe_scatter_kv_to_page(const void* keys, const void* values, int32_t in_dtyp
                            uint64_t key_scale_bytes, float* value_scales,
                            uint64_t value_scale_bytes, int device, void* stream);
 
+/* ---- MXFP4 pages ---------------------------------------------------------
+ * A 4-bit KV cache: E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives; the code's top bit is the sign) times a power of two that 32
+ * neighbouring head dims of a token share, an E8M0 byte e (2^(e - 127); 255:
+ * NaN). 4.25 bits a value, where FP8 pages with their scales take 8.25 (128
+ * dims). No counterpart in the reference.
+ *
+ * Pages hold 16 tokens, head_dim is 64 or 128. Block b of a layer has its
+ * codes at key_pool + b*half and value_pool + b*half, half =
+ * 16*kv_heads*head_dim/2 bytes, and its scales at key_scales + b*half/16 and
+ * value_scales + b*half/16. Local pools (ids 0..n-1) and a page-major arena's
+ * layer views (key_pool = arena + 2*layer*half, value_pool = key_pool + half,
+ * the scale arena likewise with half/16, page-major ids) both work, so the
+ * pages of a shared arena are handed over by pbe_runlist_create and
+ * pbe_copy_shared_kv as one-byte elements (elem_bytes 1): the codes with
+ * head_dim/2, the scales with head_dim/32 in place of head_dim.
+ * Within a block each KV head has its own stretch, head h at h*8*head_dim (of
+ * the scales h*head_dim/2), laid out as the reader's lanes take it:
+ *   K codes  [4 quarters of the dims][16 tokens][head_dim/8 bytes]
+ *   V codes  [4 quads of tokens][16 columns of head_dim/16 dims][4 tokens]
+ *            [head_dim/32 bytes]
+ *   scales   [head_dim/32 groups][16 tokens], one byte each, K and V alike
+ * where the even dim of a byte's two lies in its low four bits. */
+#define PBE_KV_MXFP4 2
+
+/* Page writer: n_tokens new tokens' K and V rows, as pbe_scatter_kv takes them
+ * (in_dtype PBE_IN_BF16 or PBE_IN_F32, [n_tokens][kv_heads*head_dim], 16-byte
+ * aligned; slot = block * 16 + offset, int32 in device memory), into MXFP4
+ * pages. A group of 32 dims whose largest magnitude is a gets the scale
+ * 2^(floor(log2 a) - 2), at least 2^-127 (E8M0 byte 0, which an all-zero group
+ * stores too); its codes are the values over the scale rounded to nearest,
+ * ties to the even code, and at most 6 in magnitude. A group that holds an
+ * infinity or a NaN stores scale 255 and reads as NaN. A negative slot, or one
+ * whose block would end beyond the pool or scale sizes given, writes nothing;
+ * a slot that a call names twice ends as a mixture of the two rows. Pools and
+ * scale pools 4-byte aligned. Asynchronous on `stream`; n_tokens = 0 queues
+ * nothing. */
+int pbe_scatter_kv_mxfp4(const void* keys, const void* values, int32_t in_dtype, int32_t n_tokens,
+                         const int32_t* slot_mapping, int32_t kv_heads, int32_t head_dim,
+                         void* key_pool, uint64_t key_pool_bytes, void* value_pool,
+                         uint64_t value_pool_bytes, uint8_t* key_scales, uint64_t key_scale_bytes,
+                         uint8_t* value_scales, uint64_t value_scale_bytes, int device,
+                         void* stream);
+/* The pages read back: the K and V rows of n_tokens slots as BF16
+ * [n_tokens][kv_heads*head_dim] (16-byte aligned), for attention over a cached
+ * prefix that takes rows, or to go on with other pages. BF16 holds the values
+ * exactly (under scale bytes 253 and 254, which the writer does not store,
+ * those of 2^128 and more become infinite). A negative slot leaves its rows as they are; one whose block
+ * would end beyond the pool or scale sizes given reads as NaN. The rest as
+ * pbe_scatter_kv_mxfp4; a slot may be named any number of times. */
+int pbe_gather_kv_mxfp4(const void* key_pool, uint64_t key_pool_bytes, const void* value_pool,
+                        uint64_t value_pool_bytes, const uint8_t* key_scales,
+                        uint64_t key_scale_bytes, const uint8_t* value_scales,
+                        uint64_t value_scale_bytes, const int32_t* slot_mapping, int32_t n_tokens,
+                        int32_t kv_heads, int32_t head_dim, void* keys, void* values, int device,
+                        void* stream);
+
 /* GPU UUID of `device` (16 bytes), as compared across processes. */
 int pbe_device_uuid(int device, uint8_t out[16]);
 /* The calling thread's current HIP device (the one a pool built without an

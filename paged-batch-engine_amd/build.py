@@ -71,12 +71,14 @@ HIP_SOURCES = [
     "csrc/kernels/decode_kernels.hip",
     "csrc/kernels/decode_split_kernels.hip",
     "csrc/kernels/scatter_kernels.hip",
+    "csrc/kernels/mxfp4_kernels.hip",
     "csrc/capi/capi_core.hip",
     "csrc/capi/capi_arena.hip",
     "csrc/capi/capi_plan.hip",
     "csrc/capi/capi_copy.hip",
     "csrc/capi/capi_decode.hip",
     "csrc/capi/capi_scatter.hip",
+    "csrc/capi/capi_mxfp4.hip",
 ]
 CPU_TESTS = ["tests/cpp/test_drop_in_api.cpp"]
 GPU_TESTS = ["tests/cpp/test_gpu_backend.cpp"]

@@ -26,6 +26,7 @@ PBE_FP8_SCALE_PER_TOKEN_HEAD = 0
 PBE_FP8_SCALE_TABLE = 1
 PBE_KV_BF16 = 0
 PBE_KV_FP8_E4M3 = 1
+PBE_KV_MXFP4 = 2
 
 
 class KvShape(C.Structure):
@@ -143,6 +144,12 @@ _SIGNATURES = [
                                          C.c_int32, C.c_int32, C.c_int32, _P, C.c_uint64, _P,
                                          C.c_uint64, _P, C.c_uint64, _P, C.c_uint64, C.c_int,
                                          _P]),
+    ("pbe_scatter_kv_mxfp4", C.c_int, [_P, _P, C.c_int32, C.c_int32, _P, C.c_int32, C.c_int32, _P,
+                                       C.c_uint64, _P, C.c_uint64, _P, C.c_uint64, _P, C.c_uint64,
+                                       C.c_int, _P]),
+    ("pbe_gather_kv_mxfp4", C.c_int, [_P, C.c_uint64, _P, C.c_uint64, _P, C.c_uint64, _P,
+                                      C.c_uint64, _P, C.c_int32, C.c_int32, C.c_int32, _P, _P,
+                                      C.c_int, _P]),
 ]
 EXPORTED = [name for name, _, _ in _SIGNATURES]
 
@@ -599,3 +606,29 @@ def paged_decode(view: ArenaView, kv_dtype: int, scales: int, scale_bytes: int, 
                                  layer, queries, outputs, batch, q_heads, tables, seq_lens,
                                  max_blocks, splits, workspace, workspace_bytes, device,
                                  stream or None))
+
+
+def scatter_kv_mxfp4(keys: int, values: int, in_dtype: int, n_tokens: int, slots: int,
+                     kv_heads: int, head_dim: int, key_pool: int, key_pool_bytes: int,
+                     value_pool: int, value_pool_bytes: int, key_scales: int,
+                     key_scale_bytes: int, value_scales: int, value_scale_bytes: int,
+                     stream: int = 0, device: int = 0) -> None:
+    """New tokens' K/V rows into MXFP4 pages (pbe_scatter_kv_mxfp4)."""
+    check(lib().pbe_scatter_kv_mxfp4(keys or None, values or None, in_dtype, n_tokens,
+                                     slots or None, kv_heads, head_dim, key_pool or None,
+                                     key_pool_bytes, value_pool or None, value_pool_bytes,
+                                     key_scales or None, key_scale_bytes, value_scales or None,
+                                     value_scale_bytes, device, stream or None))
+
+
+def gather_kv_mxfp4(key_pool: int, key_pool_bytes: int, value_pool: int, value_pool_bytes: int,
+                    key_scales: int, key_scale_bytes: int, value_scales: int,
+                    value_scale_bytes: int, slots: int, n_tokens: int, kv_heads: int,
+                    head_dim: int, keys: int, values: int, stream: int = 0,
+                    device: int = 0) -> None:
+    """BF16 K/V rows of slots in MXFP4 pages (pbe_gather_kv_mxfp4)."""
+    check(lib().pbe_gather_kv_mxfp4(key_pool or None, key_pool_bytes, value_pool or None,
+                                    value_pool_bytes, key_scales or None, key_scale_bytes,
+                                    value_scales or None, value_scale_bytes, slots or None,
+                                    n_tokens, kv_heads, head_dim, keys or None, values or None,
+                                    device, stream or None))
