@@ -524,6 +524,39 @@ int pbe_gather_kv_mxfp4(const void* key_pool, uint64_t key_pool_bytes, const voi
                         int32_t kv_heads, int32_t head_dim, void* keys, void* values, int device,
                         void* stream);
 
+/* ---- step tables ----------------------------------------------------------
+ * A decode worker's per-step integers, made on the GPU from its requests' page
+ * lists and lengths in device memory: what KVCacheManager's build_block_tables,
+ * build_seq_lens and build_slot_mapping (kv_cache_manager.cpp:167-244,639-760)
+ * make on the host for one new token a request, here for any number of them, so
+ * a captured step can follow lengths that change on the GPU.
+ *   page_ids: int32 [n_page_ids], the requests' block ids one after another,
+ *     request b's at [page_starts[b], page_starts[b+1]); page_starts int32 [batch+1].
+ *   cached_lens: int32 [batch], tokens already in the pages; new_lens: int32
+ *     [batch], tokens the step adds, or NULL for one each.
+ *   block_tables: int32 [batch][max_blocks_per_seq], a request's pages, then -1.
+ *   seq_lens: int32 [batch], cached + new: what the readers take once the new
+ *     tokens are written.
+ *   token_starts: int32 [batch+1], the first row of each request's new tokens
+ *     and their total (at most INT32_MAX).
+ *   slot_mapping, positions: int32 [max_tokens]: row token_starts[b] + i is
+ *     position cached_lens[b] + i, its slot block * block_size + offset. Rows
+ *     past the total hold -1 in both: the page writers skip them.
+ * A request with a negative length, lengths that add up to more than INT32_MAX,
+ * more tokens than its pages or than max_blocks_per_seq hold, pages outside
+ * page_ids, or rows past max_tokens gets seq_lens -1 (the readers then give
+ * NaN) and -1 in its rows; the others are not affected, a negative count of
+ * new tokens taking no rows. A negative page id, or a slot beyond INT32_MAX,
+ * gives slot -1. batch, max_blocks_per_seq, max_tokens and block_size > 0, and
+ * batch*max_blocks_per_seq at most INT32_MAX. All arrays 4-byte aligned, in
+ * memory of `device`; no output may overlap an input. Asynchronous on
+ * `stream`, one launch, no workspace. */
+int pbe_build_step_tables(const int32_t* page_ids, int64_t n_page_ids, const int32_t* page_starts,
+                          const int32_t* cached_lens, const int32_t* new_lens, int32_t batch,
+                          int32_t block_size, int32_t* block_tables, int32_t max_blocks_per_seq,
+                          int32_t* seq_lens, int32_t* token_starts, int32_t* slot_mapping,
+                          int32_t* positions, int32_t max_tokens, int device, void* stream);
+
 /* GPU UUID of `device` (16 bytes), as compared across processes. */
 int pbe_device_uuid(int device, uint8_t out[16]);
 /* The calling thread's current HIP device (the one a pool built without an

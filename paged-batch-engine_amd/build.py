@@ -72,6 +72,7 @@ HIP_SOURCES = [
     "csrc/kernels/decode_split_kernels.hip",
     "csrc/kernels/scatter_kernels.hip",
     "csrc/kernels/mxfp4_kernels.hip",
+    "csrc/kernels/step_kernels.hip",
     "csrc/capi/capi_core.hip",
     "csrc/capi/capi_arena.hip",
     "csrc/capi/capi_plan.hip",
@@ -79,6 +80,7 @@ HIP_SOURCES = [
     "csrc/capi/capi_decode.hip",
     "csrc/capi/capi_scatter.hip",
     "csrc/capi/capi_mxfp4.hip",
+    "csrc/capi/capi_step.hip",
 ]
 CPU_TESTS = ["tests/cpp/test_drop_in_api.cpp"]
 GPU_TESTS = ["tests/cpp/test_gpu_backend.cpp"]

@@ -150,6 +150,8 @@ _SIGNATURES = [
     ("pbe_gather_kv_mxfp4", C.c_int, [_P, C.c_uint64, _P, C.c_uint64, _P, C.c_uint64, _P,
                                       C.c_uint64, _P, C.c_int32, C.c_int32, C.c_int32, _P, _P,
                                       C.c_int, _P]),
+    ("pbe_build_step_tables", C.c_int, [_P, C.c_int64, _P, _P, _P, C.c_int32, C.c_int32, _P,
+                                        C.c_int32, _P, _P, _P, _P, C.c_int32, C.c_int, _P]),
 ]
 EXPORTED = [name for name, _, _ in _SIGNATURES]
 
@@ -632,3 +634,16 @@ def gather_kv_mxfp4(key_pool: int, key_pool_bytes: int, value_pool: int, value_p
                                     value_scales or None, value_scale_bytes, slots or None,
                                     n_tokens, kv_heads, head_dim, keys or None, values or None,
                                     device, stream or None))
+
+
+def build_step_tables(page_ids: int, n_page_ids: int, page_starts: int, cached_lens: int,
+                      new_lens: int, batch: int, block_size: int, block_tables: int,
+                      max_blocks: int, seq_lens: int, token_starts: int, slots: int,
+                      positions: int, max_tokens: int, stream: int = 0, device: int = 0) -> None:
+    """Block tables, lengths, slots and positions of a step, made on the GPU
+    (pbe_build_step_tables); new_lens 0: one new token each."""
+    check(lib().pbe_build_step_tables(page_ids or None, n_page_ids, page_starts or None,
+                                      cached_lens or None, new_lens or None, batch, block_size,
+                                      block_tables or None, max_blocks, seq_lens or None,
+                                      token_starts or None, slots or None, positions or None,
+                                      max_tokens, device, stream or None))

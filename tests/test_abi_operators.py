@@ -39,3 +39,17 @@ def test_mxfp4_gather_refuses(change, code):
 def test_no_tokens_are_no_work():
     P.scatter_kv_mxfp4(**POOLS, keys=0, values=0, in_dtype=P.PBE_IN_F32, n_tokens=0, slots=0, kv_heads=2, head_dim=64)
     P.gather_kv_mxfp4(**POOLS, keys=0, values=0, n_tokens=0, slots=0, kv_heads=2, head_dim=64)
+
+
+STEP = dict(page_ids=FAKE, n_page_ids=8, page_starts=FAKE + 0x1000, cached_lens=FAKE + 0x2000, new_lens=FAKE + 0x3000, batch=4, block_size=16,
+            block_tables=FAKE + 0x4000, max_blocks=4, seq_lens=FAKE + 0x5000, token_starts=FAKE + 0x6000, slots=FAKE + 0x7000,
+            positions=FAKE + 0x8000, max_tokens=9)
+
+
+@pytest.mark.parametrize("change", [
+    dict(batch=0), dict(batch=-1), dict(block_size=0), dict(max_blocks=0), dict(max_tokens=0), dict(n_page_ids=-1), dict(n_page_ids=1 << 31),
+    dict(batch=1 << 20, max_blocks=1 << 11), dict(page_ids=0), dict(page_starts=0), dict(cached_lens=0), dict(block_tables=0), dict(seq_lens=0),
+    dict(token_starts=0), dict(slots=0), dict(positions=0), dict(slots=FAKE + 0x7002), dict(device=-1),
+    dict(seq_lens=FAKE + 0x2000), dict(positions=FAKE + 0x7000 + 4 * 8), dict(block_tables=FAKE + 4 * 7), dict(token_starts=FAKE + 0x3000 - 16)])
+def test_step_tables_refuse(change):
+    refused(P.build_step_tables, STEP, change, INVALID)

@@ -1,0 +1,17 @@
+"""The step oracle against the host manager's rule and by hand."""
+import numpy as np
+
+from oracle import step as S
+
+
+def test_one_new_token_a_request_by_hand():
+    # request 0: 17 cached tokens in pages 3, 8; request 1: none cached, page 5
+    table, lens, first, slots, pos = S.tables([3, 8, 5], [0, 2, 3], [17, 0], None, 16, 3, 4)
+    assert table.tolist() == [[3, 8, -1], [5, -1, -1]] and lens.tolist() == [18, 1]
+    assert first.tolist() == [0, 1, 2] and slots.tolist() == [8 * 16 + 1, 5 * 16, -1, -1] and pos.tolist() == [17, 0, -1, -1]
+
+
+def test_slots_of_a_chunk_follow_its_pages():
+    table, lens, first, slots, pos = S.tables([6, 2, 9], [0, 3], [14], [20], 16, 3, 20)
+    assert slots.tolist() == [6 * 16 + 14, 6 * 16 + 15] + [2 * 16 + i for i in range(16)] + [9 * 16, 9 * 16 + 1]
+    assert np.array_equal(pos, np.arange(14, 34)) and lens.tolist() == [34]
