@@ -557,6 +557,51 @@ int pbe_build_step_tables(const int32_t* page_ids, int64_t n_page_ids, const int
                           int32_t* seq_lens, int32_t* token_starts, int32_t* slot_mapping,
                           int32_t* positions, int32_t max_tokens, int device, void* stream);
 
+/* ---- page writer with head norms and rotation ------------------------------
+ * What stands between a layer's projections and the decode reader, in one pass:
+ * the RMS norm of each query and key head, the rotation of their positions, the
+ * queries in the reader's form, and K and V in their page slots. No counterpart
+ * in the reference's paged-KV runtime, which is given finished rows.
+ *   q, k, v: [n_tokens] rows of q_heads, kv_heads and kv_heads heads of head_dim
+ *     (64 or 128) in_dtype values (PBE_IN_BF16 or PBE_IN_F32); row t of q begins
+ *     q_stride elements after row t - 1, so parts of one packed row work. 16-byte
+ *     aligned, strides whole multiples of 16 bytes.
+ *   q_weight, k_weight: [head_dim] of in_dtype, 16-byte aligned, or NULL for no
+ *     norm of those heads: x <- x / sqrt(mean(x^2) + eps) * weight.
+ *   positions: int32 [n_tokens]; a negative one marks a padding token, whose
+ *     q_out row stays as it is and which writes no page. NULL (rotary_dim 0
+ *     only): none is padding.
+ *   cos_sin: fp32 [max_position][rotary_dim], a position's rotary_dim/2 cosines,
+ *     then its sines; 16-byte aligned. The first rotary_dim dims of a head turn
+ *     (a multiple of 16 up to head_dim; 0: none, cos_sin may be NULL): dims i
+ *     and i + rotary_dim/2 together (PBE_ROPE_HALVES), or 2i and 2i + 1
+ *     (PBE_ROPE_PAIRS). A position at or beyond max_position gives NaN in its
+ *     q_out row and writes no page.
+ *   slot_mapping: int32 [n_tokens], block * block_size + offset; a negative
+ *     slot, or one that is not wholly inside every pool and scale pool given,
+ *     writes no page (its q_out row is written).
+ *   kv_dtype: PBE_KV_BF16 or PBE_KV_FP8_E4M3 pages as pbe_scatter_kv lays them
+ *     out (scales fp32), or PBE_KV_MXFP4 pages (block_size 16, scales bytes).
+ *   q_out: bf16 [n_tokens][q_heads][head_dim], 16-byte aligned, apart from the
+ *     inputs.
+ * Arithmetic is FP32, rounded once, to BF16; FP8 and MXFP4 pages hold what
+ * pbe_scatter_kv and pbe_scatter_kv_mxfp4 make of those BF16 rows, byte for
+ * byte. Pools aligned to 16 bytes (BF16), 8 (FP8) or 4 (MXFP4), scale pools to
+ * 4. A slot that a call names twice ends as a mixture. Asynchronous on
+ * `stream`; n_tokens = 0 queues nothing. */
+#define PBE_ROPE_HALVES 0
+#define PBE_ROPE_PAIRS 1
+int pbe_qk_norm_rope_scatter(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                             const void* v, int64_t v_stride, int32_t in_dtype, int32_t n_tokens,
+                             int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                             const void* q_weight, const void* k_weight, float eps,
+                             const int32_t* positions, const float* cos_sin, int32_t max_position,
+                             int32_t rotary_dim, int32_t rope_style, const int32_t* slot_mapping,
+                             int32_t block_size, int32_t kv_dtype, void* q_out, void* key_pool,
+                             uint64_t key_pool_bytes, void* value_pool, uint64_t value_pool_bytes,
+                             void* key_scales, uint64_t key_scale_bytes, void* value_scales,
+                             uint64_t value_scale_bytes, int device, void* stream);
+
 /* GPU UUID of `device` (16 bytes), as compared across processes. */
 int pbe_device_uuid(int device, uint8_t out[16]);
 /* The calling thread's current HIP device (the one a pool built without an

@@ -34,3 +34,20 @@ def tables(pages, starts, cached, new, block_size, max_blocks, max_tokens):
         at += rows
     first[batch] = min(at, INT32_MAX)
     return tuple(x.astype(np.int32) for x in (table, lens, first, slots, positions))
+
+
+def norm_rope(x, weight, eps, line, rotary, pairs):
+    """Heads x[heads][dim] of one token, normed (weight None: not) and turned by
+    line[rotary] (cosines, then sines); and the sum of the magnitudes that went
+    into each result, for error bounds."""
+    x = np.asarray(x, np.float64)
+    if weight is not None:
+        x = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * np.asarray(weight, np.float64)
+    out, size = x.copy(), np.abs(x)
+    n = rotary // 2
+    for i in range(n):
+        a, b = (2 * i, 2 * i + 1) if pairs else (i, i + n)
+        c, s = float(line[i]), float(line[n + i])
+        out[..., a], out[..., b] = x[..., a] * c - x[..., b] * s, x[..., b] * c + x[..., a] * s
+        size[..., a], size[..., b] = abs(x[..., a] * c) + abs(x[..., b] * s), abs(x[..., b] * c) + abs(x[..., a] * s)
+    return out, size

@@ -73,6 +73,7 @@ HIP_SOURCES = [
     "csrc/kernels/scatter_kernels.hip",
     "csrc/kernels/mxfp4_kernels.hip",
     "csrc/kernels/step_kernels.hip",
+    "csrc/kernels/rope_kernels.hip",
     "csrc/capi/capi_core.hip",
     "csrc/capi/capi_arena.hip",
     "csrc/capi/capi_plan.hip",

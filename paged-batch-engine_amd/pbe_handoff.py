@@ -152,6 +152,12 @@ _SIGNATURES = [
                                       C.c_int, _P]),
     ("pbe_build_step_tables", C.c_int, [_P, C.c_int64, _P, _P, _P, C.c_int32, C.c_int32, _P,
                                         C.c_int32, _P, _P, _P, _P, C.c_int32, C.c_int, _P]),
+    ("pbe_qk_norm_rope_scatter", C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_int32,
+                                           C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P,
+                                           C.c_float, _P, _P, C.c_int32, C.c_int32, C.c_int32, _P,
+                                           C.c_int32, C.c_int32, _P, _P, C.c_uint64, _P,
+                                           C.c_uint64, _P, C.c_uint64, _P, C.c_uint64, C.c_int,
+                                           _P]),
 ]
 EXPORTED = [name for name, _, _ in _SIGNATURES]
 
@@ -647,3 +653,29 @@ def build_step_tables(page_ids: int, n_page_ids: int, page_starts: int, cached_l
                                       block_tables or None, max_blocks, seq_lens or None,
                                       token_starts or None, slots or None, positions or None,
                                       max_tokens, device, stream or None))
+
+
+PBE_ROPE_HALVES = 0
+PBE_ROPE_PAIRS = 1
+
+
+def qk_norm_rope_scatter(q: int, q_stride: int, k: int, k_stride: int, v: int, v_stride: int,
+                         in_dtype: int, n_tokens: int, q_heads: int, kv_heads: int,
+                         head_dim: int, q_weight: int, k_weight: int, eps: float, positions: int,
+                         cos_sin: int, max_position: int, rotary_dim: int, rope_style: int,
+                         slots: int, block_size: int, kv_dtype: int, q_out: int, key_pool: int,
+                         key_pool_bytes: int, value_pool: int, value_pool_bytes: int,
+                         key_scales: int = 0, key_scale_bytes: int = 0, value_scales: int = 0,
+                         value_scale_bytes: int = 0, stream: int = 0, device: int = 0) -> None:
+    """Head norms, rotation, the reader's queries and K/V in their page slots in
+    one pass (pbe_qk_norm_rope_scatter); strides in elements."""
+    check(lib().pbe_qk_norm_rope_scatter(q or None, q_stride, k or None, k_stride, v or None,
+                                         v_stride, in_dtype, n_tokens, q_heads, kv_heads,
+                                         head_dim, q_weight or None, k_weight or None, eps,
+                                         positions or None, cos_sin or None, max_position,
+                                         rotary_dim, rope_style, slots or None, block_size,
+                                         kv_dtype, q_out or None, key_pool or None,
+                                         key_pool_bytes, value_pool or None, value_pool_bytes,
+                                         key_scales or None, key_scale_bytes,
+                                         value_scales or None, value_scale_bytes, device,
+                                         stream or None))

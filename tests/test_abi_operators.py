@@ -53,3 +53,31 @@ STEP = dict(page_ids=FAKE, n_page_ids=8, page_starts=FAKE + 0x1000, cached_lens=
     dict(seq_lens=FAKE + 0x2000), dict(positions=FAKE + 0x7000 + 4 * 8), dict(block_tables=FAKE + 4 * 7), dict(token_starts=FAKE + 0x3000 - 16)])
 def test_step_tables_refuse(change):
     refused(P.build_step_tables, STEP, change, INVALID)
+
+
+ROPE = dict(q=FAKE, q_stride=256, k=FAKE + 512, k_stride=256, v=FAKE + 768, v_stride=256, in_dtype=P.PBE_IN_BF16, n_tokens=4, q_heads=2, kv_heads=1,
+            head_dim=64, q_weight=FAKE, k_weight=FAKE, eps=1e-6, positions=FAKE, cos_sin=FAKE, max_position=64, rotary_dim=64,
+            rope_style=P.PBE_ROPE_HALVES, slots=FAKE, block_size=16, kv_dtype=P.PBE_KV_BF16, q_out=FAKE + (1 << 20), key_pool=FAKE,
+            key_pool_bytes=1 << 20, value_pool=FAKE, value_pool_bytes=1 << 20)
+SCALES = dict(key_scales=FAKE, key_scale_bytes=1 << 16, value_scales=FAKE, value_scale_bytes=1 << 16)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(in_dtype=2), INVALID), (dict(kv_dtype=3), INVALID), (dict(rope_style=2), INVALID), (dict(n_tokens=-1), INVALID), (dict(q_heads=0), INVALID),
+    (dict(kv_heads=0), INVALID), (dict(block_size=0), INVALID), (dict(head_dim=96), UNSUPPORTED), (dict(head_dim=256), UNSUPPORTED),
+    (dict(kv_dtype=P.PBE_KV_MXFP4, block_size=32, **SCALES), UNSUPPORTED), (dict(rotary_dim=24), INVALID), (dict(rotary_dim=80), INVALID),
+    (dict(rotary_dim=-16), INVALID), (dict(max_position=0), INVALID), (dict(eps=-1.0), INVALID), (dict(eps=float("nan")), INVALID),
+    (dict(eps=float("inf")), INVALID), (dict(n_tokens=2 ** 31 - 1), INVALID), (dict(q_heads=2 ** 31 - 1), INVALID), (dict(q=0), INVALID),
+    (dict(k=0), INVALID), (dict(v=0), INVALID), (dict(slots=0), INVALID), (dict(q_out=0), INVALID), (dict(key_pool=0), INVALID),
+    (dict(value_pool=0), INVALID), (dict(positions=0), INVALID), (dict(cos_sin=0), INVALID), (dict(kv_dtype=P.PBE_KV_FP8_E4M3), INVALID),
+    (dict(kv_dtype=P.PBE_KV_MXFP4), INVALID), (dict(q_stride=120), INVALID), (dict(k_stride=8), INVALID), (dict(v_stride=65), INVALID),
+    (dict(q_stride=-256), INVALID), (dict(q_stride=1 << 62), INVALID), (dict(q=FAKE + 8), INVALID), (dict(q_weight=FAKE + 4), INVALID),
+    (dict(cos_sin=FAKE + 4), INVALID), (dict(q_out=FAKE + (1 << 20) + 8), INVALID), (dict(positions=FAKE + 2), INVALID),
+    (dict(key_pool=FAKE + 8), INVALID), (dict(SCALES, kv_dtype=P.PBE_KV_FP8_E4M3, value_pool=FAKE + 4), INVALID),
+    (dict(SCALES, kv_dtype=P.PBE_KV_MXFP4, key_pool=FAKE + 2), INVALID), (dict(q_out=FAKE + 1024), INVALID), (dict(device=-1), INVALID)])
+def test_rope_writer_refuses(change, code):
+    refused(P.qk_norm_rope_scatter, ROPE, change, code)
+
+
+def test_rope_writer_without_tokens_is_no_work():
+    P.qk_norm_rope_scatter(**{**ROPE, "n_tokens": 0, "q": 0, "k": 0, "v": 0, "slots": 0, "q_out": 0})
