@@ -524,6 +524,40 @@ int pbe_gather_kv_mxfp4(const void* key_pool, uint64_t key_pool_bytes, const voi
                         int32_t kv_heads, int32_t head_dim, void* keys, void* values, int device,
                         void* stream);
 
+/* Decode reader: paged attention for one query token per sequence over MXFP4
+ * pages, as pbe_paged_decode_pools reads BF16 and FP8 ones: softmax(q . k /
+ * sqrt(head_dim)) v, FP32 sums and softmax, probabilities rounded to BF16 for
+ * the product with v and summed as rounded, BF16 outputs. pool_bytes and
+ * scale_pool_bytes are the bytes addressable from each pointer; q_heads a
+ * multiple of kv_heads, at most 16 query heads per KV head.
+ *
+ * queries / outputs: bf16 [batch][q_heads][head_dim], 16-byte aligned; pools
+ * 16-byte, scale pools 4-byte aligned. block_tables: int32
+ * [batch][max_blocks_per_seq]; seq_lens: int32 [batch] (device memory). What
+ * lies behind a sequence's last token, in its page or in its table, is not
+ * used. A length of 0 gives zeros; a negative one, one that needs more than
+ * max_blocks_per_seq blocks, and a block id outside the pools give the
+ * sequence NaN; a NaN group in a token's K or V reaches the heads that read
+ * it, as does one in the queries.
+ * A sequence is read in up to `splits` pieces (1..1024) whose partial results
+ * lie in `workspace`: pbe_paged_decode_mxfp4_workspace_bytes() bytes, 16-byte
+ * aligned, used until the call completes and holding anything when it starts;
+ * none is needed, and NULL taken, for one split. The pieces of a sequence
+ * depend on its length, max_blocks_per_seq and splits alone, so the same
+ * sequence gives the same bits in any batch with these. splits = 0 takes
+ * pbe_paged_decode_mxfp4_splits(), lowered until the workspace holds them.
+ * Asynchronous on `stream`. */
+int32_t pbe_paged_decode_mxfp4_splits(int32_t batch, int32_t kv_heads, int32_t max_blocks_per_seq);
+uint64_t pbe_paged_decode_mxfp4_workspace_bytes(int32_t batch, int32_t q_heads, int32_t head_dim,
+                                                int32_t splits);
+int pbe_paged_decode_mxfp4(const void* key_pool, const void* value_pool, uint64_t pool_bytes,
+                           const uint8_t* key_scales, const uint8_t* value_scales,
+                           uint64_t scale_pool_bytes, int32_t kv_heads, int32_t head_dim,
+                           const void* queries, void* outputs, int32_t batch, int32_t q_heads,
+                           const int32_t* block_tables, const int32_t* seq_lens,
+                           int32_t max_blocks_per_seq, int32_t splits, void* workspace,
+                           uint64_t workspace_bytes, int device, void* stream);
+
 /* ---- step tables ----------------------------------------------------------
  * A decode worker's per-step integers, made on the GPU from its requests' page
  * lists and lengths in device memory: what KVCacheManager's build_block_tables,

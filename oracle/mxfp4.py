@@ -84,11 +84,15 @@ def get(pool, scales, slots, heads, dim, is_value):
 
 
 def decode(q, pools, tables, seq_lens, heads):
-    """Attention of one query token per sequence in 64 bits. q [batch][q_heads][dim];
+    """Attention of one query token per sequence in 64 bits: (out, spread, size,
+    reach), each [batch][q_heads][dim] (reach without dim). spread = sum w |v -
+    out| and size = sum w |v| with w the softmax weights, reach the largest sum
+    |q k| / sqrt(dim): what error bounds are made of. q [batch][q_heads][dim];
     pools (k, v, k_scales, v_scales). A zero length gives zeros."""
     batch, q_heads, dim = q.shape
     group = q_heads // heads
-    out = np.zeros((batch, q_heads, dim))
+    out, spread, size = (np.zeros((batch, q_heads, dim)) for _ in range(3))
+    reach = np.zeros((batch, q_heads))
     k_pool, v_pool, k_scales, v_scales = pools
     for b in range(batch):
         n = int(seq_lens[b])
@@ -99,7 +103,12 @@ def decode(q, pools, tables, seq_lens, heads):
         k = get(k_pool, k_scales, slots, heads, dim, False)
         v = get(v_pool, v_scales, slots, heads, dim, True)
         for h in range(q_heads):
-            s = k[:, h // group] @ q[b, h].astype(np.float64) / np.sqrt(dim)
+            qh, kh, vh = q[b, h].astype(np.float64), k[:, h // group], v[:, h // group]
+            s = kh @ qh / np.sqrt(dim)
             p = np.exp(s - s.max())
-            out[b, h] = p @ v[:, h // group] / p.sum()
-    return out
+            w = p / p.sum()
+            out[b, h] = w @ vh
+            spread[b, h] = w @ np.abs(vh - out[b, h])
+            size[b, h] = w @ np.abs(vh)
+            reach[b, h] = (np.abs(kh) @ np.abs(qh)).max() / np.sqrt(dim)
+    return out, spread, size, reach

@@ -72,6 +72,7 @@ HIP_SOURCES = [
     "csrc/kernels/decode_split_kernels.hip",
     "csrc/kernels/scatter_kernels.hip",
     "csrc/kernels/mxfp4_kernels.hip",
+    "csrc/kernels/decode_mxfp4_kernels.hip",
     "csrc/kernels/step_kernels.hip",
     "csrc/kernels/rope_kernels.hip",
     "csrc/capi/capi_core.hip",

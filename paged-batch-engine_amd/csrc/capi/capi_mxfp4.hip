@@ -1,10 +1,13 @@
-// C ABI: MXFP4 pages (their writer and the gather that reads rows back).
+// C ABI: MXFP4 pages (their writer, the gather that reads rows back and the
+// decode reader).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <vector>
 
 #include "capi_internal.h"
+#include "../kernels/decode_mxfp4_kernels.h"
 #include "../kernels/mxfp4_kernels.h"
 
 using namespace pbe_capi;
@@ -109,6 +112,85 @@ int pbe_gather_kv_mxfp4(const void* key_pool, uint64_t key_pool_bytes, const voi
   p.values_out = static_cast<uint8_t*>(values);
   PBE_DEVICE_SCOPE(device);
   PBE_HIP(pbe::launch_gather_kv_mxfp4(p, head_dim, static_cast<hipStream_t>(stream)));
+  return PBE_OK;
+}
+
+int32_t pbe_paged_decode_mxfp4_splits(int32_t batch, int32_t kv_heads, int32_t max_blocks_per_seq) {
+  if (batch <= 0 || kv_heads <= 0 || max_blocks_per_seq <= 0) return 1;
+  return pbe::mxfp4_decode_splits(batch, kv_heads, max_blocks_per_seq, compute_units());
+}
+
+uint64_t pbe_paged_decode_mxfp4_workspace_bytes(int32_t batch, int32_t q_heads, int32_t head_dim,
+                                                int32_t splits) {
+  if (batch <= 0 || q_heads <= 0 || head_dim <= 0 || splits <= 0) return 0;
+  return pbe::mxfp4_decode_workspace_bytes(batch, q_heads, head_dim, splits);
+}
+
+int pbe_paged_decode_mxfp4(const void* key_pool, const void* value_pool, uint64_t pool_bytes,
+                           const uint8_t* key_scales, const uint8_t* value_scales,
+                           uint64_t scale_pool_bytes, int32_t kv_heads, int32_t head_dim,
+                           const void* queries, void* outputs, int32_t batch, int32_t q_heads,
+                           const int32_t* block_tables, const int32_t* seq_lens,
+                           int32_t max_blocks_per_seq, int32_t splits, void* workspace,
+                           uint64_t workspace_bytes, int device, void* stream) {
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || max_blocks_per_seq <= 0 || device < 0)
+    return fail(PBE_ERR_INVALID, "batch, q_heads, kv_heads, max_blocks_per_seq > 0 and a device");
+  if (head_dim != 64 && head_dim != 128) return fail(PBE_ERR_UNSUPPORTED, "MXFP4 pages hold heads of 64 or 128 dims");
+  if (q_heads % kv_heads != 0 || q_heads / kv_heads > pbe::kMxDecodeMaxGroup)
+    return fail(PBE_ERR_UNSUPPORTED, "q_heads must be 1..%d times kv_heads", pbe::kMxDecodeMaxGroup);
+  if (!key_pool || !value_pool || !key_scales || !value_scales || !queries || !outputs || !block_tables || !seq_lens)
+    return fail(PBE_ERR_INVALID, "null decode operand");
+  auto at = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr); };
+  if ((at(queries) | at(outputs) | at(key_pool) | at(value_pool) | at(workspace)) % 16 || (at(key_scales) | at(value_scales)) % 4 ||
+      (at(block_tables) | at(seq_lens)) % 4)
+    return fail(PBE_ERR_INVALID, "queries, outputs, pools and workspace must be 16-byte aligned, scale pools and tables 4-byte aligned");
+  if (splits < 0 || splits > pbe::kMxDecodeMaxSplits) return fail(PBE_ERR_INVALID, "splits must be 0..%d", pbe::kMxDecodeMaxSplits);
+  // so that no product below passes 64 bits
+  if ((int64_t)batch * q_heads > INT32_MAX || (int64_t)batch * max_blocks_per_seq > (1ll << 40))
+    return fail(PBE_ERR_INVALID, "batch * q_heads must be at most INT32_MAX and batch * max_blocks_per_seq at most 2^40");
+  const uint64_t half = kTokens * (uint64_t)kv_heads * (uint64_t)head_dim / 2;
+  if (half > 0xffffffffull) return fail(PBE_ERR_INVALID, "a block of one plane must be smaller than 4 GiB");
+  if (pool_bytes < half || scale_pool_bytes < half / 16) return fail(PBE_ERR_INVALID, "pools and scale pools must hold at least one block");
+  if (splits == 0) {
+    splits = pbe_paged_decode_mxfp4_splits(batch, kv_heads, max_blocks_per_seq);
+    const uint64_t each = (uint64_t)batch * (uint64_t)q_heads * (uint64_t)(head_dim + 2) * 4;  // bytes of one split
+    splits = (int32_t)std::max<uint64_t>(1, std::min<uint64_t>((uint64_t)splits, workspace ? workspace_bytes / each : 1));
+  }
+  const uint64_t need = pbe::mxfp4_decode_workspace_bytes(batch, q_heads, head_dim, splits);
+  if (need && !workspace) return fail(PBE_ERR_INVALID, "more than one split needs a workspace");
+  if (workspace_bytes < need)
+    return fail(PBE_ERR_INVALID, "decode workspace holds %llu of %llu bytes", (unsigned long long)workspace_bytes, (unsigned long long)need);
+  {
+    PBE_DEVICE_SCOPE(device);
+    std::vector<Range> known;
+    auto ok = [&](const void* ptr, uint64_t bytes) { return bytes == 0 || accessible(ptr, bytes, device, &known); };
+    const uint64_t rows = (uint64_t)batch * (uint64_t)q_heads * (uint64_t)head_dim * 2;
+    if (!ok(key_pool, pool_bytes) || !ok(value_pool, pool_bytes) || !ok(key_scales, scale_pool_bytes) || !ok(value_scales, scale_pool_bytes) ||
+        !ok(queries, rows) || !ok(outputs, rows) || !ok(block_tables, (uint64_t)batch * (uint64_t)max_blocks_per_seq * 4) ||
+        !ok(seq_lens, (uint64_t)batch * 4) || !ok(workspace, need))
+      return fail(PBE_ERR_INVALID, "decode operands must be memory of device %d", device);
+  }
+  pbe::Mxfp4DecodeParams p{};
+  p.key_pool = static_cast<const uint8_t*>(key_pool);
+  p.value_pool = static_cast<const uint8_t*>(value_pool);
+  p.key_scales = key_scales;
+  p.value_scales = value_scales;
+  p.q = static_cast<const uint16_t*>(queries);
+  p.out = static_cast<uint16_t*>(outputs);
+  p.tables = block_tables;
+  p.seq_lens = seq_lens;
+  p.half = (uint32_t)half;
+  p.batch = batch;
+  p.q_heads = q_heads;
+  p.kv_heads = kv_heads;
+  p.group = q_heads / kv_heads;
+  p.max_blocks = max_blocks_per_seq;
+  p.blocks = (int32_t)std::min<uint64_t>(std::min(pool_bytes / half, scale_pool_bytes / (half / 16)), INT32_MAX);
+  p.splits = splits;
+  p.scale = (1.f / std::sqrt((float)head_dim)) * 1.4426950408889634f;
+  pbe::plan_mxfp4_decode(&p, head_dim, workspace);
+  PBE_DEVICE_SCOPE(device);
+  PBE_HIP(pbe::launch_paged_decode_mxfp4(p, head_dim, static_cast<hipStream_t>(stream)));
   return PBE_OK;
 }
 

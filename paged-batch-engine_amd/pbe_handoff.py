@@ -150,6 +150,12 @@ _SIGNATURES = [
     ("pbe_gather_kv_mxfp4", C.c_int, [_P, C.c_uint64, _P, C.c_uint64, _P, C.c_uint64, _P,
                                       C.c_uint64, _P, C.c_int32, C.c_int32, C.c_int32, _P, _P,
                                       C.c_int, _P]),
+    ("pbe_paged_decode_mxfp4_splits", C.c_int32, [C.c_int32, C.c_int32, C.c_int32]),
+    ("pbe_paged_decode_mxfp4_workspace_bytes", C.c_uint64, [C.c_int32, C.c_int32, C.c_int32,
+                                                            C.c_int32]),
+    ("pbe_paged_decode_mxfp4", C.c_int, [_P, _P, C.c_uint64, _P, _P, C.c_uint64, C.c_int32,
+                                         C.c_int32, _P, _P, C.c_int32, C.c_int32, _P, _P,
+                                         C.c_int32, C.c_int32, _P, C.c_uint64, C.c_int, _P]),
     ("pbe_build_step_tables", C.c_int, [_P, C.c_int64, _P, _P, _P, C.c_int32, C.c_int32, _P,
                                         C.c_int32, _P, _P, _P, _P, C.c_int32, C.c_int, _P]),
     ("pbe_qk_norm_rope_scatter", C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_int32,
@@ -640,6 +646,28 @@ def gather_kv_mxfp4(key_pool: int, key_pool_bytes: int, value_pool: int, value_p
                                     value_scales or None, value_scale_bytes, slots or None,
                                     n_tokens, kv_heads, head_dim, keys or None, values or None,
                                     device, stream or None))
+
+
+def decode_mxfp4_splits(batch: int, kv_heads: int, max_blocks: int) -> int:
+    return int(lib().pbe_paged_decode_mxfp4_splits(batch, kv_heads, max_blocks))
+
+
+def decode_mxfp4_workspace_bytes(batch: int, q_heads: int, head_dim: int, splits: int) -> int:
+    return int(lib().pbe_paged_decode_mxfp4_workspace_bytes(batch, q_heads, head_dim, splits))
+
+
+def paged_decode_mxfp4(key_pool: int, value_pool: int, pool_bytes: int, key_scales: int,
+                       value_scales: int, scale_pool_bytes: int, kv_heads: int, head_dim: int,
+                       queries: int, outputs: int, batch: int, q_heads: int, tables: int,
+                       seq_lens: int, max_blocks: int, splits: int, workspace: int,
+                       workspace_bytes: int, stream: int = 0, device: int = 0) -> None:
+    """Decode attention over MXFP4 pages (pbe_paged_decode_mxfp4)."""
+    check(lib().pbe_paged_decode_mxfp4(key_pool or None, value_pool or None, pool_bytes,
+                                       key_scales or None, value_scales or None,
+                                       scale_pool_bytes, kv_heads, head_dim, queries or None,
+                                       outputs or None, batch, q_heads, tables or None,
+                                       seq_lens or None, max_blocks, splits, workspace or None,
+                                       workspace_bytes, device, stream or None))
 
 
 def build_step_tables(page_ids: int, n_page_ids: int, page_starts: int, cached_lens: int,

@@ -63,3 +63,18 @@ def test_rows_come_back_as_they_were_put():
         scales = rng.integers(0, 256, len(pool) // 16).astype(np.uint8)
         M.put(pool, scales, slots, codes, sc, is_value)
         assert np.array_equal(M.get(pool, scales, slots, heads, dim, is_value), M.values(codes, sc))
+
+
+def test_attention_of_equal_scores_is_the_mean_and_of_one_token_its_value():
+    rng = np.random.default_rng(5)
+    heads, dim, blocks = 2, 64, 3
+    pools = [rng.integers(0, 256, blocks * M.half_bytes(heads, dim) // d).astype(np.uint8) for d in (1, 1, 16, 16)]
+    for s in pools[2:]:
+        s[:] = rng.integers(120, 130, len(s))
+    q = np.zeros((2, 4, dim))
+    out, spread, size, reach = M.decode(q, pools, [[2, 0], [1, 1]], [20, 1], heads)
+    v = M.get(pools[1], pools[3], np.r_[32:48, 0:4], heads, dim, True)
+    np.testing.assert_allclose(out[0], np.repeat(v.mean(0), 2, 0), rtol=1e-12, atol=1e-12)
+    one = M.get(pools[1], pools[3], [16], heads, dim, True)[0]
+    np.testing.assert_array_equal(out[1], np.repeat(one, 2, 0))
+    assert (spread[1] == 0).all() and (reach == 0).all() and np.array_equal(size[1], np.abs(out[1]))
