@@ -359,6 +359,8 @@ def _plain_read(s):
 
 # ------------------------------------------------------------------ the calls
 def _package():
+    if "pbe_handoff" in sys.modules:  # imported once, not looked for in every pass
+        return sys.modules["pbe_handoff"]
     path = str(Path(__file__).resolve().parent.parent / "paged-batch-engine_amd")
     if path not in sys.path:
         sys.path.insert(0, path)
@@ -394,9 +396,11 @@ def _own_rows(s):
     pools = (s["k_pool"].data_ptr(), half, s["v_pool"].data_ptr(), half, s["k_scales"].data_ptr(), half // 16, s["v_scales"].data_ptr(), half // 16)
     if "rows_in" in s:
         rows = s["rows_in"]
-        P.scatter_kv_mxfp4(rows[0].data_ptr(), rows[1].data_ptr(), P.PBE_IN_F32 if rows.dtype == torch.float32 else P.PBE_IN_BF16, n,
+        at = rows.data_ptr()
+        P.scatter_kv_mxfp4(at, at + n * heads * dim * rows.element_size(), P.PBE_IN_F32 if rows.dtype == torch.float32 else P.PBE_IN_BF16, n,
                            s["slots"].data_ptr(), heads, dim, *pools, stream=stream)
-    P.gather_kv_mxfp4(*pools, s["slots"].data_ptr(), n, heads, dim, s["rows_out"][0].data_ptr(), s["rows_out"][1].data_ptr(), stream=stream)
+    out = s["rows_out"].data_ptr()
+    P.gather_kv_mxfp4(*pools, s["slots"].data_ptr(), n, heads, dim, out, out + n * heads * dim * 2, stream=stream)
 
 
 def _own_read(s):
