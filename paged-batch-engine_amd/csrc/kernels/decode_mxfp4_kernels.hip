@@ -5,17 +5,26 @@
 // A workgroup of four waves reads one piece of a sequence for one KV head, its
 // waves tiles of four blocks (64 tokens) in turn.
 //  - loads: a block's codes of one head lie in the order of the lanes that
-//    take them, so one load instruction reads all of K, and one all of V.
-//  - scores, transposed: A = the block's 16 keys, B = the query heads of the KV
-//    head (columns, padded to 16), one v_mfma_f32_16x16x32_bf16 per 32 dims.
-//    Lane (g, j) holds quarter g of key j's dims, an eighth of them an MFMA, and
-//    ends with tokens 4g..4g+3 of query head j. The scaled converters make two
-//    BF16 values of a byte and its scale, exactly.
+//    take them, so one load instruction reads all of K, and one all of V. The
+//    next tile's K is asked for when the scores have used this one's, its V
+//    after the values' products.
+//  - scores, transposed, on the codes as they are: one scaled 16x16x128 MFMA
+//    takes a block's 16 keys (A, E2M1 with the pages' own E8M0 scales) and the
+//    query heads of the KV head (B, E4M3, columns). A query is split into two
+//    E4M3 numbers of four significant bits, which hold a BF16 number's eight
+//    exactly down to 2^-13 of the head's largest, and to 2^-21 of that below;
+//    the second pair of MFMA operands adds the lower parts. The MFMA sums a
+//    group's products to about 2^-17 of their magnitudes (measured), which is
+//    what a score is good for. Lane (g, j) ends with tokens 4g..4g+3 of head j.
 //  - values: lane (g, i) holds tokens 4g..4g+3 of column i, the D/16 dims
-//    [i*D/16, (i+1)*D/16): two blocks give the eight tokens of the A operand
-//    of O^T += V^T P^T (row i of MFMA n is dim i*D/16 + n), which are the eight
-//    tokens whose probabilities the lane holds as the B operand. Only pairs of
-//    tokens have to be put side by side, so values pass no LDS.
+//    [i*D/16, (i+1)*D/16). The scaled converters make a BF16 pair of a byte, an
+//    even and an odd dim of one token, exactly. Both count as terms of one
+//    contraction: A row i, of MFMA n, holds dims 2n and 2n + 1 of column i for
+//    four tokens a lane, B the probability against the even dims in the
+//    columns of heads 0..7 and against the odd ones in columns 8..15 (which
+//    carry the same heads again), zero elsewhere. So no two tokens have to be
+//    put side by side and no column of B is idle. More than 8 query heads take
+//    two such products, of the even and of the odd dims.
 //  - probabilities are rounded to BF16 for that product, and the sum they are
 //    divided by is of the rounded ones: each weight is off by at most 2^-8 of
 //    itself, and they still add up to one.
@@ -23,6 +32,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "decode_device.h"
 #include "decode_mxfp4_kernels.h"
@@ -33,6 +43,8 @@ namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kTile = 4;  // blocks of a wave's tile
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // A lane's part of one tile.
 template <int D>
@@ -48,7 +60,7 @@ __device__ __forceinline__ float token_scale(uint32_t bytes) {  // the converter
   return __uint_as_float(kToken == 3 ? bytes >> 1 : bytes << (23 - 8 * kToken));
 }
 
-// Tokens kT of column i as BF16 pairs of dims: c[m] holds dims 2m and 2m + 1.
+// Token kT's part of column i as BF16 pairs: c[n] holds dims 2n and 2n + 1.
 template <int D, int kT>
 __device__ __forceinline__ void token_pairs(const uint32_t (&v)[D / 32], uint32_t scales, uint32_t (&c)[D / 32]) {
   const float s = token_scale<kT>(scales);
@@ -63,13 +75,49 @@ __device__ __forceinline__ void token_pairs(const uint32_t (&v)[D / 32], uint32_
   }
 }
 
-template <int D>
-__global__ __launch_bounds__(kThreads, 2) void paged_decode_mxfp4_kernel(const Mxfp4DecodeParams p) {
-  constexpr int W = D / 32;   // words of K (and of V) codes per lane and block
-  constexpr int NK = D / 32;  // score MFMAs per block
-  constexpr int NT = D / 16;  // value MFMAs per two blocks
+// A query head's 32 dims of this lane, BF16 pairs x, as E4M3 numbers hi + lo:
+// value = hi * 2^(hi_byte - 127) + lo * 2^(lo_byte - 127). `amax`: FP32 bits of
+// the head's largest magnitude, which hi takes to [2^7, 2^8); an infinity or a
+// NaN gives byte 255, the NaN scale.
+struct SplitQuery {
+  i32x8 hi, lo;
+  int hi_byte, lo_byte;
+};
+__device__ __forceinline__ SplitQuery split_query(const u32x4 (&x)[4], uint32_t amax) {
+  SplitQuery q;
+  const int e = (int)(amax >> 23);
+  const int byte = max(e - 7, 4);  // both parts' scales stay within a byte
+  q.hi_byte = e == 255 ? 255 : byte;
+  q.lo_byte = byte - 4;
+  // x * 2^(127 - byte) in two steps, either of them within FP32's exponents
+  const int down = 127 - byte, half = down / 2;
+  const float s0 = __uint_as_float((uint32_t)(half + 127) << 23), s1 = __uint_as_float((uint32_t)(down - half + 127) << 23);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const uint32_t a = x[w / 2][2 * (w % 2)], b = x[w / 2][2 * (w % 2) + 1];
+    const float v[4] = {bf16_lo(a) * s0 * s1, bf16_hi(a) * s0 * s1, bf16_lo(b) * s0 * s1, bf16_hi(b) * s0 * s1};
+    uint32_t hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], hi, true);
+    const float r[4] = {(v[0] - __builtin_amdgcn_cvt_f32_fp8(hi, 0)) * 16.f, (v[1] - __builtin_amdgcn_cvt_f32_fp8(hi, 1)) * 16.f,
+                        (v[2] - __builtin_amdgcn_cvt_f32_fp8(hi, 2)) * 16.f, (v[3] - __builtin_amdgcn_cvt_f32_fp8(hi, 3)) * 16.f};
+    uint32_t lo = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], lo, true);
+    q.hi[w] = (int)(e == 255 ? 0u : hi);
+    q.lo[w] = (int)(e == 255 ? 0u : lo);
+  }
+  return q;
+}
+
+// kWide: more than 8 query heads per KV head.
+template <int D, bool kWide>
+__global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_kernel(const Mxfp4DecodeParams p) {
+  constexpr int W = D / 32;                  // words of K (and of V) codes per lane and block
+  constexpr int NT = D / 32;                 // value MFMAs per block (of each parity, kWide)
+  constexpr int PARTS = kWide ? 2 : 1;       // accumulators: both parities in one, or even and odd
+  constexpr int STEP = kTile * kWaves;       // blocks from a wave's tile to its next
+  constexpr int AHEAD = 64 / kTile;          // tiles whose ids a window holds
   constexpr int PITCH = D + 4;
-  __shared__ __attribute__((aligned(16))) float lds_o[kWaves][kMxDecodeMaxGroup][PITCH];
+  __shared__ __attribute__((aligned(16))) float lds_o[kWaves][kWide ? 16 : 8][PITCH];
   __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -81,171 +129,201 @@ __global__ __launch_bounds__(kThreads, 2) void paged_decode_mxfp4_kernel(const M
   const int pieces = bad ? 1 : max(1, (nblk + p.chunk - 1) / p.chunk);
   if (s >= pieces) return;
   const int per = bad ? 0 : (nblk + pieces - 1) / pieces;
-  const int c0 = s * per;
-  int c1 = bad ? c0 : min(c0 + per, nblk);
-
-  const int32_t* table = p.tables + (int64_t)b * p.max_blocks;
-  // The wave's tiles: kTile blocks of every kTile * kWaves. Lane l holds the id
-  // of block l % kTile of the tile l / kTile further on.
+  const int c0 = s * per, c1 = bad ? c0 : min(c0 + per, nblk);
   const int first = c0 + w * kTile;
-  auto ids_from = [&](int tile) {
-    return table[min(first + (tile + lane / kTile) * (kTile * kWaves) + lane % kTile, p.max_blocks - 1)];
+  const int tiles = c1 > first ? (c1 - first + STEP - 1) / STEP : 0;  // of this wave
+
+  // Lane l holds the id of block l % kTile of the wave's tile l / kTile of
+  // AHEAD; -1 for one past the piece's end, or outside the pools.
+  const int32_t* table = p.tables + (int64_t)b * p.max_blocks;
+  int32_t window;
+  auto open_window = [&](int tile) {
+    const int blk = first + (tile + lane / kTile) * STEP + lane % kTile;
+    const int32_t id = table[min(blk, p.max_blocks - 1)];
+    const bool ok = id >= 0 && id < p.blocks;
+    if (__ballot(blk < c1 && !ok) != 0) bad = true;
+    window = blk < c1 && ok ? id : -1;
   };
-  int32_t window = ids_from(0);
-  const uint32_t head_codes = h * mx_head_bytes(D), head_scales = h * mx_head_scales(D);
+  open_window(0);
   const uint32_t code_at = lane * (D / 8);
   const uint32_t ks_at = (D == 128 ? g : g / 2) * kMxTokens + j;
   const uint32_t vs_at = (D == 128 ? j / 4 : j / 8) * kMxTokens + 4 * g;
-  // Every call issues the same loads. A block past the piece's end, or whose id
-  // is none of the pools', is an empty buffer: zeros, and no memory read.
-  auto load = [&](int tile, Tile<D>& r) {
-    if (tile && tile % (64 / kTile) == 0) window = ids_from(tile);
+  // Where a tile's blocks lie: a head's codes from the pools' start, a 16th of
+  // that for its scales. A block that is none is an empty buffer: its loads
+  // return zeros and read no memory.
+  uint64_t from[kTile];
+  bool live[kTile];
+  auto find = [&](int tile) {
+    if (tile && tile % AHEAD == 0) open_window(tile);
 #pragma unroll
     for (int u = 0; u < kTile; ++u) {
-      const int blk = first + tile * (kTile * kWaves) + u;
-      int32_t id = __builtin_amdgcn_readlane(window, (tile % (64 / kTile)) * kTile + u);
-      const bool want = blk < c1, ok = id >= 0 && id < p.blocks;
-      if (want && !ok) bad = true, c1 = min(c1, blk);
-      if (!ok) id = 0;
-      const uint64_t codes = (uint64_t)id * p.half + head_codes, scales = (uint64_t)id * (p.half / 16) + head_scales;
-      const uint32_t code_span = want && ok ? mx_head_bytes(D) : 0, scale_span = want && ok ? mx_head_scales(D) : 0;
-      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)(p.key_pool + codes), (short)0, code_span, 0x00020000);
-      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)(p.value_pool + codes), (short)0, code_span, 0x00020000);
-      const __amdgpu_buffer_rsrc_t rks = __builtin_amdgcn_make_buffer_rsrc((void*)(p.key_scales + scales), (short)0, scale_span, 0x00020000);
-      const __amdgpu_buffer_rsrc_t rvs = __builtin_amdgcn_make_buffer_rsrc((void*)(p.value_scales + scales), (short)0, scale_span, 0x00020000);
-      if constexpr (D == 128) {
-        const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(rk, code_at, 0, 0), y = __builtin_amdgcn_raw_buffer_load_b128(rv, code_at, 0, 0);
-#pragma unroll
-        for (int e = 0; e < W; ++e) r.k[u][e] = x[e], r.v[u][e] = y[e];
-      } else {
-        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(rk, code_at, 0, 0), y = __builtin_amdgcn_raw_buffer_load_b64(rv, code_at, 0, 0);
-#pragma unroll
-        for (int e = 0; e < W; ++e) r.k[u][e] = x[e], r.v[u][e] = y[e];
-      }
-      r.ks[u] = __builtin_amdgcn_raw_buffer_load_b8(rks, ks_at, 0, 0);
-      r.vs[u] = __builtin_amdgcn_raw_buffer_load_b32(rvs, vs_at, 0, 0);
+      const int32_t id = __builtin_amdgcn_readlane(window, (tile % AHEAD) * kTile + u);
+      live[u] = id >= 0;
+      from[u] = (uint64_t)(uint32_t)max(id, 0) * p.half + (uint32_t)h * mx_head_bytes(D);
     }
   };
-
-  // Query rows as the B operand: lane (g, j) holds head j's dims [g*D/4 + 8kk, +8).
-  bf16x8 q[NK];
-  {
-    const bool has = j < p.group;
-    const uint16_t* row = p.q + ((int64_t)b * p.q_heads + (int64_t)h * p.group + (has ? j : 0)) * D + g * (D / 4);
+  auto fetch = [&](const uint8_t* pool, const uint8_t* scale_pool, int u, uint32_t (&words)[W], uint32_t& scale, auto wide_scale) {
+    const __amdgpu_buffer_rsrc_t codes = __builtin_amdgcn_make_buffer_rsrc((void*)(pool + from[u]), (short)0, live[u] ? mx_head_bytes(D) : 0, 0x00020000);
+    const __amdgpu_buffer_rsrc_t scales =
+        __builtin_amdgcn_make_buffer_rsrc((void*)(scale_pool + from[u] / 16), (short)0, live[u] ? mx_head_scales(D) : 0, 0x00020000);
+    if constexpr (D == 128) {
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(codes, code_at, 0, 0);
 #pragma unroll
-    for (int kk = 0; kk < NK; ++kk) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(row + 8 * kk);
-      q[kk] = __builtin_bit_cast(bf16x8, has ? x : u32x4{0u, 0u, 0u, 0u});
+      for (int e = 0; e < W; ++e) words[e] = x[e];
+    } else {
+      const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(codes, code_at, 0, 0);
+#pragma unroll
+      for (int e = 0; e < W; ++e) words[e] = x[e];
+    }
+    if constexpr (decltype(wide_scale)::value) scale = __builtin_amdgcn_raw_buffer_load_b32(scales, vs_at, 0, 0);
+    else scale = __builtin_amdgcn_raw_buffer_load_b8(scales, ks_at, 0, 0);
+  };
+  Tile<D> r;
+  auto load_keys = [&] {
+#pragma unroll
+    for (int u = 0; u < kTile; ++u) fetch(p.key_pool, p.key_scales, u, r.k[u], r.ks[u], std::false_type{});
+  };
+  auto load_values = [&] {
+#pragma unroll
+    for (int u = 0; u < kTile; ++u) fetch(p.value_pool, p.value_scales, u, r.v[u], r.vs[u], std::true_type{});
+  };
+
+  // B of the scores: the scaled MFMA takes terms [16g, 16g + 16) and [64 + 16g,
+  // +16) of column j from lane (g, j), where A's lane (g, i) has terms [32g,
+  // +32): its key's dims in order, or (D = 64) 16 of them and 16 zeros.
+  u32x4 q_in[4] = {};
+  const int head = kWide ? j : j % 8;
+  {
+    const bool has = head < p.group;
+    const uint16_t* row = p.q + ((int64_t)b * p.q_heads + (int64_t)h * p.group + (has ? head : 0)) * D;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const uint16_t* at = row + (D == 128 ? 64 * part + 16 * g : 32 * part + 16 * (g / 2));
+      const bool mine = has && (D == 128 || g % 2 == 0);
+      const u32x4 x = *reinterpret_cast<const u32x4*>(at), y = *reinterpret_cast<const u32x4*>(at + 8);
+      q_in[2 * part] = mine ? x : u32x4{0u, 0u, 0u, 0u};
+      q_in[2 * part + 1] = mine ? y : u32x4{0u, 0u, 0u, 0u};
     }
   }
-  float m = -INFINITY, l = 0.f;  // of head j; l of this lane's tokens
-  f32x4 acc[NT];                 // lane (g, j): head j, dims (4g + r)*D/16 + n
-#pragma unroll
-  for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  find(0);
+  load_keys();
+  load_values();
+  uint32_t amax = max(max(mx_amax_bf16(q_in[0]), mx_amax_bf16(q_in[1])), max(mx_amax_bf16(q_in[2]), mx_amax_bf16(q_in[3])));
+  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16, 64));
+  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32, 64));
+  const SplitQuery q = split_query(q_in, amax);
+  // Which half of a BF16 pair (p, p) meets this lane's column.
+  const uint32_t parity = kWide || j >= 8 ? 0xffff0000u : 0x0000ffffu;
 
-  auto compute = [&](int tile, Tile<D>& r) {
-    // Tokens of this tile; fewer than 64 only at the piece's end.
-    const int blk0 = first + tile * (kTile * kWaves);
-    const int valid = min(seq, c1 * kBlockTokens) - blk0 * kBlockTokens;
-    const bool part = valid < kTile * kBlockTokens;
-    float sv[kTile][4];
-    float top = -INFINITY;
+  float m = -INFINITY, l = 0.f;  // of head j: its largest score, and (where parity keeps the upper half) this lane's sum
+  f32x4 acc[PARTS][NT];
+#pragma unroll
+  for (int x = 0; x < PARTS; ++x)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[x][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // One tile; `part`: fewer than 64 tokens of it count, the piece's last.
+  auto compute = [&](int tile, auto part) {
+    constexpr bool kPart = decltype(part)::value;
+    const int valid = kPart ? min(seq, c1 * kBlockTokens) - (first + tile * STEP) * kBlockTokens : 0;
+    f32x4 x[kTile];
 #pragma unroll
     for (int u = 0; u < kTile; ++u) {
-      const float scale = mx_scale(r.ks[u]);
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      i32x8 a = {};
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk) {
-        const u32x4 kb = mx_values(r.k[u][kk], scale);
-        x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kb), q[kk], x, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sv[u][i] = x[i] * p.scale;
+      for (int e = 0; e < W; ++e) a[e] = (int)r.k[u][e];
+      x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      x[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q.hi, x[u], 4, 0, 0, (int)r.ks[u], 0, q.hi_byte);
+      x[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q.lo, x[u], 4, 0, 0, (int)r.ks[u], 0, q.lo_byte);
     }
-    if (part) {
+    if constexpr (kPart) {
       // Tokens past the end: no score, and zeros for values that may be NaN.
 #pragma unroll
       for (int u = 0; u < kTile; ++u) {
         const int mine = min(max(valid - kBlockTokens * u - 4 * g, 0), 4);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i >= mine) sv[u][i] = -INFINITY;
-        const uint32_t keep = mine == 4 ? 0xffffffffu : (1u << 8 * mine) - 1u;
-        r.vs[u] &= keep;
+        for (int i = 0; i < 4; ++i) x[u][i] = i < mine ? x[u][i] : -INFINITY;
+        r.vs[u] &= mine == 4 ? 0xffffffffu : (1u << 8 * mine) - 1u;
 #pragma unroll
         for (int e = 0; e < W; ++e) {
           if constexpr (D == 128) r.v[u][e] = e < mine ? r.v[u][e] : 0u;
           else r.v[u][e] = 2 * e + 2 <= mine ? r.v[u][e] : 2 * e < mine ? r.v[u][e] & 0xffffu : 0u;
         }
       }
+    } else {
+      find(tile + 1);
+      load_keys();
     }
+    float top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kTile; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, sv[u][i]);
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, x[u][i]);
     const float mn = fmaxf(m, group_max4(top));
-    const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-    uint32_t pb[kTile][2];
+    const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * p.scale);
+    const float base = -mn * p.scale;
     float sum = 0.f;
+    uint32_t pb[kTile][4];
 #pragma unroll
-    for (int u = 0; u < kTile; ++u) {
+    for (int u = 0; u < kTile; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; i += 2) {
+      for (int i = 0; i < 4; ++i) {
         // a token past the end gets 0, or NaN where its head has no other score
         // than -infinity or NaN and is NaN whatever this token adds
-        const float a = __builtin_amdgcn_exp2f(sv[u][i] - mn), c = __builtin_amdgcn_exp2f(sv[u][i + 1] - mn);
-        const uint32_t pair = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, c}), mx_bf16x2));
-        pb[u][i / 2] = pair;
-        sum += bf16_lo(pair) + bf16_hi(pair);
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][i], p.scale, base));
+        pb[u][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{e, e}), mx_bf16x2));
+        sum += __uint_as_float(pb[u][i] & 0xffff0000u);
       }
-    }
     l = l * alpha + sum;
     m = mn;
     if (__ballot(alpha != 1.f) != 0) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int y = 0; y < PARTS; ++y)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] *= alpha;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[y][n][i] *= alpha;
     }
 #pragma unroll
-    for (int u = 0; u < kTile; u += 2) {
-      const bf16x8 pv = __builtin_bit_cast(bf16x8, u32x4{pb[u][0], pb[u][1], pb[u + 1][0], pb[u + 1][1]});
-      uint32_t c[2][4][W];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        token_pairs<D, 0>(r.v[u + x], r.vs[u + x], c[x][0]);
-        token_pairs<D, 1>(r.v[u + x], r.vs[u + x], c[x][1]);
-        token_pairs<D, 2>(r.v[u + x], r.vs[u + x], c[x][2]);
-        token_pairs<D, 3>(r.v[u + x], r.vs[u + x], c[x][3]);
-      }
+    for (int u = 0; u < kTile; ++u) {
+      uint32_t c[4][W];
+      token_pairs<D, 0>(r.v[u], r.vs[u], c[0]);
+      token_pairs<D, 1>(r.v[u], r.vs[u], c[1]);
+      token_pairs<D, 2>(r.v[u], r.vs[u], c[2]);
+      token_pairs<D, 3>(r.v[u], r.vs[u], c[3]);
+      const u32x4 even{pb[u][0] & 0xffffu, pb[u][1] & 0xffffu, pb[u][2] & 0xffffu, pb[u][3] & 0xffffu};
+      const u32x4 kept{pb[u][0] & parity, pb[u][1] & parity, pb[u][2] & parity, pb[u][3] & parity};
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const uint32_t pick = n % 2 ? 0x07060302u : 0x05040100u;  // the upper or the lower halves of two words
-        u32x4 a;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) a[x] = __builtin_amdgcn_perm(c[x / 2][2 * (x % 2) + 1][n / 2], c[x / 2][2 * (x % 2)][n / 2], pick);
-        acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), pv, acc[n], 0, 0, 0);
+        const bf16x8 a = __builtin_bit_cast(bf16x8, u32x4{c[0][n], c[1][n], c[2][n], c[3][n]});
+        acc[0][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, kept), acc[0][n], 0, 0, 0);
+        if constexpr (kWide) acc[PARTS - 1][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, even), acc[PARTS - 1][n], 0, 0, 0);
       }
     }
+    if constexpr (!kPart) load_values();
   };
 
-  Tile<D> r;
-  for (int tile = 0; first + tile * (kTile * kWaves) < c1; ++tile) {
-    load(tile, r);
-    compute(tile, r);
-  }
+  // Only the piece's last tile can be a partial one. A wave asks for a tile
+  // past its last one too: its blocks are empty buffers.
+  const bool cut = tiles > 0 && min(seq, c1 * kBlockTokens) < (first + (tiles - 1) * STEP + kTile) * kBlockTokens;
+  const int whole = cut ? tiles - 1 : tiles;
+  for (int tile = 0; tile < whole; ++tile) compute(tile, std::false_type{});
+  if (cut) compute(tiles - 1, std::true_type{});
 
-  // The waves' results into one: lane (g, j) holds head j.
+  // The waves' results into one. Lane (g, j) holds dims (4g + r)*D/16 + 2n + (its parity).
   l = group_sum4(l);
-  if (g == 0) {
-    lds_m[w][j] = m;
-    lds_l[w][j] = bad ? __builtin_nanf("") : l;
+  if (g == 0 && (kWide || j >= 8)) {
+    lds_m[w][head] = m * p.scale;
+    lds_l[w][head] = bad ? __builtin_nanf("") : l;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int x = 0; x < PARTS; ++x) {
+    const int odd = kWide ? 1 - x : j / 8;
 #pragma unroll
-    for (int n = 0; n < NT; n += 4)
-      *reinterpret_cast<f32x4*>(&lds_o[w][j][(4 * g + i) * (D / 16) + n]) = f32x4{acc[n][i], acc[n + 1][i], acc[n + 2][i], acc[n + 3][i]};
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lds_o[w][head][(4 * g + i) * (D / 16) + 2 * n + odd] = acc[x][n][i];
+  }
   __syncthreads();
   for (int unit = threadIdx.x; unit < p.group * (D / 4); unit += kThreads) {
     const int hj = unit / (D / 4), col = unit % (D / 4);
@@ -332,7 +410,9 @@ hipError_t launch(const Mxfp4DecodeParams& p, hipStream_t stream) {
       q.part_acc += first * p.q_heads * p.splits * D;
       q.part_ml += first * p.q_heads * p.splits * 2;
     }
-    hipLaunchKernelGGL((paged_decode_mxfp4_kernel<D>), dim3(p.kv_heads, p.splits, q.batch), dim3(kThreads), 0, stream, q);
+    const dim3 grid(p.kv_heads, p.splits, q.batch);
+    if (p.group > 8) hipLaunchKernelGGL((paged_decode_mxfp4_kernel<D, true>), grid, dim3(kThreads), 0, stream, q);
+    else hipLaunchKernelGGL((paged_decode_mxfp4_kernel<D, false>), grid, dim3(kThreads), 0, stream, q);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (p.splits == 1) continue;
