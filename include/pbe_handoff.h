@@ -538,15 +538,20 @@ int pbe_gather_kv_mxfp4(const void* key_pool, uint64_t key_pool_bytes, const voi
  * used. A length of 0 gives zeros; a negative one, one that needs more than
  * max_blocks_per_seq blocks, and a block id outside the pools give the
  * sequence NaN; a NaN group in a token's K or V reaches the heads that read
- * it, as does one in the queries.
- * A sequence is read in up to `splits` pieces (1..1024) whose partial results
- * lie in `workspace`: pbe_paged_decode_mxfp4_workspace_bytes() bytes, 16-byte
- * aligned, used until the call completes and holding anything when it starts;
- * none is needed, and NULL taken, for one split. The pieces of a sequence
- * depend on its length, max_blocks_per_seq and splits alone, so the same
- * sequence gives the same bits in any batch with these. splits = 0 takes
- * pbe_paged_decode_mxfp4_splits(), lowered until the workspace holds them.
- * Asynchronous on `stream`. */
+ * it, as does a NaN or an infinity in the queries; V values of 2^128 and more
+ * (scale bytes 253 and 254, which the writer does not store) give NaN.
+ * A batch's blocks are cut into pieces of one length, at most batch * splits of
+ * them and 1,024 of a sequence, whatever the lengths (the kernel looks at
+ * them); splits = 1 leaves every sequence whole. So the order of a sequence's
+ * sums, and with it the last bits of its output, depends on its batch unless
+ * splits is 1; for one batch they are the same on every call. splits 1..1024;
+ * 0 takes pbe_paged_decode_mxfp4_splits(), lowered to what the workspace holds.
+ * workspace: pbe_paged_decode_mxfp4_workspace_bytes() bytes of device memory
+ * (it takes 64-bit atomics), 16-byte aligned, used until the call completes and
+ * holding anything when it starts; none is needed, and NULL taken, for one
+ * split. A captured call keeps its marks in it: no other work may write the
+ * workspace while a replay runs, and one that was disturbed that way needs it
+ * cleared before the next replay. Asynchronous on `stream`. */
 int32_t pbe_paged_decode_mxfp4_splits(int32_t batch, int32_t kv_heads, int32_t max_blocks_per_seq);
 uint64_t pbe_paged_decode_mxfp4_workspace_bytes(int32_t batch, int32_t q_heads, int32_t head_dim,
                                                 int32_t splits);

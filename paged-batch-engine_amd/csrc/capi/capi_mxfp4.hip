@@ -153,8 +153,8 @@ int pbe_paged_decode_mxfp4(const void* key_pool, const void* value_pool, uint64_
   if (pool_bytes < half || scale_pool_bytes < half / 16) return fail(PBE_ERR_INVALID, "pools and scale pools must hold at least one block");
   if (splits == 0) {
     splits = pbe_paged_decode_mxfp4_splits(batch, kv_heads, max_blocks_per_seq);
-    const uint64_t each = (uint64_t)batch * (uint64_t)q_heads * (uint64_t)(head_dim + 2) * 4;  // bytes of one split
-    splits = (int32_t)std::max<uint64_t>(1, std::min<uint64_t>((uint64_t)splits, workspace ? workspace_bytes / each : 1));
+    const uint64_t two = pbe::mxfp4_decode_workspace_bytes(batch, q_heads, head_dim, 2);  // linear in the splits
+    splits = (int32_t)std::max<uint64_t>(1, std::min<uint64_t>((uint64_t)splits, workspace ? workspace_bytes / (two / 2) : 1));
   }
   const uint64_t need = pbe::mxfp4_decode_workspace_bytes(batch, q_heads, head_dim, splits);
   if (need && !workspace) return fail(PBE_ERR_INVALID, "more than one split needs a workspace");
@@ -169,6 +169,8 @@ int pbe_paged_decode_mxfp4(const void* key_pool, const void* value_pool, uint64_
         !ok(queries, rows) || !ok(outputs, rows) || !ok(block_tables, (uint64_t)batch * (uint64_t)max_blocks_per_seq * 4) ||
         !ok(seq_lens, (uint64_t)batch * 4) || !ok(workspace, need))
       return fail(PBE_ERR_INVALID, "decode operands must be memory of device %d", device);
+    // Arrival tickets are device atomics, which not every link carries to host memory.
+    if (need && on_host(workspace, known)) return fail(PBE_ERR_INVALID, "the decode workspace must be device memory");
   }
   pbe::Mxfp4DecodeParams p{};
   p.key_pool = static_cast<const uint8_t*>(key_pool);
@@ -186,11 +188,9 @@ int pbe_paged_decode_mxfp4(const void* key_pool, const void* value_pool, uint64_
   p.group = q_heads / kv_heads;
   p.max_blocks = max_blocks_per_seq;
   p.blocks = (int32_t)std::min<uint64_t>(std::min(pool_bytes / half, scale_pool_bytes / (half / 16)), INT32_MAX);
-  p.splits = splits;
   p.scale = (1.f / std::sqrt((float)head_dim)) * 1.4426950408889634f;
-  pbe::plan_mxfp4_decode(&p, head_dim, workspace);
   PBE_DEVICE_SCOPE(device);
-  PBE_HIP(pbe::launch_paged_decode_mxfp4(p, head_dim, static_cast<hipStream_t>(stream)));
+  PBE_HIP(pbe::launch_paged_decode_mxfp4(p, head_dim, splits, workspace, compute_units(device), static_cast<hipStream_t>(stream)));
   return PBE_OK;
 }
 

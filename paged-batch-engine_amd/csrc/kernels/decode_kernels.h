@@ -83,6 +83,9 @@ uint64_t decode_workspace_bytes(int32_t batch, int32_t q_heads, int32_t head_dim
 // `atomics`: whether the workspace takes device atomics, which the slots need.
 void plan_decode_slots(DecodeParams* p, bool fp8, int32_t splits, void* workspace, uint64_t bytes, bool atomics);
 
+// A launch's tag in the arrival tickets (arrival.h).
+uint64_t decode_tag();
+
 hipError_t launch_paged_decode(const DecodeParams& p, bool fp8, hipStream_t stream);
 hipError_t launch_paged_decode_splits(const DecodeParams& p, bool fp8, hipStream_t stream);
 

@@ -55,6 +55,7 @@
 #include <atomic>
 #include <chrono>
 
+#include "arrival.h"
 #include "decode_device.h"
 
 namespace pbe {
@@ -225,33 +226,7 @@ __device__ __forceinline__ Slot find_slot(uint32_t (*fit)[kWaves], const int32_t
 // so no L2 write-back or invalidate is needed: the writer waits for its
 // stores to complete, then takes a ticket; whoever takes the last one reads.
 constexpr int kAgent = 0x10;  // buffer access policy: agent scope
-
-// Arrival tickets. A word holds tag << kTicketBits | arrivals of launch `tag`;
-// anything else in it (a workspace may hold anything) counts as none. The last
-// arrival leaves 0, so a replayed launch, which has the same tag, starts anew.
-constexpr int kTicketBits = 11;
 static_assert(kDecodeMaxSplits < (1 << kTicketBits), "arrivals fit the ticket");
-// Makes a word that is 0 ready for arrivals; nothing waits for it.
-__device__ __forceinline__ void open_ticket(gptr<uint64_t> word, uint64_t tag) {
-  uint64_t none = 0;
-  (void)__hip_atomic_compare_exchange_strong(word, &none, tag << kTicketBits, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
-                                             __HIP_MEMORY_SCOPE_AGENT);
-}
-// Whether this is the last of `members` arrivals: one round trip where the
-// word was opened; a word that held something else is claimed by exchange.
-__device__ __forceinline__ bool last_arrival(gptr<uint64_t> word, uint64_t tag, uint32_t members) {
-  uint64_t now = __hip_atomic_fetch_add(word, (uint64_t)1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
-  if ((now >> kTicketBits) != tag) {
-    uint64_t seen = now;
-    do {
-      now = (seen >> kTicketBits) == tag ? seen + 1 : (tag << kTicketBits) | 1u;
-    } while (!__hip_atomic_compare_exchange_strong(word, &seen, now, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
-                                                   __HIP_MEMORY_SCOPE_AGENT));
-  }
-  if ((now & ((1u << kTicketBits) - 1)) != members) return false;
-  __hip_atomic_store(word, (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return true;
-}
 
 // One head's running combination of partials: maximum, sum and output, the
 // latter two weighted by 2^(m_i - m) (paged_mha_fast_kernel.cu:730-799). A NaN
@@ -820,7 +795,6 @@ uint64_t decode_workspace_bytes(int32_t batch, int32_t q_heads, int32_t head_dim
   return rows * head_dim * 4ull + 2ull * rows * 4ull;
 }
 
-namespace {
 // A launch's tag in the arrival tickets: never the same twice in a process,
 // and a word no float, code or id pattern makes (all twelve top bits set). The
 // clock keeps processes apart, and unlike a random device it cannot throw.
@@ -828,7 +802,6 @@ uint64_t decode_tag() {
   static std::atomic<uint64_t> next{(uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() * 0x9e3779b97f4a7c15ull};
   return 0xfffull << 41 | (next.fetch_add(1, std::memory_order_relaxed) & ((1ull << 41) - 1));
 }
-}  // namespace
 
 namespace {
 // How the batch is read; `slots` of one_round are one workgroup per compute

@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "decode_kernels.h"  // FastDiv
+
 namespace pbe {
 
 constexpr int kMxDecodeMaxGroup = 16;     // query heads per KV head
@@ -17,23 +19,25 @@ struct Mxfp4DecodeParams {
   uint16_t* out;
   const int32_t* tables;      // [batch][max_blocks]
   const int32_t* seq_lens;    // [batch]
-  float* part_acc;            // [batch][q_heads][splits][dim], splits > 1
-  float* part_ml;             // [batch][q_heads][splits][2]: maximum, sum
   uint32_t half;
   int32_t batch, q_heads, kv_heads, group, max_blocks;
   int32_t blocks;             // ids below it lie in all four pools
-  int32_t splits, chunk;      // a sequence of n blocks takes ceil(n / chunk) <= splits pieces
   float scale;                // log2(e) / sqrt(dim): scores in base 2
+  // Set by launch_paged_decode_mxfp4.
+  int32_t most;               // pieces there is room for; batch: every sequence whole
+  uint32_t wanted;            // pieces that fill the chip
+  int32_t min_chunk;          // blocks of a piece, at least
+  FastDiv by_heads;
+  float* part_acc;            // [most][q_heads][dim]: results of pieces
+  float* part_ml;             // [most][q_heads][2]: maximum, sum
+  uint64_t* tickets;          // [most][kv_heads]: arrivals (arrival.h)
+  uint64_t tag;               // of this launch
 };
 
-// Pieces of a sequence that the longest of a batch is cut into.
+// Pieces a sequence to make room for, and the bytes they take (one: none).
 int32_t mxfp4_decode_splits(int32_t batch, int32_t kv_heads, int32_t max_blocks, int64_t compute_units);
-// Bytes of partial results; one split has none.
 uint64_t mxfp4_decode_workspace_bytes(int32_t batch, int32_t q_heads, int32_t dim, int32_t splits);
 
-// Parts the workspace into the partial results and sets p.chunk.
-void plan_mxfp4_decode(Mxfp4DecodeParams* p, int dim, void* workspace);
-
-hipError_t launch_paged_decode_mxfp4(const Mxfp4DecodeParams& p, int dim, hipStream_t stream);
+hipError_t launch_paged_decode_mxfp4(Mxfp4DecodeParams p, int dim, int32_t splits, void* workspace, int64_t compute_units, hipStream_t stream);
 
 }  // namespace pbe

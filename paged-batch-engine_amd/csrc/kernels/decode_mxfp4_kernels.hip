@@ -3,7 +3,7 @@
 // output = sum(p v) / sum(p) in BF16.
 //
 // A workgroup of four waves reads one piece of a sequence for one KV head, its
-// waves tiles of four blocks (64 tokens) in turn.
+// waves tiles of two blocks (32 tokens) in turn.
 //  - loads: a block's codes of one head lie in the order of the lanes that
 //    take them, so one load instruction reads all of K, and one all of V. The
 //    next tile's K is asked for when the scores have used this one's, its V
@@ -12,8 +12,8 @@
 //    takes a block's 16 keys (A, E2M1 with the pages' own E8M0 scales) and the
 //    query heads of the KV head (B, E4M3, columns). A query is split into two
 //    E4M3 numbers of four significant bits, which hold a BF16 number's eight
-//    exactly down to 2^-13 of the head's largest, and to 2^-21 of that below;
-//    the second pair of MFMA operands adds the lower parts. The MFMA sums a
+//    exactly down to 2^-13 of the head's largest, and to 2^-21 of it below that;
+//    a second MFMA adds the lower parts. The MFMA sums a
 //    group's products to about 2^-17 of their magnitudes (measured), which is
 //    what a score is good for. Lane (g, j) ends with tokens 4g..4g+3 of head j.
 //  - values: lane (g, i) holds tokens 4g..4g+3 of column i, the D/16 dims
@@ -25,6 +25,13 @@
 //    carry the same heads again), zero elsewhere. So no two tokens have to be
 //    put side by side and no column of B is idle. More than 8 query heads take
 //    two such products, of the even and of the odd dims.
+//  - pieces: a batch's blocks are cut into pieces of one length c, the last of a
+//    sequence shorter, about as many as fill the chip, whatever the sequences'
+//    lengths: those are device memory, so every workgroup finds c and its piece
+//    from them (find_piece). The workgroup of a sequence's and KV head's that
+//    finishes last joins their results, in their order; they are written and
+//    read at agent scope (written through, read past the XCD's own L2), so no
+//    L2 is written back: a workgroup waits for its stores, then takes a ticket.
 //  - probabilities are rounded to BF16 for that product, and the sum they are
 //    divided by is of the rounded ones: each weight is off by at most 2^-8 of
 //    itself, and they still add up to one.
@@ -34,7 +41,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "decode_device.h"
+#include "arrival.h"
 #include "decode_mxfp4_kernels.h"
 #include "mxfp4_device.h"
 
@@ -42,7 +49,91 @@ namespace pbe {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kTile = 4;  // blocks of a wave's tile
+constexpr int kTile = 2;  // blocks of a wave's tile
+constexpr int kMinChunk = kTile * kWaves;  // blocks of a piece: a tile for every wave
+constexpr int kPiecesPerUnit = 2;  // wanted workgroups per compute unit
+constexpr int kJoin = 16;  // pieces' results that a thread has in flight
+constexpr int kAgent = 0x10;  // buffer access policy: agent scope
+static_assert(kMxDecodeMaxSplits < (1 << kTicketBits), "arrivals fit the ticket");
+
+// ---- which blocks a workgroup reads ----
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int scan_step(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false);
+}
+// Inclusive prefix sum over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+  x = scan_step<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: within rows of 16
+  x = scan_step<0x112, 0xf>(x);
+  x = scan_step<0x114, 0xf>(x);
+  x = scan_step<0x118, 0xf>(x);
+  x = scan_step<0x142, 0xa>(x);     // row_bcast 15 into rows 1 and 3
+  return scan_step<0x143, 0xc>(x);  // row_bcast 31 into rows 2 and 3
+}
+
+struct Piece {
+  int b = -1;       // sequence; -1: none for this workgroup
+  int seq = 0;      // its length
+  int s = 0, k = 1; // which of the sequence's pieces, and how many it has
+  int c = 0;        // blocks of a piece
+};
+
+// Piece z of the batch. c is the total over the pieces that are wanted, or what
+// fits the workspace: with `most` pieces to hold, sum of ceil(n / c) <= total /
+// c + batch <= most for c >= total / (most - batch).
+__device__ __forceinline__ Piece find_piece(const Mxfp4DecodeParams& p, int z, int lane) {
+  Piece r;
+  if (p.most == p.batch) {  // every sequence whole
+    r.b = z;
+    r.seq = p.seq_lens[z];
+    r.c = p.max_blocks;
+    return r;
+  }
+  constexpr int kKept = 4;  // sequences of a lane that stay in registers
+  int seqs[kKept], sum = 0, longest = 0;
+  for (int i0 = 0; i0 < p.batch; i0 += 64 * kKept) {
+    int now[kKept];
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) now[i] = i0 + 64 * i + lane < p.batch ? p.seq_lens[i0 + 64 * i + lane] : 0;
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) {
+      const int n = blocks_of(now[i], p.max_blocks);
+      sum += n;
+      longest = max(longest, n);
+      if (i0 == 0) seqs[i] = now[i];
+    }
+  }
+  const uint32_t total = (uint32_t)__builtin_amdgcn_readlane(wave_scan(sum), 63);
+  const uint32_t wanted = max((uint32_t)p.min_chunk, (total + p.wanted - 1) / p.wanted);
+  const uint32_t held = (uint32_t)(p.most - p.batch), fits = (total + held - 1) / held;
+  // Joining takes a workgroup about 1.3 times as long for a piece as reading
+  // takes it for a block: for n blocks in pieces of c, c + 1.3 n / c is least at
+  // c = sqrt(1.3 n).
+  const uint32_t n = (uint32_t)wave_max_int(longest);
+  const uint32_t joined = max((uint32_t)__builtin_amdgcn_sqrtf(1.3f * (float)n), (n + kMxDecodeMaxSplits - 1) / kMxDecodeMaxSplits);
+  const uint32_t c = max(max(wanted, fits), joined);
+  int before = 0;
+  for (int i = 0; i < p.batch; i += 64) {
+    int seq = seqs[0];
+#pragma unroll
+    for (int e = 1; e < kKept; ++e) seq = i == 64 * e ? seqs[e] : seq;
+    if (i >= 64 * kKept) seq = i + lane < p.batch ? p.seq_lens[i + lane] : 0;
+    const int k = i + lane < p.batch ? max(1, (int)(((uint32_t)blocks_of(seq, p.max_blocks) + c - 1) / c)) : 0;
+    const int upto = wave_scan(k) + before;
+    const uint64_t past = __ballot(upto > z);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      r.b = i + at;
+      r.seq = __builtin_amdgcn_readlane(seq, at);
+      r.k = __builtin_amdgcn_readlane(k, at);
+      r.s = z - (__builtin_amdgcn_readlane(upto, at) - r.k);
+      r.c = (int)c;
+      return r;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return r;
+}
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
@@ -51,7 +142,7 @@ template <int D>
 struct Tile {
   static constexpr int W = D / 32;  // words of codes
   uint32_t k[kTile][W], v[kTile][W];
-  uint32_t ks[kTile];  // scale byte of its key's quarter
+  uint32_t ks[kTile];  // scale bytes of its key's quarter, of four keys
   uint32_t vs[kTile];  // scale bytes of its four tokens' columns
 };
 
@@ -75,37 +166,26 @@ __device__ __forceinline__ void token_pairs(const uint32_t (&v)[D / 32], uint32_
   }
 }
 
-// A query head's 32 dims of this lane, BF16 pairs x, as E4M3 numbers hi + lo:
-// value = hi * 2^(hi_byte - 127) + lo * 2^(lo_byte - 127). `amax`: FP32 bits of
-// the head's largest magnitude, which hi takes to [2^7, 2^8); an infinity or a
-// NaN gives byte 255, the NaN scale.
+// Four BF16 dims of a query head (two pairs) as E4M3 numbers hi + lo: value =
+// hi * 2^(byte - 127) + lo * 2^(byte - 4 - 127), byte as split_byte() gives it.
 struct SplitQuery {
-  i32x8 hi, lo;
-  int hi_byte, lo_byte;
+  uint32_t hi, lo;
 };
-__device__ __forceinline__ SplitQuery split_query(const u32x4 (&x)[4], uint32_t amax) {
-  SplitQuery q;
-  const int e = (int)(amax >> 23);
-  const int byte = max(e - 7, 4);  // both parts' scales stay within a byte
-  q.hi_byte = e == 255 ? 255 : byte;
-  q.lo_byte = byte - 4;
-  // x * 2^(127 - byte) in two steps, either of them within FP32's exponents
-  const int down = 127 - byte, half = down / 2;
-  const float s0 = __uint_as_float((uint32_t)(half + 127) << 23), s1 = __uint_as_float((uint32_t)(down - half + 127) << 23);
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const uint32_t a = x[w / 2][2 * (w % 2)], b = x[w / 2][2 * (w % 2) + 1];
-    const float v[4] = {bf16_lo(a) * s0 * s1, bf16_hi(a) * s0 * s1, bf16_lo(b) * s0 * s1, bf16_hi(b) * s0 * s1};
-    uint32_t hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], hi, true);
-    const float r[4] = {(v[0] - __builtin_amdgcn_cvt_f32_fp8(hi, 0)) * 16.f, (v[1] - __builtin_amdgcn_cvt_f32_fp8(hi, 1)) * 16.f,
-                        (v[2] - __builtin_amdgcn_cvt_f32_fp8(hi, 2)) * 16.f, (v[3] - __builtin_amdgcn_cvt_f32_fp8(hi, 3)) * 16.f};
-    uint32_t lo = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], lo, true);
-    q.hi[w] = (int)(e == 255 ? 0u : hi);
-    q.lo[w] = (int)(e == 255 ? 0u : lo);
-  }
-  return q;
+// `amax`: FP32 bits of the head's largest magnitude, which hi takes to [2^7, 2^8).
+// Both parts' scales stay within a byte.
+__device__ __forceinline__ uint32_t split_byte(uint32_t amax) { return (uint32_t)max((int)(amax >> 23) - 7, 4); }
+__device__ __forceinline__ SplitQuery split_query(u32x2 x, uint32_t byte) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  const float hi_scale = mx_scale(byte), lo_scale = mx_scale(byte - 4);
+  const uint32_t a = x.x, b = x.y;
+  s16x2 hi = {0, 0}, lo = {0, 0};
+  hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, __builtin_bit_cast(mx_bf16x2, a), hi_scale, false);
+  hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, __builtin_bit_cast(mx_bf16x2, b), hi_scale, true);
+  const uint32_t h = __builtin_bit_cast(uint32_t, hi);
+  const f32x2 ha = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(h, hi_scale, false), hb = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(h, hi_scale, true);
+  lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, bf16_lo(a) - ha[0], bf16_hi(a) - ha[1], lo_scale, false);
+  lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, bf16_lo(b) - hb[0], bf16_hi(b) - hb[1], lo_scale, true);
+  return {h, __builtin_bit_cast(uint32_t, lo)};
 }
 
 // kWide: more than 8 query heads per KV head.
@@ -116,115 +196,160 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
   constexpr int PARTS = kWide ? 2 : 1;       // accumulators: both parities in one, or even and odd
   constexpr int STEP = kTile * kWaves;       // blocks from a wave's tile to its next
   constexpr int AHEAD = 64 / kTile;          // tiles whose ids a window holds
+  constexpr int HEADS = kWide ? 16 : 8;
   constexpr int PITCH = D + 4;
-  __shared__ __attribute__((aligned(16))) float lds_o[kWaves][kWide ? 16 : 8][PITCH];
+  __shared__ __attribute__((aligned(16))) float lds_o[kWaves][HEADS][PITCH];
   __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
+  __shared__ __attribute__((aligned(16))) uint32_t lds_q[2][HEADS][D / 4];  // the query heads' upper and lower parts
+  __shared__ uint32_t lds_byte[HEADS];
+  __shared__ int lds_last;
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, j = lane & 15;
-  const int h = blockIdx.x, s = blockIdx.y, b = blockIdx.z;
-  const int seq = p.seq_lens[b];
+  const int z = (int)fast_div(blockIdx.x, p.by_heads), h = (int)blockIdx.x - z * p.kv_heads;
+  const Piece piece = find_piece(p, z, lane);
+  if (piece.b < 0) return;
+  const int b = piece.b, seq = piece.seq, s = piece.s, pieces = piece.k;
   const int nblk = seq > 0 ? (int)(((uint32_t)seq + kBlockTokens - 1) / kBlockTokens) : 0;
-  bool bad = seq < 0 || nblk > p.max_blocks;
-  const int pieces = bad ? 1 : max(1, (nblk + p.chunk - 1) / p.chunk);
-  if (s >= pieces) return;
-  const int per = bad ? 0 : (nblk + pieces - 1) / pieces;
-  const int c0 = s * per, c1 = bad ? c0 : min(c0 + per, nblk);
-  const int first = c0 + w * kTile;
+  bool bad = seq < 0 || nblk > p.max_blocks;  // then it has one piece
+  const int c0 = s * piece.c, first = c0 + w * kTile;
+  const int c1 = bad ? c0 : min(c0 + piece.c, nblk);
   const int tiles = c1 > first ? (c1 - first + STEP - 1) / STEP : 0;  // of this wave
+  const int32_t* table = p.tables + (int64_t)b * p.max_blocks;
+  auto ids_of = [&](int tile) { return table[min(first + (tile + lane / kTile) * STEP + lane % kTile, p.max_blocks - 1)]; };
+  int32_t window = ids_of(0);
+  // The queries, four dims a thread, D/4 threads a head: asked for before the
+  // first tile, as loads come back in their order.
+  constexpr int ROUNDS = (HEADS * D / 4 + kThreads - 1) / kThreads;
+  const int64_t row0 = (int64_t)b * p.q_heads + (int64_t)h * p.group;  // the KV head's first query head
+  u32x2 q_in[ROUNDS];
+#pragma unroll
+  for (int n = 0; n < ROUNDS; ++n) {
+    const int unit = n * kThreads + (int)threadIdx.x, hj = unit / (D / 4);
+    q_in[n] = *reinterpret_cast<const u32x2*>(p.q + (row0 + min(hj, p.group - 1)) * D + 4 * (unit % (D / 4)));
+    if (hj >= p.group) q_in[n] = u32x2{0u, 0u};
+  }
 
   // Lane l holds the id of block l % kTile of the wave's tile l / kTile of
   // AHEAD; -1 for one past the piece's end, or outside the pools.
-  const int32_t* table = p.tables + (int64_t)b * p.max_blocks;
-  int32_t window;
-  auto open_window = [&](int tile) {
-    const int blk = first + (tile + lane / kTile) * STEP + lane % kTile;
-    const int32_t id = table[min(blk, p.max_blocks - 1)];
-    const bool ok = id >= 0 && id < p.blocks;
-    if (__ballot(blk < c1 && !ok) != 0) bad = true;
-    window = blk < c1 && ok ? id : -1;
+  auto check_ids = [&](int tile) {
+    const bool mine = first + (tile + lane / kTile) * STEP + lane % kTile < c1, ok = window >= 0 && window < p.blocks;
+    if (__ballot(mine && !ok) != 0) bad = true;
+    window = mine && ok ? window : -1;
   };
-  open_window(0);
+  check_ids(0);
   const uint32_t code_at = lane * (D / 8);
-  const uint32_t ks_at = (D == 128 ? g : g / 2) * kMxTokens + j;
-  const uint32_t vs_at = (D == 128 ? j / 4 : j / 8) * kMxTokens + 4 * g;
-  // Where a tile's blocks lie: a head's codes from the pools' start, a 16th of
-  // that for its scales. A block that is none is an empty buffer: its loads
-  // return zeros and read no memory.
+  const uint32_t key_scales_at = (D == 128 ? g : g / 2) * kMxTokens + (j & ~3), ks_shift = 8 * (j & 3);
+  const uint32_t value_scales_at = (D == 128 ? j / 4 : j / 8) * kMxTokens + 4 * g;
+  // Where a tile's blocks lie: bytes of codes from a pool's start, a 16th of
+  // that of scales. A block that is none is read from the pools' first: what a
+  // tile holds past the piece's end is not used, and a bad id makes NaN.
+  gptr<const uint8_t> k_codes = (gptr<const uint8_t>)p.key_pool + (uint32_t)h * mx_head_bytes(D);
+  gptr<const uint8_t> v_codes = (gptr<const uint8_t>)p.value_pool + (uint32_t)h * mx_head_bytes(D);
+  gptr<const uint8_t> k_scales = (gptr<const uint8_t>)p.key_scales + (uint32_t)h * mx_head_scales(D);
+  gptr<const uint8_t> v_scales = (gptr<const uint8_t>)p.value_scales + (uint32_t)h * mx_head_scales(D);
   uint64_t from[kTile];
-  bool live[kTile];
   auto find = [&](int tile) {
-    if (tile && tile % AHEAD == 0) open_window(tile);
 #pragma unroll
-    for (int u = 0; u < kTile; ++u) {
-      const int32_t id = __builtin_amdgcn_readlane(window, (tile % AHEAD) * kTile + u);
-      live[u] = id >= 0;
-      from[u] = (uint64_t)(uint32_t)max(id, 0) * p.half + (uint32_t)h * mx_head_bytes(D);
-    }
+    for (int u = 0; u < kTile; ++u)
+      from[u] = (uint64_t)(uint32_t)max(__builtin_amdgcn_readlane(window, (tile % AHEAD) * kTile + u), 0) * p.half;
   };
-  auto fetch = [&](const uint8_t* pool, const uint8_t* scale_pool, int u, uint32_t (&words)[W], uint32_t& scale, auto wide_scale) {
-    const __amdgpu_buffer_rsrc_t codes = __builtin_amdgcn_make_buffer_rsrc((void*)(pool + from[u]), (short)0, live[u] ? mx_head_bytes(D) : 0, 0x00020000);
-    const __amdgpu_buffer_rsrc_t scales =
-        __builtin_amdgcn_make_buffer_rsrc((void*)(scale_pool + from[u] / 16), (short)0, live[u] ? mx_head_scales(D) : 0, 0x00020000);
+  auto codes = [&](gptr<const uint8_t> at, uint32_t (&words)[W]) {
     if constexpr (D == 128) {
-      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(codes, code_at, 0, 0);
+      const u32x4 x = *(gptr<const u32x4>)at;
 #pragma unroll
       for (int e = 0; e < W; ++e) words[e] = x[e];
     } else {
-      const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(codes, code_at, 0, 0);
+      const u32x2 x = *(gptr<const u32x2>)at;
 #pragma unroll
       for (int e = 0; e < W; ++e) words[e] = x[e];
     }
-    if constexpr (decltype(wide_scale)::value) scale = __builtin_amdgcn_raw_buffer_load_b32(scales, vs_at, 0, 0);
-    else scale = __builtin_amdgcn_raw_buffer_load_b8(scales, ks_at, 0, 0);
   };
-  Tile<D> r;
-  auto load_keys = [&] {
-#pragma unroll
-    for (int u = 0; u < kTile; ++u) fetch(p.key_pool, p.key_scales, u, r.k[u], r.ks[u], std::false_type{});
+  // A block's address stays scalar, hidden from the compiler, which would add the
+  // lane's offset to the pool's address once and the block's to that with 64-bit
+  // vector additions.
+  auto block_at = [&](gptr<const uint8_t> pool, uint64_t offset) {
+    gptr<const uint8_t> at = pool + offset;
+    asm volatile("" : "+s"(at));
+    return at;
   };
-  auto load_values = [&] {
+  auto load_keys = [&](Tile<D>& r) {
 #pragma unroll
-    for (int u = 0; u < kTile; ++u) fetch(p.value_pool, p.value_scales, u, r.v[u], r.vs[u], std::true_type{});
+    for (int u = 0; u < kTile; ++u) {
+      codes(block_at(k_codes, from[u]) + code_at, r.k[u]);
+      r.ks[u] = *(gptr<const uint32_t>)(block_at(k_scales, from[u] / 16) + key_scales_at);
+    }
+  };
+  auto load_values = [&](Tile<D>& r) {
+#pragma unroll
+    for (int u = 0; u < kTile; ++u) {
+      codes(block_at(v_codes, from[u]) + code_at, r.v[u]);
+      r.vs[u] = *(gptr<const uint32_t>)(block_at(v_scales, from[u] / 16) + value_scales_at);
+    }
   };
 
+  Tile<D> r;
+  find(0);
+  if (tiles > 0) {
+    load_keys(r);
+    load_values(r);
+  }
+  const int z0 = z - s;  // the sequence's first piece
+  const gptr<uint64_t> ticket = (gptr<uint64_t>)p.tickets + (int64_t)z0 * p.kv_heads + h;
+  if (pieces > 1 && threadIdx.x == 0) open_ticket(ticket, p.tag);
+  // The queries, split once for the workgroup.
+#pragma unroll
+  for (int n = 0; n < ROUNDS; ++n) {
+    const int unit = n * kThreads + (int)threadIdx.x, hj = unit / (D / 4), at = unit % (D / 4);
+    if (hj >= HEADS) break;
+    const u32x2 x = q_in[n];
+    uint32_t amax = max(max(x.x & 0x7fff0000u, (x.x << 16) & 0x7fff0000u), max(x.y & 0x7fff0000u, (x.y << 16) & 0x7fff0000u));
+    amax = quad_max(amax);
+    amax = max(amax, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)amax, 0x141, 0xf, 0xf, false));
+    amax = max(amax, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)amax, 0x140, 0xf, 0xf, false));
+    if constexpr (D == 128) amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16, 64));
+    // an infinity or a NaN: the NaN scale
+    const bool fine = amax < 0x7f800000u;
+    const uint32_t byte = split_byte(amax);
+    const SplitQuery q = split_query(fine ? x : u32x2{0u, 0u}, byte);
+    lds_q[0][hj][at] = q.hi;
+    lds_q[1][hj][at] = q.lo;
+    if (at == 0) lds_byte[hj] = fine ? byte : 0xffu;
+  }
+  __syncthreads();
   // B of the scores: the scaled MFMA takes terms [16g, 16g + 16) and [64 + 16g,
   // +16) of column j from lane (g, j), where A's lane (g, i) has terms [32g,
   // +32): its key's dims in order, or (D = 64) 16 of them and 16 zeros.
-  u32x4 q_in[4] = {};
   const int head = kWide ? j : j % 8;
-  {
-    const bool has = head < p.group;
-    const uint16_t* row = p.q + ((int64_t)b * p.q_heads + (int64_t)h * p.group + (has ? head : 0)) * D;
+  i32x8 q[2];
 #pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      const uint16_t* at = row + (D == 128 ? 64 * part + 16 * g : 32 * part + 16 * (g / 2));
-      const bool mine = has && (D == 128 || g % 2 == 0);
-      const u32x4 x = *reinterpret_cast<const u32x4*>(at), y = *reinterpret_cast<const u32x4*>(at + 8);
-      q_in[2 * part] = mine ? x : u32x4{0u, 0u, 0u, 0u};
-      q_in[2 * part + 1] = mine ? y : u32x4{0u, 0u, 0u, 0u};
+  for (int part = 0; part < 2; ++part)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(&lds_q[part][head][(D == 128 ? 64 * half + 16 * g : 32 * half + 16 * (g / 2)) / 4]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[part][4 * half + e] = D == 128 || g % 2 == 0 ? (int)x[e] : 0;
     }
-  }
-  find(0);
-  load_keys();
-  load_values();
-  uint32_t amax = max(max(mx_amax_bf16(q_in[0]), mx_amax_bf16(q_in[1])), max(mx_amax_bf16(q_in[2]), mx_amax_bf16(q_in[3])));
-  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16, 64));
-  amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32, 64));
-  const SplitQuery q = split_query(q_in, amax);
+  const int hi_byte = (int)lds_byte[head], lo_byte = hi_byte == 0xff ? 0xff : hi_byte - 4;
   // Which half of a BF16 pair (p, p) meets this lane's column.
   const uint32_t parity = kWide || j >= 8 ? 0xffff0000u : 0x0000ffffu;
 
-  float m = -INFINITY, l = 0.f;  // of head j: its largest score, and (where parity keeps the upper half) this lane's sum
+  float m = -INFINITY;  // of head j: its largest score
   f32x4 acc[PARTS][NT];
+  f32x4 l = {0.f, 0.f, 0.f, 0.f};  // its sum of probabilities, by the MFMA against ones (four times the same)
+  const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
 #pragma unroll
   for (int x = 0; x < PARTS; ++x)
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[x][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // One tile; `part`: fewer than 64 tokens of it count, the piece's last.
-  auto compute = [&](int tile, auto part) {
-    constexpr bool kPart = decltype(part)::value;
+  // One tile. kNext: another one follows; kPart: fewer than 64 tokens count.
+  auto compute = [&](int tile, auto next, auto part) {
+    constexpr bool kNext = decltype(next)::value, kPart = decltype(part)::value;
+    if (kNext && (tile + 1) % AHEAD == 0) {
+      window = ids_of(tile + 1);
+      check_ids(tile + 1);
+    }
     const int valid = kPart ? min(seq, c1 * kBlockTokens) - (first + tile * STEP) * kBlockTokens : 0;
     f32x4 x[kTile];
 #pragma unroll
@@ -232,9 +357,10 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
       i32x8 a = {};
 #pragma unroll
       for (int e = 0; e < W; ++e) a[e] = (int)r.k[u][e];
+      const int ks = (int)(r.ks[u] >> ks_shift);  // the MFMA reads the lowest byte
       x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      x[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q.hi, x[u], 4, 0, 0, (int)r.ks[u], 0, q.hi_byte);
-      x[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q.lo, x[u], 4, 0, 0, (int)r.ks[u], 0, q.lo_byte);
+      x[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[0], x[u], 4, 0, 0, ks, 0, hi_byte);
+      x[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[1], x[u], 4, 0, 0, ks, 0, lo_byte);
     }
     if constexpr (kPart) {
       // Tokens past the end: no score, and zeros for values that may be NaN.
@@ -250,9 +376,11 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
           else r.v[u][e] = 2 * e + 2 <= mine ? r.v[u][e] : 2 * e < mine ? r.v[u][e] & 0xffffu : 0u;
         }
       }
-    } else {
+    }
+    if constexpr (kNext) {
+      __builtin_amdgcn_sched_barrier(0);  // into the registers that the scores have read
       find(tile + 1);
-      load_keys();
+      load_keys(r);
     }
     float top = -INFINITY;
 #pragma unroll
@@ -262,7 +390,6 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
     const float mn = fmaxf(m, group_max4(top));
     const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * p.scale);
     const float base = -mn * p.scale;
-    float sum = 0.f;
     uint32_t pb[kTile][4];
 #pragma unroll
     for (int u = 0; u < kTile; ++u)
@@ -272,11 +399,11 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
         // than -infinity or NaN and is NaN whatever this token adds
         const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][i], p.scale, base));
         pb[u][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{e, e}), mx_bf16x2));
-        sum += __uint_as_float(pb[u][i] & 0xffff0000u);
       }
-    l = l * alpha + sum;
     m = mn;
     if (__ballot(alpha != 1.f) != 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) l[i] *= alpha;
 #pragma unroll
       for (int y = 0; y < PARTS; ++y)
 #pragma unroll
@@ -293,6 +420,7 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
       token_pairs<D, 3>(r.v[u], r.vs[u], c[3]);
       const u32x4 even{pb[u][0] & 0xffffu, pb[u][1] & 0xffffu, pb[u][2] & 0xffffu, pb[u][3] & 0xffffu};
       const u32x4 kept{pb[u][0] & parity, pb[u][1] & parity, pb[u][2] & parity, pb[u][3] & parity};
+      l = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(bf16x8, kept), l, 0, 0, 0);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const bf16x8 a = __builtin_bit_cast(bf16x8, u32x4{c[0][n], c[1][n], c[2][n], c[3][n]});
@@ -300,21 +428,21 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
         if constexpr (kWide) acc[PARTS - 1][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, even), acc[PARTS - 1][n], 0, 0, 0);
       }
     }
-    if constexpr (!kPart) load_values();
+    if constexpr (kNext) load_values(r);
   };
 
-  // Only the piece's last tile can be a partial one. A wave asks for a tile
-  // past its last one too: its blocks are empty buffers.
+  // Only the piece's last tile can be a partial one.
   const bool cut = tiles > 0 && min(seq, c1 * kBlockTokens) < (first + (tiles - 1) * STEP + kTile) * kBlockTokens;
-  const int whole = cut ? tiles - 1 : tiles;
-  for (int tile = 0; tile < whole; ++tile) compute(tile, std::false_type{});
-  if (cut) compute(tiles - 1, std::true_type{});
+  const std::true_type yes;
+  const std::false_type no;
+  for (int tile = 0; tile < tiles - 1; ++tile) compute(tile, yes, no);
+  if (cut) compute(tiles - 1, no, yes);
+  else if (tiles > 0) compute(tiles - 1, no, no);
 
   // The waves' results into one. Lane (g, j) holds dims (4g + r)*D/16 + 2n + (its parity).
-  l = group_sum4(l);
-  if (g == 0 && (kWide || j >= 8)) {
+  if (g == 0) {  // lanes j and j + 8 hold the same
     lds_m[w][head] = m * p.scale;
-    lds_l[w][head] = bad ? __builtin_nanf("") : l;
+    lds_l[w][head] = bad ? __builtin_nanf("") : l[0];
   }
 #pragma unroll
   for (int x = 0; x < PARTS; ++x) {
@@ -325,6 +453,22 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
       for (int i = 0; i < 4; ++i) lds_o[w][head][(4 * g + i) * (D / 16) + 2 * n + odd] = acc[x][n][i];
   }
   __syncthreads();
+  // From here on a thread holds four dims of a head, more than one after another
+  // where the heads have more dims than the workgroup threads.
+  auto finish = [&](int hj, int col, const f32x4& o, float sum) {
+    uint16_t e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = to_bf16(sum != sum ? sum : sum > 0.f ? o[i] / sum : 0.f);
+    *reinterpret_cast<u32x2*>(p.out + (row0 + hj) * D + 4 * col) = u32x2{e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16};
+  };
+  // The sequence's partial results [piece][query head]; a piece's bytes times
+  // 1,024 fit 31 bits.
+  const uint32_t acc_pitch = (uint32_t)p.q_heads * (D * 4), ml_pitch = (uint32_t)p.q_heads * 8;
+  const __amdgpu_buffer_rsrc_t r_acc = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(p.part_acc + (int64_t)z0 * p.q_heads * D), (short)0, pieces > 1 ? (uint32_t)pieces * acc_pitch : 0, 0x00020000);
+  const __amdgpu_buffer_rsrc_t r_ml = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(p.part_ml + (int64_t)z0 * p.q_heads * 2), (short)0, pieces > 1 ? (uint32_t)pieces * ml_pitch : 0, 0x00020000);
+  const uint32_t head0 = (uint32_t)(h * p.group);
   for (int unit = threadIdx.x; unit < p.group * (D / 4); unit += kThreads) {
     const int hj = unit / (D / 4), col = unit % (D / 4);
     float top = -INFINITY, sum = 0.f;
@@ -337,116 +481,113 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
       sum += li != li ? li : li * wt;
       if (wt > 0.f) o += *reinterpret_cast<const f32x4*>(&lds_o[i][hj][4 * col]) * wt;
     }
-    const int64_t row = (int64_t)b * p.q_heads + (int64_t)h * p.group + hj;
-    if (pieces > 1) {
-      const int64_t at = row * p.splits + s;
-      *reinterpret_cast<f32x4*>(p.part_acc + at * D + 4 * col) = o;
-      if (col == 0) *reinterpret_cast<f32x2*>(p.part_ml + at * 2) = f32x2{top, sum};
+    if (pieces == 1) {
+      finish(hj, col, o, sum);
     } else {
-      uint16_t e[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) e[i] = to_bf16(sum != sum ? sum : sum > 0.f ? o[i] / sum : 0.f);
-      *reinterpret_cast<u32x2*>(p.out + row * D + 4 * col) = u32x2{e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16};
+      const uint32_t head = head0 + hj;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), r_acc, s * acc_pitch + head * (D * 4) + 16 * col, 0, kAgent);
+      if (col == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, f32x2{top, sum}), r_ml, s * ml_pitch + head * 8, 0, kAgent);
     }
   }
-}
-
-// The pieces of a sequence into its output: a workgroup per query head, its
-// lanes four dims each, D/4 of them a piece.
-template <int D>
-__global__ __launch_bounds__(kThreads) void paged_decode_mxfp4_join_kernel(const Mxfp4DecodeParams p) {
-  constexpr int COLS = D / 4, TEAMS = kThreads / COLS;
-  __shared__ f32x4 lds_o[TEAMS][COLS];
-  __shared__ f32x2 lds_ml[TEAMS];
-  const int row_head = blockIdx.x, b = blockIdx.y;
-  const int seq = p.seq_lens[b];
-  const int nblk = seq > 0 ? (int)(((uint32_t)seq + kBlockTokens - 1) / kBlockTokens) : 0;
-  if (nblk > p.max_blocks) return;
-  const int pieces = (nblk + p.chunk - 1) / p.chunk;
-  if (pieces <= 1) return;
-  const int team = threadIdx.x / COLS, col = threadIdx.x % COLS;
-  const int64_t row = (int64_t)b * p.q_heads + row_head;
-  const float* acc = p.part_acc + row * p.splits * D + 4 * col;
-  const float* ml = p.part_ml + row * p.splits * 2;
-  float m = -INFINITY, l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  auto join = [&](float mi, float li, const f32x4& x) {
-    const float mn = fmaxf(m, mi);
-    const float keep = l > 0.f ? __builtin_amdgcn_exp2f(m - mn) : 0.f, wt = li > 0.f ? __builtin_amdgcn_exp2f(mi - mn) : 0.f;
-    l = (l != l ? l : l * keep) + (li != li ? li : li * wt);
-    o = (keep > 0.f ? o * keep : f32x4{0.f, 0.f, 0.f, 0.f}) + (wt > 0.f ? x * wt : f32x4{0.f, 0.f, 0.f, 0.f});
-    m = mn;
-  };
-  for (int s = team; s < pieces; s += TEAMS) {
-    const f32x2 q = *reinterpret_cast<const f32x2*>(ml + 2 * s);
-    join(q[0], q[1], *reinterpret_cast<const f32x4*>(acc + (int64_t)s * D));
-  }
-  lds_o[team][col] = o;
-  if (col == 0) lds_ml[team] = f32x2{m, l};
+  if (pieces == 1) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's results have been written
   __syncthreads();
-  if (team != 0) return;
+  if (threadIdx.x == 0) lds_last = last_arrival(ticket, p.tag, (uint32_t)pieces);
+  __syncthreads();
+  if (!__builtin_amdgcn_readfirstlane(lds_last)) return;
+  for (int unit = threadIdx.x; unit < p.group * (D / 4); unit += kThreads) {
+    const int hj = unit / (D / 4), col = unit % (D / 4);
+    float top = -INFINITY, sum = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < pieces; s0 += kJoin) {
+      f32x2 ml[kJoin];
+      f32x4 x[kJoin];
 #pragma unroll
-  for (int i = 1; i < TEAMS; ++i) join(lds_ml[i][0], lds_ml[i][1], lds_o[i][col]);
-  uint16_t e[4];
+      for (int i = 0; i < kJoin; ++i) {  // past the end: nothing read
+        const uint32_t at = (uint32_t)min(s0 + i, pieces), head = head0 + hj;
+        ml[i] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(r_ml, at * ml_pitch + head * 8, 0, kAgent));
+        x[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r_acc, at * acc_pitch + head * (D * 4) + 16 * col, 0, kAgent));
+      }
+      float mn = top;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) e[i] = to_bf16(l != l ? l : l > 0.f ? o[i] / l : 0.f);
-  *reinterpret_cast<u32x2*>(p.out + row * D + 4 * col) = u32x2{e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16};
+      for (int i = 0; i < kJoin; ++i) mn = fmaxf(mn, s0 + i < pieces ? ml[i][0] : -INFINITY);
+      const float keep = sum > 0.f ? __builtin_amdgcn_exp2f(top - mn) : 0.f;
+      sum = sum != sum ? sum : sum * keep;
+      o = keep > 0.f ? o * keep : f32x4{0.f, 0.f, 0.f, 0.f};
+      top = mn;
+#pragma unroll
+      for (int i = 0; i < kJoin; ++i) {  // a NaN sum stays; a result of weight 0 is left out whatever it holds
+        const float li = ml[i][1], wt = li > 0.f ? __builtin_amdgcn_exp2f(ml[i][0] - mn) : 0.f;
+        sum += li != li ? li : li * wt;
+        if (wt > 0.f) o += x[i] * wt;
+      }
+    }
+    finish(hj, col, o, sum);
+  }
 }
 
-// A launch takes fewer than 2^32 threads: a batch of more workgroups is read in
-// parts, one after another on the stream.
 template <int D>
-hipError_t launch(const Mxfp4DecodeParams& p, hipStream_t stream) {
-  const int64_t most = std::min<int64_t>(0xffffffffll / kThreads / std::max<int64_t>((int64_t)p.kv_heads * p.splits, p.q_heads), 65535);
-  if (most < 1) return hipErrorInvalidConfiguration;
-  for (int64_t first = 0; first < p.batch; first += most) {
-    Mxfp4DecodeParams q = p;
-    q.batch = (int32_t)std::min<int64_t>(most, p.batch - first);
-    q.seq_lens += first;
-    q.tables += first * p.max_blocks;
-    q.q += first * p.q_heads * D;
-    q.out += first * p.q_heads * D;
-    if (p.splits > 1) {  // the workspace may be none otherwise
-      q.part_acc += first * p.q_heads * p.splits * D;
-      q.part_ml += first * p.q_heads * p.splits * 2;
-    }
-    const dim3 grid(p.kv_heads, p.splits, q.batch);
-    if (p.group > 8) hipLaunchKernelGGL((paged_decode_mxfp4_kernel<D, true>), grid, dim3(kThreads), 0, stream, q);
-    else hipLaunchKernelGGL((paged_decode_mxfp4_kernel<D, false>), grid, dim3(kThreads), 0, stream, q);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    if (p.splits == 1) continue;
-    hipLaunchKernelGGL((paged_decode_mxfp4_join_kernel<D>), dim3(p.q_heads, q.batch), dim3(kThreads), 0, stream, q);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  return hipSuccess;
+hipError_t launch(const Mxfp4DecodeParams& p, int64_t pieces, hipStream_t stream) {
+  const dim3 grid((unsigned)(pieces * p.kv_heads));
+  if (p.group > 8) hipLaunchKernelGGL((paged_decode_mxfp4_kernel<D, true>), grid, dim3(kThreads), 0, stream, p);
+  else hipLaunchKernelGGL((paged_decode_mxfp4_kernel<D, false>), grid, dim3(kThreads), 0, stream, p);
+  return hipGetLastError();
 }
+
+// Pieces that fill the chip, of the whole batch.
+int64_t wanted_pieces(int32_t kv_heads, int64_t compute_units) { return std::max<int64_t>(1, kPiecesPerUnit * compute_units / kv_heads); }
 
 }  // namespace
 
 int32_t mxfp4_decode_splits(int32_t batch, int32_t kv_heads, int32_t max_blocks, int64_t compute_units) {
-  const int64_t rows = (int64_t)batch * kv_heads;
-  const int64_t most = (max_blocks + kTile * kWaves - 1) / (kTile * kWaves);  // a tile for every wave
-  return (int32_t)std::max<int64_t>(1, std::min<int64_t>({4 * compute_units / rows, most, kMxDecodeMaxSplits}));
+  // Room for the wanted pieces and one more of each sequence, which a cut of
+  // unequal lengths can take; no sequence has more than its shortest pieces.
+  // Many whole sequences fill the chip by themselves, and their results would
+  // take gigabytes.
+  if ((int64_t)batch * kv_heads >= 16 * compute_units) return 1;
+  const int64_t pieces = wanted_pieces(kv_heads, compute_units) + batch, most = (max_blocks + kMinChunk - 1) / kMinChunk;
+  return (int32_t)std::max<int64_t>(1, std::min<int64_t>({(pieces + batch - 1) / batch, most, kMxDecodeMaxSplits}));
 }
 
 uint64_t mxfp4_decode_workspace_bytes(int32_t batch, int32_t q_heads, int32_t dim, int32_t splits) {
   if (splits <= 1) return 0;
-  return (uint64_t)batch * q_heads * splits * (dim + 2) * 4;
+  // a ticket a piece and KV head, of which there are no more than query heads
+  return (uint64_t)batch * q_heads * splits * ((uint64_t)(dim + 2) * 4 + 8);
 }
 
-void plan_mxfp4_decode(Mxfp4DecodeParams* p, int dim, void* workspace) {
-  p->chunk = (p->max_blocks + p->splits - 1) / p->splits;
-  if (p->splits == 1) return;
-  p->part_acc = static_cast<float*>(workspace);
-  p->part_ml = p->part_acc + (uint64_t)p->batch * p->q_heads * p->splits * dim;
-}
-
-hipError_t launch_paged_decode_mxfp4(const Mxfp4DecodeParams& p, int dim, hipStream_t stream) {
-  if (dim == 128) return launch<128>(p, stream);
-  if (dim == 64) return launch<64>(p, stream);
-  return hipErrorInvalidValue;
+hipError_t launch_paged_decode_mxfp4(Mxfp4DecodeParams p, int dim, int32_t splits, void* workspace, int64_t compute_units, hipStream_t stream) {
+  // A launch takes fewer than 2^32 threads: a batch of more workgroups is read in
+  // parts, one after another on the stream, in the same workspace.
+  const int64_t limit = 0xffffffffll / kThreads / p.kv_heads;
+  if (limit < 2) return hipErrorInvalidConfiguration;
+  const int32_t batch = p.batch;
+  // Totals of blocks are 32-bit sums, a sequence's results are addressed with 31 bits.
+  if ((int64_t)batch * p.max_blocks > INT32_MAX || (int64_t)p.q_heads * dim * 4 * kMxDecodeMaxSplits > INT32_MAX) splits = 1;
+  const int64_t wanted = wanted_pieces(p.kv_heads, compute_units);
+  const int64_t part = splits > 1 ? std::max<int64_t>(1, limit - wanted) : limit;
+  for (int64_t first = 0; first < batch; first += part) {
+    Mxfp4DecodeParams q = p;
+    q.batch = (int32_t)std::min<int64_t>(part, batch - first);
+    q.seq_lens += first;
+    q.tables += first * p.max_blocks;
+    q.q += first * p.q_heads * dim;
+    q.out += first * p.q_heads * dim;
+    const int64_t each = std::min<int64_t>(splits, (p.max_blocks + kMinChunk - 1) / kMinChunk);
+    const int64_t pieces = std::min<int64_t>({(int64_t)q.batch * each, wanted + q.batch, limit});
+    q.most = (int32_t)pieces;
+    q.wanted = (uint32_t)wanted;
+    q.min_chunk = kMinChunk;
+    q.by_heads = make_fast_div((uint32_t)p.kv_heads);
+    if (pieces > q.batch) {
+      q.part_acc = static_cast<float*>(workspace);
+      q.part_ml = q.part_acc + (uint64_t)pieces * p.q_heads * dim;
+      q.tickets = reinterpret_cast<uint64_t*>(q.part_ml + (uint64_t)pieces * p.q_heads * 2);
+      q.tag = decode_tag();
+    }
+    const hipError_t e = dim == 128 ? launch<128>(q, pieces, stream) : dim == 64 ? launch<64>(q, pieces, stream) : hipErrorInvalidValue;
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace pbe

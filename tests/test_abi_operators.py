@@ -94,7 +94,7 @@ READ = dict(key_pool=FAKE, value_pool=FAKE, pool_bytes=1 << 20, key_scales=FAKE,
     (dict(key_scales=0), INVALID), (dict(value_scales=0), INVALID), (dict(queries=0), INVALID), (dict(outputs=0), INVALID), (dict(tables=0), INVALID),
     (dict(seq_lens=0), INVALID), (dict(queries=FAKE + 8), INVALID), (dict(outputs=FAKE + 2), INVALID), (dict(value_pool=FAKE + 8), INVALID),
     (dict(key_scales=FAKE + 2), INVALID), (dict(workspace=FAKE + 8), INVALID), (dict(splits=-1), INVALID), (dict(splits=1025), INVALID),
-    (dict(workspace=0), INVALID), (dict(workspace_bytes=2 * 12 * 2 * 130 * 4 - 1), INVALID), (dict(pool_bytes=2047), INVALID),
+    (dict(workspace=0), INVALID), (dict(workspace_bytes=2 * 12 * 2 * (130 * 4 + 8) - 1), INVALID), (dict(pool_bytes=2047), INVALID),
     (dict(scale_pool_bytes=127), INVALID), (dict(kv_heads=2 ** 27, q_heads=2 ** 27), INVALID), (dict(batch=2 ** 30, q_heads=32), INVALID),
     (dict(batch=2 ** 20, max_blocks=2 ** 30), INVALID), (dict(device=-1), INVALID)])
 def test_mxfp4_reader_refuses(change, code):
@@ -103,9 +103,9 @@ def test_mxfp4_reader_refuses(change, code):
 
 def test_mxfp4_splits_and_workspace():
     assert P.decode_mxfp4_splits(0, 2, 10) == P.decode_mxfp4_splits(2, 0, 10) == P.decode_mxfp4_splits(2, 2, 0) == 1
-    assert P.decode_mxfp4_splits(100000, 8, 4096) == 1
+    assert P.decode_mxfp4_splits(100000, 8, 4096) == P.decode_mxfp4_splits(512, 8, 4096) == 1
     for batch, heads, blocks in ((1, 2, 315), (64, 4, 2048), (7, 1, 1), (1, 1, 1 << 27)):
         assert 1 <= P.decode_mxfp4_splits(batch, heads, blocks) <= min(1024, blocks)
     assert P.decode_mxfp4_workspace_bytes(3, 12, 128, 1) == 0
-    assert P.decode_mxfp4_workspace_bytes(3, 12, 128, 7) == 3 * 12 * 7 * 130 * 4
+    assert P.decode_mxfp4_workspace_bytes(3, 12, 128, 7) == 3 * 12 * 7 * (130 * 4 + 8)
     assert P.decode_mxfp4_workspace_bytes(0, 12, 128, 7) == 0

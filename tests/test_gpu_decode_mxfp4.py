@@ -157,26 +157,43 @@ def test_smallest_scales_give_equal_weights(torch_cuda):
     c.check()
 
 
-def test_a_sequence_has_the_same_bits_in_any_batch(torch_cuda):
+def test_bits_of_repeated_calls_and_of_whole_sequences(torch_cuda):
+    """A batch gives the same bits on every call; a sequence read whole (one
+    split) the same in any batch."""
     torch = torch_cuda
     say("decode mxfp4 bits in batches")
     c = Case(torch, [1000, 37, 640, 0, 999], 2, 6, 128, seed=6)
-    for splits in (1, 4, 40):
+    whole = None
+    for splits in (4, 40, 1):
         c.call(splits)
         torch.cuda.synchronize()
         whole = c.out.clone()
-        for again in range(3):
+        for again in range(4):
             c.out.fill_(1.0)
             c.call(splits)
             torch.cuda.synchronize()
-            assert torch.equal(whole.view(torch.int16), c.out.view(torch.int16))
-        order = [4, 2, 0, 3, 1]
-        d = Case(torch, [1000, 37, 640, 0, 999], 2, 6, 128, seed=6)
-        d.tables_dev, d.lens_dev = d.tables_dev[order].contiguous(), d.lens_dev[order].contiguous()
-        d.q = d.q[order].contiguous()
-        d.call(splits)
-        torch.cuda.synchronize()
-        assert torch.equal(d.out.view(torch.int16), whole[order].view(torch.int16)), splits
+            assert torch.equal(whole.view(torch.int16), c.out.view(torch.int16)), splits
+    order = [4, 2, 0, 3, 1]
+    d = Case(torch, [1000, 37, 640, 0, 999], 2, 6, 128, seed=6)
+    d.tables_dev, d.lens_dev = d.tables_dev[order].contiguous(), d.lens_dev[order].contiguous()
+    d.q = d.q[order].contiguous()
+    d.call(1)
+    torch.cuda.synchronize()
+    assert torch.equal(d.out.view(torch.int16), whole[order].view(torch.int16))
+
+
+@pytest.mark.parametrize("batch", [63, 64, 65, 256, 257, 700])
+def test_many_mixed_sequences_find_their_pieces(torch_cuda, batch):
+    say(f"decode mxfp4 {batch} mixed sequences")
+    rng = np.random.default_rng(batch)
+    lens = np.where(rng.random(batch) < 0.1, rng.integers(0, 2000, batch), rng.integers(0, 40, batch))
+    lens[batch // 2] = 2500
+    c = Case(torch_cuda, lens.tolist(), 1, 2, 64, seed=batch)
+    want = None
+    for splits in (0, 2, 9):
+        c.out.fill_(5.0)
+        c.call(splits)
+        want = c.check(want=want)
 
 
 @pytest.mark.parametrize("splits", [1, 8])
@@ -323,3 +340,34 @@ def test_workspace_rules(torch_cuda):
     with pytest.raises(P.PbeError) as e:
         c.call(4, workspace=Pageable)
     assert e.value.code == P.PBE_ERR_INVALID
+    pinned = torch.empty(P.decode_mxfp4_workspace_bytes(2, 12, 128, 4), dtype=torch.uint8).pin_memory()
+    with pytest.raises(P.PbeError) as e:  # its tickets are device atomics
+        c.call(4, workspace=pinned)
+    assert e.value.code == P.PBE_ERR_INVALID
+
+
+def test_two_graphs_share_a_workspace(torch_cuda):
+    """Replayed one after the other, with other work in the workspace between."""
+    torch = torch_cuda
+    say("decode mxfp4 two graphs, one workspace")
+    cases = [Case(torch, [700, 90, 1500], 2, 6, 128, seed=16), Case(torch, [64, 900], 4, 12, 64, seed=17)]
+    ws = torch.full((max(c.workspace(12).numel() for c in cases),), 0x55, dtype=torch.uint8, device="cuda")
+    graphs = []
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for c in cases:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.stream(side):
+            with torch.cuda.graph(graphs[-1], stream=side):
+                c.call(12, workspace=ws, stream=side.cuda_stream)
+    want = [None, None]
+    for rep in range(4):
+        if rep == 2:
+            ws.random_(0, 256)
+        for i in (0, 1, 1, 0):
+            cases[i].out.fill_(5.0)
+            torch.cuda.synchronize()
+            graphs[i].replay()
+            want[i] = cases[i].check(want=want[i])
+        cases[0].call(5, workspace=ws)
+        cases[0].check(want=want[0])
