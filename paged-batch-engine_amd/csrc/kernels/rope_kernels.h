@@ -28,12 +28,13 @@ struct RopeParams {
   uint32_t n_tokens, q_heads, kv_heads;
   uint32_t max_position, rotary;
   float eps;
-  uint32_t runs;             // of heads per token
+  uint32_t runs;             // of heads per token: q_runs + 2 * kv_runs
+  uint32_t q_runs, kv_runs;
   uint32_t units;            // lanes (< 2^31)
   FastDiv by_runs;
 };
 
-// Sets runs, units and by_runs; n_tokens * (q_heads + 2 * kv_heads) * dim / 8 < 2^31.
+// Sets runs to by_runs; n_tokens * (q_heads + 2 * kv_heads) * dim / 8 < 2^31.
 hipError_t launch_qk_norm_rope(RopeParams p, int dim, bool f32_input, bool pairs, PageKind pages, int64_t compute_units, hipStream_t stream);
 
 }  // namespace pbe

@@ -140,10 +140,13 @@ def test_norms_are_optional_for_queries_and_keys(torch_cuda, norm):
     r.check_bf16(bufs)
 
 
-@pytest.mark.parametrize("n,heads,group,dim", [(700, 4, 7, 128), (2100, 2, 3, 64), (1500, 2, 6, 128)])
-def test_long_prompts_take_runs_of_heads(torch_cuda, n, heads, group, dim):
+@pytest.mark.parametrize("n,heads,group,dim,rotary", [
+    (700, 4, 7, 128, 128), (2100, 2, 3, 64, 64),          # a head at a time
+    (1000, 4, 7, 128, 128), (3700, 2, 7, 64, 64), (1100, 3, 9, 128, 96),   # two
+    (2800, 4, 7, 128, 128), (2001, 5, 7, 128, 64), (11000, 2, 7, 64, 64)])  # four
+def test_long_prompts_take_runs_of_heads(torch_cuda, n, heads, group, dim, rotary):
     say(f"qk_norm_rope n={n} H={heads}x{group} D={dim}")
-    r = Rope(torch_cuda, n, heads, group, dim, dim, seed=n)
+    r = Rope(torch_cuda, n, heads, group, dim, rotary, pairs=rotary == 64 and dim == 128, seed=n)
     bufs, args = r.pools(P.PBE_KV_BF16)
     r.call(P.PBE_KV_BF16, args, stream_ptr(torch_cuda))
     r.check_bf16(bufs)
@@ -151,7 +154,7 @@ def test_long_prompts_take_runs_of_heads(torch_cuda, n, heads, group, dim):
 
 @pytest.mark.parametrize("kind", [P.PBE_KV_FP8_E4M3, P.PBE_KV_MXFP4], ids=["fp8", "mxfp4"])
 @pytest.mark.parametrize("n,heads,group,dim,f32", [(1, 2, 6, 128, False), (90, 2, 7, 64, False), (77, 4, 7, 128, True), (1600, 3, 5, 128, False),
-                                                   (1700, 2, 4, 64, True)])
+                                                   (3000, 4, 7, 64, True), (3000, 4, 7, 128, False)])
 def test_quantised_pages_are_those_of_the_page_writers(torch_cuda, kind, n, heads, group, dim, f32):
     """The BF16 rows of one call, written by the page writer of the other type."""
     torch = torch_cuda
