@@ -25,7 +25,7 @@ struct StepTablesParams {
 };
 
 // Tokens and table entries that one workgroup writes.
-constexpr uint32_t kStepTokens = 1024, kStepEntries = 2048;
+constexpr uint32_t kStepTokens = 256, kStepEntries = 1024;
 
 hipError_t launch_step_tables(StepTablesParams p, hipStream_t stream);
 

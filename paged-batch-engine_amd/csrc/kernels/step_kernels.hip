@@ -5,12 +5,18 @@
 //   token t of request b: position p = cached_b + t - start_b,
 //   slot = page[p / block_size] * block_size + p % block_size.
 //
-// One launch. A workgroup writes the slots and positions of 1,024 tokens, or
-// 2,048 entries of the tables, which need no sums; the first one writes
+// One launch. A workgroup writes the slots and positions of 256 tokens, or
+// 1,024 entries of the tables, which need no sums; the first one writes
 // lengths and starts as well. The tokens' requests follow from a prefix sum
 // over new_lens, which every token workgroup makes for itself, 1,024 requests
 // at a time, up to the last request of its tokens: the lengths are a few KB
 // out of L2, and a second launch would cost more than the sum.
+//
+// What bounds it: the launch and three round trips (lengths and lists, page,
+// store). us in a graph: one request 3.0, 256 decoding ones with tables of 440
+// blocks 3.7, 48 requests up to 32,768 tokens that add 12,288 3.9. With four
+// tokens a thread, one after another, the last took 6.0, side by side 5.1 and the
+// second 4.6.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -21,7 +27,7 @@ namespace pbe {
 namespace {
 
 constexpr int kThreads = 256, kPer = 4, kChunk = kThreads * kPer;  // requests summed at a time
-static_assert(kStepTokens == kChunk, "a thread sums four requests and writes four tokens");
+static_assert(kStepTokens == kThreads, "a token a thread");
 
 template <int kCtrl, int kRows>
 __device__ __forceinline__ int scan_step(int x) {
@@ -37,24 +43,12 @@ __device__ __forceinline__ int wave_scan(int x) {
   return scan_step<0x143, 0xc>(x);  // row_bcast 31 into rows 2 and 3
 }
 
-// A request's pages, and whether its lengths and pages make sense.
-struct Request {
-  int64_t len;     // cached + new
-  uint32_t first;  // of page_ids
-  uint32_t pages;
-  bool ok;
-};
-__device__ __forceinline__ Request request(const StepTablesParams& p, uint32_t b, int32_t added) {
-  Request r;
-  const int32_t cached = p.cached_lens[b], lo = p.page_starts[b], hi = p.page_starts[b + 1];
-  r.len = (int64_t)cached + added;
-  const bool listed = lo >= 0 && hi >= lo && (uint32_t)hi <= p.n_page_ids;
-  r.first = listed ? (uint32_t)lo : 0u;
-  r.pages = listed ? (uint32_t)(hi - lo) : 0u;
-  const uint32_t last = (uint32_t)min(max(r.len - 1, (int64_t)0), (int64_t)0x7ffffffe);
-  const uint32_t blocks = r.len > 0 ? fast_div(last, p.by_block_size) + 1 : 0;
-  r.ok = listed && cached >= 0 && added >= 0 && r.len <= 0x7fffffff && blocks <= r.pages && blocks <= p.max_blocks;
-  return r;
+// Whether a request's lengths and pages make sense, and its length then.
+__device__ __forceinline__ bool fits(const StepTablesParams& p, int32_t cached, int32_t added, int32_t lo, int32_t hi) {
+  if (lo < 0 || hi < lo || (uint32_t)hi > p.n_page_ids || cached < 0 || added < 0 || (int64_t)cached + added > 0x7fffffff) return false;
+  const uint32_t len = (uint32_t)cached + (uint32_t)added;
+  const uint32_t blocks = len ? fast_div(len - 1, p.by_block_size) + 1 : 0;
+  return blocks <= (uint32_t)(hi - lo) && blocks <= p.max_blocks;
 }
 
 // Exclusive prefix sum of `mine` over the workgroup and the workgroup's sum.
@@ -77,16 +71,25 @@ __device__ __forceinline__ uint64_t group_scan(uint64_t mine, uint64_t* sums, ui
 __device__ __forceinline__ uint32_t capped(uint64_t start) { return (uint32_t)min(start, (uint64_t)0x7fffffff); }
 
 __device__ __forceinline__ void write_tables(const StepTablesParams& p, uint32_t group) {
+  constexpr int kEach = kStepEntries / kThreads;  // a thread's entries, in flight together
   const uint32_t entries = p.batch * p.max_blocks, first = group * kStepEntries + threadIdx.x;
+  uint32_t j[kEach];
+  int32_t lo[kEach], hi[kEach], id[kEach];
 #pragma unroll
-  for (uint32_t i = 0; i < kStepEntries; i += kThreads) {
-    const uint32_t e = first + i;
-    if (e >= entries) return;
-    const uint32_t b = fast_div(e, p.by_max_blocks), j = e - b * p.max_blocks;
-    const int32_t lo = p.page_starts[b], hi = p.page_starts[b + 1];
-    const bool there = lo >= 0 && hi >= lo && (uint32_t)hi <= p.n_page_ids && j < (uint32_t)(hi - lo);
-    p.block_tables[e] = there ? p.page_ids[(uint32_t)lo + j] : -1;
+  for (int i = 0; i < kEach; ++i) {
+    const uint32_t e = min(first + i * kThreads, entries - 1), b = fast_div(e, p.by_max_blocks);
+    j[i] = e - b * p.max_blocks;
+    lo[i] = p.page_starts[b];
+    hi[i] = p.page_starts[b + 1];
   }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const bool there = lo[i] >= 0 && hi[i] >= lo[i] && (uint32_t)hi[i] <= p.n_page_ids && j[i] < (uint32_t)(hi[i] - lo[i]);
+    id[i] = there ? p.page_ids[(uint32_t)lo[i] + j[i]] : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (first + i * kThreads < entries) p.block_tables[first + i * kThreads] = id[i];
 }
 
 __global__ __launch_bounds__(kThreads) void step_tables_kernel(const StepTablesParams p) {
@@ -94,73 +97,71 @@ __global__ __launch_bounds__(kThreads) void step_tables_kernel(const StepTablesP
     write_tables(p, blockIdx.x - p.token_groups);
     return;
   }
+  // Of the chunk's requests: first row, cached tokens and first page (-1: a wrong one).
   __shared__ uint32_t starts[kChunk + 1];
+  __shared__ int32_t cached_of[kChunk], page_of[kChunk];
   __shared__ uint64_t sums[2][kThreads / 64];  // chunks take them in turn
   const uint32_t t = threadIdx.x;
   const bool lengths = blockIdx.x == 0;  // this workgroup writes these as well
-  const uint32_t first = blockIdx.x * kStepTokens, end = min(first + kStepTokens, p.max_tokens);
-  int32_t slot[kPer], position[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) slot[i] = position[i] = -1;
+  const uint32_t token = blockIdx.x * kStepTokens + t, end = min((blockIdx.x + 1) * kStepTokens, p.max_tokens);
+  int32_t slot = -1, position = -1;
   uint64_t before = 0;  // tokens of the requests before this chunk's
   for (uint32_t b0 = 0, turn = 0; b0 < p.batch && (lengths || before < end); b0 += kChunk, turn ^= 1) {
-    int32_t added[kPer];
+    // All that is known of a request is asked for at once: one round trip.
+    int32_t added[kPer], cached[kPer], lo[kPer], hi[kPer];
     uint64_t mine = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const uint32_t b = b0 + kPer * t + i;
-      added[i] = b < p.batch ? (p.new_lens ? p.new_lens[b] : 1) : 0;
+      const bool there = b < p.batch;
+      added[i] = !there ? 0 : p.new_lens ? p.new_lens[b] : 1;
+      cached[i] = there ? p.cached_lens[b] : 0;
+      lo[i] = there ? p.page_starts[b] : 0;
+      hi[i] = there ? p.page_starts[b + 1] : 0;
       mine += (uint32_t)max(added[i], 0);
     }
     uint64_t total, at = before + group_scan(mine, sums[turn], t, &total);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const uint32_t b = b0 + kPer * t + i;
-      starts[kPer * t + i] = capped(at);  // beyond any token: a thread's tokens are below max_tokens
+      const uint32_t r = kPer * t + i, b = b0 + r;
+      const uint64_t past = at + (uint32_t)max(added[i], 0);
+      const bool ok = fits(p, cached[i], added[i], lo[i], hi[i]) && past <= p.max_tokens;
+      starts[r] = capped(at);  // beyond any token: a thread's tokens are below max_tokens
+      cached_of[r] = cached[i];
+      page_of[r] = ok ? lo[i] : -1;
       if (lengths && b < p.batch) {
-        const uint64_t past = at + (uint32_t)max(added[i], 0);
-        const Request r = request(p, b, added[i]);
         p.token_starts[b] = (int32_t)capped(at);
-        p.seq_lens[b] = r.ok && past <= p.max_tokens ? (int32_t)r.len : -1;
+        p.seq_lens[b] = ok ? cached[i] + added[i] : -1;
         if (b + 1 == p.batch) p.token_starts[p.batch] = (int32_t)capped(past);
       }
-      at += (uint32_t)max(added[i], 0);
+      at = past;
     }
     if (t == kThreads - 1) starts[kChunk] = capped(at);
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const uint32_t token = first + i * kThreads + t;
-      if (token >= end || token < before || token >= before + total) continue;
-      // the last request that starts at or before the token: an empty one
-      // starts where the next does
-      uint32_t lo = 0, hi = kChunk;  // starts[lo] <= token < starts[hi]
-#pragma unroll
-      for (int step = 0; step < 10; ++step) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (starts[mid] <= token) lo = mid;
-        else hi = mid;
+    if (token < end && token >= before && token < before + total) {
+      // the last request that starts at or before the token (an empty one
+      // starts where the next does): starts[low] <= token < starts[high]
+      uint32_t low = 0, high = min(p.batch - b0, (uint32_t)kChunk);
+      for (uint32_t span = high; span > 1; span = (span + 1) / 2) {  // high - low is at most that
+        const uint32_t mid = (low + high) / 2;                       // low, where the two are next to each other
+        const bool down = starts[mid] > token;
+        high = down ? mid : high;
+        low = down ? low : mid;
       }
-      const uint32_t b = b0 + lo, row = token - starts[lo];
-      const int32_t n = p.new_lens ? p.new_lens[b] : 1;
-      const Request r = request(p, b, n);
-      if (!r.ok || starts[lo] + (uint32_t)n > p.max_tokens) continue;
-      const uint32_t pos = (uint32_t)(r.len - n) + row;
-      const uint32_t block = fast_div(pos, p.by_block_size);
-      const int32_t page = p.page_ids[r.first + block];
-      const int64_t s = (int64_t)page * p.block_size + (pos - block * p.block_size);
-      position[i] = (int32_t)pos;
-      slot[i] = page >= 0 && s <= 0x7fffffff ? (int32_t)s : -1;
+      if (page_of[low] >= 0) {
+        const uint32_t pos = (uint32_t)cached_of[low] + token - starts[low], block = fast_div(pos, p.by_block_size);
+        const int32_t page = p.page_ids[(uint32_t)page_of[low] + block];
+        const int64_t s = (int64_t)page * p.block_size + (pos - block * p.block_size);
+        position = (int32_t)pos;
+        slot = page >= 0 && s <= 0x7fffffff ? (int32_t)s : -1;
+      }
     }
     before += total;
     __syncthreads();  // the next chunk rewrites the starts
   }
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const uint32_t token = first + i * kThreads + t;
-    if (token >= end) continue;
-    p.slots[token] = slot[i];
-    p.positions[token] = position[i];
+  if (token < end) {
+    p.slots[token] = slot;
+    p.positions[token] = position;
   }
 }
 
