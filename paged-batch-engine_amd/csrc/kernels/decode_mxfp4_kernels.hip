@@ -25,9 +25,9 @@
 //    carry the same heads again), zero elsewhere. So no two tokens have to be
 //    put side by side and no column of B is idle. More than 8 query heads take
 //    two such products, of the even and of the odd dims.
-//  - pieces: a batch's blocks are cut into pieces of one length c, the last of a
-//    sequence shorter, about as many as fill the chip, whatever the sequences'
-//    lengths: those are device memory, so every workgroup finds c and its piece
+//  - pieces: a batch's blocks are cut into pieces of at most c blocks, even within
+//    a sequence, about as many as fill the chip, whatever the sequences' lengths:
+//    those are device memory, so every workgroup finds c and its piece
 //    from them (find_piece). The workgroup of a sequence's and KV head's that
 //    finishes last joins their results, in their order; they are written and
 //    read at agent scope (written through, read past the XCD's own L2), so no
@@ -52,7 +52,6 @@ constexpr int kWaves = 4, kThreads = 64 * kWaves;
 constexpr int kTile = 2;  // blocks of a wave's tile
 constexpr int kMinChunk = kTile * kWaves;  // blocks of a piece: a tile for every wave
 constexpr int kPiecesPerUnit = 2;  // wanted workgroups per compute unit
-constexpr int kJoin = 16;  // pieces' results that a thread has in flight
 constexpr int kAgent = 0x10;  // buffer access policy: agent scope
 static_assert(kMxDecodeMaxSplits < (1 << kTicketBits), "arrivals fit the ticket");
 
@@ -75,7 +74,7 @@ struct Piece {
   int b = -1;       // sequence; -1: none for this workgroup
   int seq = 0;      // its length
   int s = 0, k = 1; // which of the sequence's pieces, and how many it has
-  int c = 0;        // blocks of a piece
+  int c = 0;        // blocks of each but the last
 };
 
 // Piece z of the batch. c is the total over the pieces that are wanted, or what
@@ -127,7 +126,11 @@ __device__ __forceinline__ Piece find_piece(const Mxfp4DecodeParams& p, int z, i
       r.seq = __builtin_amdgcn_readlane(seq, at);
       r.k = __builtin_amdgcn_readlane(k, at);
       r.s = z - (__builtin_amdgcn_readlane(upto, at) - r.k);
-      r.c = (int)c;
+      // even pieces, of which the sequence may need fewer
+      const uint32_t n = (uint32_t)max(1, __builtin_amdgcn_readlane(blocks_of(seq, p.max_blocks), at));
+      r.c = (int)((n + (uint32_t)r.k - 1) / (uint32_t)r.k);
+      r.k = (int)((n + (uint32_t)r.c - 1) / (uint32_t)r.c);
+      if (r.s >= r.k) r.b = -1;
       return r;
     }
     before = __builtin_amdgcn_readlane(upto, 63);
@@ -495,35 +498,40 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
   if (threadIdx.x == 0) lds_last = last_arrival(ticket, p.tag, (uint32_t)pieces);
   __syncthreads();
   if (!__builtin_amdgcn_readfirstlane(lds_last)) return;
-  for (int unit = threadIdx.x; unit < p.group * (D / 4); unit += kThreads) {
-    const int hj = unit / (D / 4), col = unit % (D / 4);
-    float top = -INFINITY, sum = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < pieces; s0 += kJoin) {
-      f32x2 ml[kJoin];
-      f32x4 x[kJoin];
+  auto join = [&](auto in_flight) {
+    constexpr int kJoin = decltype(in_flight)::value;
+    for (int unit = threadIdx.x; unit < p.group * (D / 4); unit += kThreads) {
+      const int hj = unit / (D / 4), col = unit % (D / 4);
+      float top = -INFINITY, sum = 0.f;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      for (int s0 = 0; s0 < pieces; s0 += kJoin) {
+        f32x2 ml[kJoin];
+        f32x4 x[kJoin];
 #pragma unroll
-      for (int i = 0; i < kJoin; ++i) {  // past the end: nothing read
-        const uint32_t at = (uint32_t)min(s0 + i, pieces), head = head0 + hj;
-        ml[i] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(r_ml, at * ml_pitch + head * 8, 0, kAgent));
-        x[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r_acc, at * acc_pitch + head * (D * 4) + 16 * col, 0, kAgent));
+        for (int i = 0; i < kJoin; ++i) {  // past the end: nothing read
+          const uint32_t at = (uint32_t)min(s0 + i, pieces), head = head0 + hj;
+          ml[i] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(r_ml, at * ml_pitch + head * 8, 0, kAgent));
+          x[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r_acc, at * acc_pitch + head * (D * 4) + 16 * col, 0, kAgent));
+        }
+        float mn = top;
+#pragma unroll
+        for (int i = 0; i < kJoin; ++i) mn = fmaxf(mn, s0 + i < pieces ? ml[i][0] : -INFINITY);
+        const float keep = sum > 0.f ? __builtin_amdgcn_exp2f(top - mn) : 0.f;
+        sum = sum != sum ? sum : sum * keep;
+        o = keep > 0.f ? o * keep : f32x4{0.f, 0.f, 0.f, 0.f};
+        top = mn;
+#pragma unroll
+        for (int i = 0; i < kJoin; ++i) {  // a NaN sum stays; a result of weight 0 is left out whatever it holds
+          const float li = ml[i][1], wt = li > 0.f ? __builtin_amdgcn_exp2f(ml[i][0] - mn) : 0.f;
+          sum += li != li ? li : li * wt;
+          if (wt > 0.f) o += x[i] * wt;
+        }
       }
-      float mn = top;
-#pragma unroll
-      for (int i = 0; i < kJoin; ++i) mn = fmaxf(mn, s0 + i < pieces ? ml[i][0] : -INFINITY);
-      const float keep = sum > 0.f ? __builtin_amdgcn_exp2f(top - mn) : 0.f;
-      sum = sum != sum ? sum : sum * keep;
-      o = keep > 0.f ? o * keep : f32x4{0.f, 0.f, 0.f, 0.f};
-      top = mn;
-#pragma unroll
-      for (int i = 0; i < kJoin; ++i) {  // a NaN sum stays; a result of weight 0 is left out whatever it holds
-        const float li = ml[i][1], wt = li > 0.f ? __builtin_amdgcn_exp2f(ml[i][0] - mn) : 0.f;
-        sum += li != li ? li : li * wt;
-        if (wt > 0.f) o += x[i] * wt;
-      }
+      finish(hj, col, o, sum);
     }
-    finish(hj, col, o, sum);
-  }
+  };
+  if (pieces <= 4) join(std::integral_constant<int, 4>{});
+  else join(std::integral_constant<int, 16>{});
 }
 
 template <int D>
