@@ -27,7 +27,7 @@ struct Mxfp4DecodeParams {
   int32_t most;               // pieces there is room for; batch: every sequence whole
   uint32_t wanted;            // pieces that fill the chip
   int32_t min_chunk;          // blocks of a piece, at least
-  FastDiv by_heads;
+  FastDiv by_eight;           // workgroups of eight pieces
   float* part_acc;            // [most][q_heads][dim]: results of pieces
   float* part_ml;             // [most][q_heads][2]: maximum, sum
   uint64_t* tickets;          // [most][kv_heads]: arrivals (arrival.h)

@@ -44,6 +44,7 @@
 #include "arrival.h"
 #include "decode_mxfp4_kernels.h"
 #include "mxfp4_device.h"
+#include "xcd_order.h"  // kXcds
 
 namespace pbe {
 namespace {
@@ -83,6 +84,7 @@ struct Piece {
 __device__ __forceinline__ Piece find_piece(const Mxfp4DecodeParams& p, int z, int lane) {
   Piece r;
   if (p.most == p.batch) {  // every sequence whole
+    if (z >= p.batch) return r;
     r.b = z;
     r.seq = p.seq_lens[z];
     r.c = p.max_blocks;
@@ -209,7 +211,12 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, j = lane & 15;
-  const int z = (int)fast_div(blockIdx.x, p.by_heads), h = (int)blockIdx.x - z * p.kv_heads;
+  // A piece's KV heads go to one XCD, eight pieces side by side: two to four heads'
+  // scales share a cache line, which several XCDs would read each for itself (64
+  // x 5,040 tokens of 2 x 128 fetch 90.6 MB of the 88.2 that they need, in the order
+  // of the heads 96.0; 18.3 us and 18.9).
+  const int eight = (int)fast_div(blockIdx.x, p.by_eight), in_eight = (int)blockIdx.x - eight * (int)p.by_eight.d;
+  const int z = eight * (int)kXcds + in_eight % (int)kXcds, h = in_eight / (int)kXcds;
   const Piece piece = find_piece(p, z, lane);
   if (piece.b < 0) return;
   const int b = piece.b, seq = piece.seq, s = piece.s, pieces = piece.k;
@@ -536,7 +543,7 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
 
 template <int D>
 hipError_t launch(const Mxfp4DecodeParams& p, int64_t pieces, hipStream_t stream) {
-  const dim3 grid((unsigned)(pieces * p.kv_heads));
+  const dim3 grid((unsigned)((pieces + kXcds - 1) / kXcds * kXcds * p.kv_heads));
   if (p.group > 8) hipLaunchKernelGGL((paged_decode_mxfp4_kernel<D, true>), grid, dim3(kThreads), 0, stream, p);
   else hipLaunchKernelGGL((paged_decode_mxfp4_kernel<D, false>), grid, dim3(kThreads), 0, stream, p);
   return hipGetLastError();
@@ -566,7 +573,7 @@ uint64_t mxfp4_decode_workspace_bytes(int32_t batch, int32_t q_heads, int32_t di
 hipError_t launch_paged_decode_mxfp4(Mxfp4DecodeParams p, int dim, int32_t splits, void* workspace, int64_t compute_units, hipStream_t stream) {
   // A launch takes fewer than 2^32 threads: a batch of more workgroups is read in
   // parts, one after another on the stream, in the same workspace.
-  const int64_t limit = 0xffffffffll / kThreads / p.kv_heads;
+  const int64_t limit = 0xffffffffll / kThreads / p.kv_heads / kXcds * kXcds;
   if (limit < 2) return hipErrorInvalidConfiguration;
   const int32_t batch = p.batch;
   // Totals of blocks are 32-bit sums, a sequence's results are addressed with 31 bits.
@@ -585,7 +592,7 @@ hipError_t launch_paged_decode_mxfp4(Mxfp4DecodeParams p, int dim, int32_t split
     q.most = (int32_t)pieces;
     q.wanted = (uint32_t)wanted;
     q.min_chunk = kMinChunk;
-    q.by_heads = make_fast_div((uint32_t)p.kv_heads);
+    q.by_eight = make_fast_div(kXcds * (uint32_t)p.kv_heads);
     if (pieces > q.batch) {
       q.part_acc = static_cast<float*>(workspace);
       q.part_ml = q.part_acc + (uint64_t)pieces * p.q_heads * dim;
