@@ -35,6 +35,14 @@
 //  - probabilities are rounded to BF16 for that product, and the sum they are
 //    divided by is of the rounded ones: each weight is off by at most 2^-8 of
 //    itself, and they still add up to one.
+//
+// Bound by the pages' bytes and, for few of them, by the chain of dependent reads
+// (arguments, lengths, ids, pages, ticket, results). Calls back to back in a
+// graph, on pages that stay: 64 x 5,040 tokens of 2 x 128 18.3 us, 4.8 TB/s of the
+// bytes needed; 64 mixed up to 32,768 of 4 x 128 32.8 us, 4.9 TB/s; 1 x 5,040 of 2
+// x 64 7.9 us. Of the first, calls that end after each part take: launch 2.2, its
+// piece found 2.7, queries split 3.6, all but the tiles and the join 4.7, all but
+// the join 16.5.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -50,9 +58,19 @@ namespace pbe {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kTile = 2;  // blocks of a wave's tile
-constexpr int kMinChunk = kTile * kWaves;  // blocks of a piece: a tile for every wave
-constexpr int kPiecesPerUnit = 2;  // wanted workgroups per compute unit
+// Below, in us: A 64 x 5,040 tokens of 2 x 128, B 64 mixed up to 32,768 of 4 x 128,
+// C 150 mixed up to 3,000 of 2 x 64, D 256 mixed up to 600 of 4 x 128.
+// Blocks of a wave's tile. A / B / C / D with tiles of 1: 18.9 / 31.5 / 14.2 / 14.2,
+// of 2: 18.3 / 32.8 / 13.0 / 13.6, of 4 (14 registers spill): 20.0 / 34.9 / 12.6 /
+// 16.1. Half the workgroups of eight waves: 19.7 / 34.6 / 14.7 / 18.4.
+constexpr int kTile = 2;
+// Blocks of a piece that joining is worth: two tiles for every wave. With one, 64
+// mixed up to 250 of 2 x 128 took 6.6 us for 4.7, 8 mixed up to 2,000 of 8 x 128
+// 8.8 for 8.1, 1 x 600 of 2 x 128 6.7 for 7.3, A to D the same.
+constexpr int kMinChunk = 2 * kTile * kWaves;
+// Wanted workgroups per compute unit. A / B / C / D with 1: 18.7 / 32.9 / 15.0 /
+// 13.5, 2: 18.3 / 32.8 / 13.0 / 13.6, 3: 20.9 / 34.2 / 14.3 / 19.1.
+constexpr int kPiecesPerUnit = 2;
 constexpr int kAgent = 0x10;  // buffer access policy: agent scope
 static_assert(kMxDecodeMaxSplits < (1 << kTicketBits), "arrivals fit the ticket");
 
@@ -193,7 +211,10 @@ __device__ __forceinline__ SplitQuery split_query(u32x2 x, uint32_t byte) {
   return {h, __builtin_bit_cast(uint32_t, lo)};
 }
 
-// kWide: more than 8 query heads per KV head.
+// kWide: more than 8 query heads per KV head. The wide form holds for any number
+// of them, in 151 registers and three waves a SIMD for 119 and four; for up to
+// eight it takes, A / B / C / D above, 19.2 / 34.5 / 13.9 / 18.2 us, this one 18.3
+// / 32.8 / 13.0 / 13.6.
 template <int D, bool kWide>
 __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_kernel(const Mxfp4DecodeParams p) {
   constexpr int W = D / 32;                  // words of K (and of V) codes per lane and block
@@ -353,7 +374,7 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[x][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // One tile. kNext: another one follows; kPart: fewer than 64 tokens count.
+  // One tile. kNext: another one follows; kPart: fewer than all of its tokens count.
   auto compute = [&](int tile, auto next, auto part) {
     constexpr bool kNext = decltype(next)::value, kPart = decltype(part)::value;
     if (kNext && (tile + 1) % AHEAD == 0) {
@@ -537,6 +558,9 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
       finish(hj, col, o, sum);
     }
   };
+  // Few results want few loads, many want them together. Always 16: 64 x 5,040 of
+  // 2 x 128 19.2 us for 18.3, 1 x 600 7.4 for 6.7. Always 4: 1 x 32,768 of 4 x 128
+  // 16.3 us for 14.7, 1 x 5,040 of 2 x 64 8.7 for 7.9.
   if (pieces <= 4) join(std::integral_constant<int, 4>{});
   else join(std::integral_constant<int, 16>{});
 }
@@ -557,8 +581,10 @@ int64_t wanted_pieces(int32_t kv_heads, int64_t compute_units) { return std::max
 int32_t mxfp4_decode_splits(int32_t batch, int32_t kv_heads, int32_t max_blocks, int64_t compute_units) {
   // Room for the wanted pieces and one more of each sequence, which a cut of
   // unequal lengths can take; no sequence has more than its shortest pieces.
-  // Many whole sequences fill the chip by themselves, and their results would
-  // take gigabytes.
+  // Many whole sequences fill the chip by themselves, with no piece to find and
+  // none to join: 1,024 mixed sequences of 4 KV heads, the fewest that 256 compute
+  // units take whole, up to 600 tokens 32.1 us, in pieces 50.2; up to 4,000 191
+  // and 196.
   if ((int64_t)batch * kv_heads >= 16 * compute_units) return 1;
   const int64_t pieces = wanted_pieces(kv_heads, compute_units) + batch, most = (max_blocks + kMinChunk - 1) / kMinChunk;
   return (int32_t)std::max<int64_t>(1, std::min<int64_t>({(pieces + batch - 1) / batch, most, kMxDecodeMaxSplits}));
