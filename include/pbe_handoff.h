@@ -606,7 +606,9 @@ int pbe_build_step_tables(const int32_t* page_ids, int64_t n_page_ids, const int
  *     q_stride elements after row t - 1, so parts of one packed row work. 16-byte
  *     aligned, strides whole multiples of 16 bytes.
  *   q_weight, k_weight: [head_dim] of in_dtype, 16-byte aligned, or NULL for no
- *     norm of those heads: x <- x / sqrt(mean(x^2) + eps) * weight.
+ *     norm of those heads: x <- x / sqrt(mean(x^2) + eps) * weight, eps finite
+ *     and at least 2^-126. The squares are summed in FP32, so a head whose
+ *     squares add up to 2^128 or more comes out as zeros.
  *   positions: int32 [n_tokens]; a negative one marks a padding token, whose
  *     q_out row stays as it is and which writes no page. NULL (rotary_dim 0
  *     only): none is padding.

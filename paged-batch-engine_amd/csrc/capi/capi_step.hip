@@ -4,6 +4,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
+#include <utility>
 #include <vector>
 
 #include "capi_internal.h"
@@ -101,12 +103,15 @@ int pbe_qk_norm_rope_scatter(const void* q, int64_t q_stride, const void* k, int
     return fail(PBE_ERR_INVALID, "rotary_dim must be a multiple of 16 up to head_dim");
   if (rotary_dim && max_position <= 0) return fail(PBE_ERR_INVALID, "a rotation needs max_position > 0");
   if (!(eps >= 0.f) || std::isinf(eps)) return fail(PBE_ERR_INVALID, "eps must be finite and not negative");
+  // The root of a mean below FP32's normal numbers, which v_rsq_f32 takes for 0.
+  if ((q_weight || k_weight) && eps < std::numeric_limits<float>::min()) return fail(PBE_ERR_INVALID, "a norm needs eps of at least 2^-126");
   if (n_tokens == 0) return PBE_OK;
   const bool f32 = in_dtype == PBE_IN_F32, fp8 = kv_dtype == PBE_KV_FP8_E4M3, mx = kv_dtype == PBE_KV_MXFP4;
   const int64_t elem = f32 ? 4 : 2, dim = head_dim;
   // A token's heads fit one launch's 2^31 lanes, so the products below fit 64 bits.
   if (((int64_t)q_heads + 2 * (int64_t)kv_heads) * (dim / 8) >= (1ll << 31) / n_tokens)
     return fail(PBE_ERR_INVALID, "too many tokens for one launch");
+  if (std::max(q_heads, kv_heads) * dim * elem > 0xffffffffll) return fail(PBE_ERR_INVALID, "a token's heads must be smaller than 4 GiB");
   if (!q || !k || !v || !slot_mapping || !q_out || !key_pool || !value_pool || (rotary_dim && (!positions || !cos_sin)))
     return fail(PBE_ERR_INVALID, "null operand");
   if ((fp8 || mx) && (!key_scales || !value_scales)) return fail(PBE_ERR_INVALID, "FP8 and MXFP4 pools need K and V scale pools");
@@ -123,15 +128,18 @@ int pbe_qk_norm_rope_scatter(const void* q, int64_t q_stride, const void* k, int
   const uint64_t q_span = span(q_stride, q_heads), k_span = span(k_stride, kv_heads), v_span = span(v_stride, kv_heads);
   const uint64_t out_bytes = (uint64_t)n_tokens * (uint64_t)q_heads * (uint64_t)dim * 2;
   auto meets = [&](const void* in, uint64_t bytes) { return at(in) < at(q_out) + out_bytes && at(q_out) < at(in) + bytes; };
-  if (meets(q, q_span) || meets(k, k_span) || meets(v, v_span)) return fail(PBE_ERR_INVALID, "q_out must lie apart from q, k and v");
+  const uint64_t weight = (uint64_t)(dim * elem), table = rotary_dim ? (uint64_t)max_position * (uint64_t)rotary_dim * 4 : 0;
+  const uint64_t ints = (uint64_t)n_tokens * 4;
+  if (meets(q, q_span) || meets(k, k_span) || meets(v, v_span) || (q_weight && meets(q_weight, weight)) ||
+      (k_weight && meets(k_weight, weight)) || (table && meets(cos_sin, table)) || (positions && meets(positions, ints)) ||
+      meets(slot_mapping, ints))
+    return fail(PBE_ERR_INVALID, "q_out must lie apart from the inputs");
   {
     PBE_DEVICE_SCOPE(device);
     std::vector<Range> known;
     auto ok = [&](const void* ptr, uint64_t bytes) { return !ptr || bytes == 0 || accessible(ptr, bytes, device, &known); };
-    const uint64_t weight = (uint64_t)(dim * elem), line = (uint64_t)rotary_dim * 4;
     if (!ok(q, q_span) || !ok(k, k_span) || !ok(v, v_span) || !ok(q_weight, weight) || !ok(k_weight, weight) ||
-        !ok(positions, (uint64_t)n_tokens * 4) || !ok(slot_mapping, (uint64_t)n_tokens * 4) ||
-        (rotary_dim && !ok(cos_sin, (uint64_t)max_position * line)) || !ok(q_out, out_bytes) || !ok(key_pool, key_pool_bytes) ||
+        !ok(positions, ints) || !ok(slot_mapping, ints) || (table && !ok(cos_sin, table)) || !ok(q_out, out_bytes) || !ok(key_pool, key_pool_bytes) ||
         !ok(value_pool, value_pool_bytes) ||
         ((fp8 || mx) && (!ok(key_scales, key_scale_bytes) || !ok(value_scales, value_scale_bytes))))
       return fail(PBE_ERR_INVALID, "operands must be memory of device %d", device);

@@ -79,6 +79,18 @@ def test_rope_writer_refuses(change, code):
     refused(P.qk_norm_rope_scatter, ROPE, change, code)
 
 
+@pytest.mark.parametrize("change,says", [
+    (dict(eps=0.0), "eps"), (dict(eps=2.0 ** -127), "eps"), (dict(eps=0.0, q_weight=0), "eps"),
+    (dict(n_tokens=1, q_heads=2 ** 24, head_dim=128), "4 GiB"),
+    (dict(n_tokens=1, q_heads=2 ** 23, head_dim=128, in_dtype=P.PBE_IN_F32), "4 GiB"),
+    (dict(q_weight=FAKE + (1 << 20)), "apart"), (dict(k_weight=FAKE + (1 << 20) + 1008), "apart"), (dict(cos_sin=FAKE + (1 << 20) - 256), "apart"),
+    (dict(positions=FAKE + (1 << 20) - 12), "apart"), (dict(slots=FAKE + (1 << 20) + 4), "apart")])
+def test_rope_writer_names_what_it_refuses(change, says):
+    with pytest.raises(P.PbeError, match=says) as e:
+        P.qk_norm_rope_scatter(**{**ROPE, **change})
+    assert e.value.code == INVALID
+
+
 def test_rope_writer_without_tokens_is_no_work():
     P.qk_norm_rope_scatter(**{**ROPE, "n_tokens": 0, "q": 0, "k": 0, "v": 0, "slots": 0, "q_out": 0})
 

@@ -193,6 +193,19 @@ def test_no_positions_without_a_rotation(torch_cuda):
     r.check_bf16(bufs)
 
 
+def test_smallest_eps_under_squares_that_vanish(torch_cuda):
+    """Squares below FP32's smallest number leave eps alone under the root: 1e-50
+    against 2^-126 is far below the bound's 2^-18."""
+    torch = torch_cuda
+    say("qk_norm_rope with eps 2^-126")
+    r = Rope(torch, 6, 2, 2, 128, 128, seed=9, eps=2.0 ** -126)
+    r.bufs[0][3] *= 1e-13
+    r.x = r.bufs[0].double().cpu().numpy().reshape(r.x.shape)
+    bufs, args = r.pools(P.PBE_KV_BF16)
+    r.call(P.PBE_KV_BF16, args, stream_ptr(torch))
+    r.check_bf16(bufs)
+
+
 def test_not_a_number_stays_in_its_head(torch_cuda):
     torch = torch_cuda
     say("qk_norm_rope with NaN and infinity")
