@@ -381,7 +381,8 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
       window = ids_of(tile + 1);
       check_ids(tile + 1);
     }
-    const int valid = kPart ? min(seq, c1 * kBlockTokens) - (first + tile * STEP) * kBlockTokens : 0;
+    // of tokens up to 2^31, counted without a sign
+    const int valid = kPart ? (int)(min((uint32_t)seq, (uint32_t)c1 * kBlockTokens) - (uint32_t)(first + tile * STEP) * kBlockTokens) : 0;
     f32x4 x[kTile];
 #pragma unroll
     for (int u = 0; u < kTile; ++u) {
@@ -463,7 +464,7 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
   };
 
   // Only the piece's last tile can be a partial one.
-  const bool cut = tiles > 0 && min(seq, c1 * kBlockTokens) < (first + (tiles - 1) * STEP + kTile) * kBlockTokens;
+  const bool cut = tiles > 0 && min((uint32_t)seq, (uint32_t)c1 * kBlockTokens) < (uint32_t)(first + (tiles - 1) * STEP + kTile) * kBlockTokens;
   const std::true_type yes;
   const std::false_type no;
   for (int tile = 0; tile < tiles - 1; ++tile) compute(tile, yes, no);

@@ -275,6 +275,43 @@ def test_pool_offsets_beyond_32_bits(torch_cuda):
     c.check()
 
 
+@pytest.mark.parametrize("spare", [0, 17])
+def test_longest_sequence_ends_inside_its_last_block(torch_cuda, spare):
+    """2^31 - 1 - spare tokens: one block again and again, then another that is
+    cut. The block's scores are 0; the last one's 64 above, so that all the others
+    together weigh below 2^31 e^-64 < 2^-61; the token past the end's, 96. With equal
+    scores the output is the mean of the last block's values that count: off by
+    half a step of BF16 and, of 16 terms at most 6, by less than 2^-18."""
+    torch = torch_cuda
+    say("decode mxfp4 of 2^31 - 1 - %d tokens" % spare)
+    rng = np.random.default_rng(3)
+    n, dim = 2 ** 31 - 1 - spare, 64
+    blocks, end = -(-n // T), (n - 1) % T + 1
+    assert end < T
+    k, v = np.zeros((2 * T, dim)), np.zeros((2 * T, dim))
+    k[T:T + end], k[T + end:] = 8.0, 12.0
+    v[T:] = rng.choice([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], (T, dim)) * rng.choice([-1.0, 1.0], (T, dim))
+    v[T:, ::32] = 4.0
+    rows = [torch.tensor(x, dtype=torch.bfloat16, device="cuda") for x in (k, v)]
+    half = M.half_bytes(1, dim)
+    pools = [torch.zeros(2 * size, dtype=torch.uint8, device="cuda") for size in (half, half, half // 16, half // 16)]
+    slots = torch.arange(2 * T, dtype=torch.int32, device="cuda")
+    P.scatter_kv_mxfp4(rows[0].data_ptr(), rows[1].data_ptr(), P.PBE_IN_BF16, 2 * T, slots.data_ptr(), 1, dim,
+                       *(x for pool in pools for x in (pool.data_ptr(), pool.numel())), stream=stream_ptr(torch))
+    tables = torch.zeros(blocks, dtype=torch.int32, device="cuda")
+    tables[-1] = 1
+    q, out = torch.ones(1, 1, dim, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 1, dim, dtype=torch.bfloat16, device="cuda")
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    ws = torch.full((P.decode_mxfp4_workspace_bytes(1, 1, dim, 1024),), 0xff, dtype=torch.uint8, device="cuda")
+    P.paged_decode_mxfp4(pools[0].data_ptr(), pools[1].data_ptr(), pools[0].numel(), pools[2].data_ptr(), pools[3].data_ptr(), pools[2].numel(),
+                         1, dim, q.data_ptr(), out.data_ptr(), 1, 1, tables.data_ptr(), lens.data_ptr(), blocks, 0, ws.data_ptr(), ws.numel(),
+                         stream=stream_ptr(torch))
+    torch.cuda.synchronize()
+    want = v[T:T + end].mean(0)
+    off = np.abs(out.double().cpu().numpy()[0, 0] - want)
+    assert (off <= 2.0 ** -8 * np.abs(want) + 2.0 ** -18).all(), off.max()
+
+
 def test_decode_replays_from_a_graph_as_lengths_grow(torch_cuda):
     torch = torch_cuda
     say("decode mxfp4 in a graph")
