@@ -576,6 +576,8 @@ hipError_t launch(const Mxfp4DecodeParams& p, int64_t pieces, hipStream_t stream
 
 // Pieces that fill the chip, of the whole batch.
 int64_t wanted_pieces(int32_t kv_heads, int64_t compute_units) { return std::max<int64_t>(1, kPiecesPerUnit * compute_units / kv_heads); }
+// Pieces that a sequence of max_blocks blocks can be cut into: tables may be as wide as 2^31 - 1.
+int64_t most_pieces(int32_t max_blocks) { return ((int64_t)max_blocks + kMinChunk - 1) / kMinChunk; }
 
 }  // namespace
 
@@ -587,7 +589,7 @@ int32_t mxfp4_decode_splits(int32_t batch, int32_t kv_heads, int32_t max_blocks,
   // units take whole, up to 600 tokens 32.1 us, in pieces 50.2; up to 4,000 191
   // and 196.
   if ((int64_t)batch * kv_heads >= 16 * compute_units) return 1;
-  const int64_t pieces = wanted_pieces(kv_heads, compute_units) + batch, most = (max_blocks + kMinChunk - 1) / kMinChunk;
+  const int64_t pieces = wanted_pieces(kv_heads, compute_units) + batch, most = most_pieces(max_blocks);
   return (int32_t)std::max<int64_t>(1, std::min<int64_t>({(pieces + batch - 1) / batch, most, kMxDecodeMaxSplits}));
 }
 
@@ -614,7 +616,7 @@ hipError_t launch_paged_decode_mxfp4(Mxfp4DecodeParams p, int dim, int32_t split
     q.tables += first * p.max_blocks;
     q.q += first * p.q_heads * dim;
     q.out += first * p.q_heads * dim;
-    const int64_t each = std::min<int64_t>(splits, (p.max_blocks + kMinChunk - 1) / kMinChunk);
+    const int64_t each = std::min<int64_t>(splits, most_pieces(p.max_blocks));
     const int64_t pieces = std::min<int64_t>({(int64_t)q.batch * each, wanted + q.batch, limit});
     q.most = (int32_t)pieces;
     q.wanted = (uint32_t)wanted;
