@@ -538,8 +538,9 @@ int pbe_gather_kv_mxfp4(const void* key_pool, uint64_t key_pool_bytes, const voi
  * used. A length of 0 gives zeros; a negative one, one that needs more than
  * max_blocks_per_seq blocks, and a block id outside the pools give the
  * sequence NaN; a NaN group in a token's K or V reaches the heads that read
- * it, as does a NaN or an infinity in the queries; V values of 2^128 and more
- * (scale bytes 253 and 254, which the writer does not store) give NaN.
+ * it, as does a NaN or an infinity in the queries. Values of 2^128 and more
+ * (scale bytes 253 and 254, which the writer does not store) count as
+ * infinities: in V they give NaN, in K NaN or a weight of zero.
  * A batch's blocks are cut into pieces of one length, at most batch * splits of
  * them and 1,024 of a sequence, whatever the lengths (the kernel looks at
  * them); splits = 1 leaves every sequence whole. So the order of a sequence's

@@ -8,14 +8,14 @@
 //    take them, so one load instruction reads all of K, and one all of V. The
 //    next tile's K is asked for when the scores have used this one's, its V
 //    after the values' products.
-//  - scores, transposed, on the codes as they are: one scaled 16x16x128 MFMA
-//    takes a block's 16 keys (A, E2M1 with the pages' own E8M0 scales) and the
-//    query heads of the KV head (B, E4M3, columns). A query is split into two
-//    E4M3 numbers of four significant bits, which hold a BF16 number's eight
-//    exactly down to 2^-13 of the head's largest, and to 2^-21 of it below that;
-//    a second MFMA adds the lower parts. The MFMA sums a
-//    group's products to about 2^-17 of their magnitudes (measured), which is
-//    what a score is good for. Lane (g, j) ends with tokens 4g..4g+3 of head j.
+//  - scores, transposed: lane (g, i) holds key i's dims of quarter g, which the
+//    scaled converters make BF16 of, exactly; each MFMA takes eight of every quarter
+//    (A) and the same of the query heads of the KV head (B, columns), as they are.
+//    So terms are exact and sums those of the BF16 MFMA, FP32 (measured: within
+//    2^-22 of the terms' magnitudes). The scaled MFMA, which would take the codes as
+//    they are, wants the queries in eight bits or less and sums terms of unlike
+//    size within 2^-12 alone (measured). Lane (g, j) ends with tokens 4g..4g+3 of
+//    head j.
 //  - values: lane (g, i) holds tokens 4g..4g+3 of column i, the D/16 dims
 //    [i*D/16, (i+1)*D/16). The scaled converters make a BF16 pair of a byte, an
 //    even and an odd dim of one token, exactly. Both count as terms of one
@@ -158,14 +158,12 @@ __device__ __forceinline__ Piece find_piece(const Mxfp4DecodeParams& p, int z, i
   return r;
 }
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
 // A lane's part of one tile.
 template <int D>
 struct Tile {
   static constexpr int W = D / 32;  // words of codes
   uint32_t k[kTile][W], v[kTile][W];
-  uint32_t ks[kTile];  // scale bytes of its key's quarter, of four keys
+  uint32_t ks[kTile];  // scale bytes of its quarter, of four keys
   uint32_t vs[kTile];  // scale bytes of its four tokens' columns
 };
 
@@ -189,28 +187,6 @@ __device__ __forceinline__ void token_pairs(const uint32_t (&v)[D / 32], uint32_
   }
 }
 
-// Four BF16 dims of a query head (two pairs) as E4M3 numbers hi + lo: value =
-// hi * 2^(byte - 127) + lo * 2^(byte - 4 - 127), byte as split_byte() gives it.
-struct SplitQuery {
-  uint32_t hi, lo;
-};
-// `amax`: FP32 bits of the head's largest magnitude, which hi takes to [2^7, 2^8).
-// Both parts' scales stay within a byte.
-__device__ __forceinline__ uint32_t split_byte(uint32_t amax) { return (uint32_t)max((int)(amax >> 23) - 7, 4); }
-__device__ __forceinline__ SplitQuery split_query(u32x2 x, uint32_t byte) {
-  typedef short s16x2 __attribute__((ext_vector_type(2)));
-  const float hi_scale = mx_scale(byte), lo_scale = mx_scale(byte - 4);
-  const uint32_t a = x.x, b = x.y;
-  s16x2 hi = {0, 0}, lo = {0, 0};
-  hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, __builtin_bit_cast(mx_bf16x2, a), hi_scale, false);
-  hi = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(hi, __builtin_bit_cast(mx_bf16x2, b), hi_scale, true);
-  const uint32_t h = __builtin_bit_cast(uint32_t, hi);
-  const f32x2 ha = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(h, hi_scale, false), hb = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(h, hi_scale, true);
-  lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, bf16_lo(a) - ha[0], bf16_hi(a) - ha[1], lo_scale, false);
-  lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, bf16_lo(b) - hb[0], bf16_hi(b) - hb[1], lo_scale, true);
-  return {h, __builtin_bit_cast(uint32_t, lo)};
-}
-
 // kWide: more than 8 query heads per KV head. The wide form holds for any number
 // of them, in 151 registers and three waves a SIMD for 119 and four; for up to
 // eight it takes, A / B / C / D above, 19.2 / 34.5 / 13.9 / 18.2 us, this one 18.3
@@ -226,8 +202,6 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
   constexpr int PITCH = D + 4;
   __shared__ __attribute__((aligned(16))) float lds_o[kWaves][HEADS][PITCH];
   __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
-  __shared__ __attribute__((aligned(16))) uint32_t lds_q[2][HEADS][D / 4];  // the query heads' upper and lower parts
-  __shared__ uint32_t lds_byte[HEADS];
   __shared__ int lds_last;
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -249,17 +223,15 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
   const int32_t* table = p.tables + (int64_t)b * p.max_blocks;
   auto ids_of = [&](int tile) { return table[min(first + (tile + lane / kTile) * STEP + lane % kTile, p.max_blocks - 1)]; };
   int32_t window = ids_of(0);
-  // The queries, four dims a thread, D/4 threads a head: asked for before the
-  // first tile, as loads come back in their order.
-  constexpr int ROUNDS = (HEADS * D / 4 + kThreads - 1) / kThreads;
+  // B of the scores: lane (g, j) holds head j's dims of quarter g, as the keys lie.
+  // Asked for before the first tile, as loads come back in their order; every wave
+  // reads its own, which took no longer than one reading for all of them.
   const int64_t row0 = (int64_t)b * p.q_heads + (int64_t)h * p.group;  // the KV head's first query head
-  u32x2 q_in[ROUNDS];
+  const int head = kWide ? j : j % 8;
+  u32x4 q[W];
 #pragma unroll
-  for (int n = 0; n < ROUNDS; ++n) {
-    const int unit = n * kThreads + (int)threadIdx.x, hj = unit / (D / 4);
-    q_in[n] = *reinterpret_cast<const u32x2*>(p.q + (row0 + min(hj, p.group - 1)) * D + 4 * (unit % (D / 4)));
-    if (hj >= p.group) q_in[n] = u32x2{0u, 0u};
-  }
+  for (int n = 0; n < W; ++n)
+    q[n] = *reinterpret_cast<const u32x4*>(p.q + (row0 + min(head, p.group - 1)) * D + g * (D / 4) + 8 * n);
 
   // Lane l holds the id of block l % kTile of the wave's tile l / kTile of
   // AHEAD; -1 for one past the piece's end, or outside the pools.
@@ -270,7 +242,8 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
   };
   check_ids(0);
   const uint32_t code_at = lane * (D / 8);
-  const uint32_t key_scales_at = (D == 128 ? g : g / 2) * kMxTokens + (j & ~3), ks_shift = 8 * (j & 3);
+  // A turn by ks_turn takes key j's scale byte to the exponent's bits.
+  const uint32_t key_scales_at = (D == 128 ? g : g / 2) * kMxTokens + (j & ~3), ks_turn = 8 * (j & 3) + 9;
   const uint32_t value_scales_at = (D == 128 ? j / 4 : j / 8) * kMxTokens + 4 * g;
   // Where a tile's blocks lie: bytes of codes from a pool's start, a 16th of
   // that of scales. A block that is none is read from the pools' first: what a
@@ -328,40 +301,10 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
   const int z0 = z - s;  // the sequence's first piece
   const gptr<uint64_t> ticket = (gptr<uint64_t>)p.tickets + (int64_t)z0 * p.kv_heads + h;
   if (pieces > 1 && threadIdx.x == 0) open_ticket(ticket, p.tag);
-  // The queries, split once for the workgroup.
+  if (head >= p.group) {
 #pragma unroll
-  for (int n = 0; n < ROUNDS; ++n) {
-    const int unit = n * kThreads + (int)threadIdx.x, hj = unit / (D / 4), at = unit % (D / 4);
-    if (hj >= HEADS) break;
-    const u32x2 x = q_in[n];
-    uint32_t amax = max(max(x.x & 0x7fff0000u, (x.x << 16) & 0x7fff0000u), max(x.y & 0x7fff0000u, (x.y << 16) & 0x7fff0000u));
-    amax = quad_max(amax);
-    amax = max(amax, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)amax, 0x141, 0xf, 0xf, false));
-    amax = max(amax, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)amax, 0x140, 0xf, 0xf, false));
-    if constexpr (D == 128) amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16, 64));
-    // an infinity or a NaN: the NaN scale
-    const bool fine = amax < 0x7f800000u;
-    const uint32_t byte = split_byte(amax);
-    const SplitQuery q = split_query(fine ? x : u32x2{0u, 0u}, byte);
-    lds_q[0][hj][at] = q.hi;
-    lds_q[1][hj][at] = q.lo;
-    if (at == 0) lds_byte[hj] = fine ? byte : 0xffu;
+    for (int n = 0; n < W; ++n) q[n] = u32x4{0u, 0u, 0u, 0u};
   }
-  __syncthreads();
-  // B of the scores: the scaled MFMA takes terms [16g, 16g + 16) and [64 + 16g,
-  // +16) of column j from lane (g, j), where A's lane (g, i) has terms [32g,
-  // +32): its key's dims in order, or (D = 64) 16 of them and 16 zeros.
-  const int head = kWide ? j : j % 8;
-  i32x8 q[2];
-#pragma unroll
-  for (int part = 0; part < 2; ++part)
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(&lds_q[part][head][(D == 128 ? 64 * half + 16 * g : 32 * half + 16 * (g / 2)) / 4]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) q[part][4 * half + e] = D == 128 || g % 2 == 0 ? (int)x[e] : 0;
-    }
-  const int hi_byte = (int)lds_byte[head], lo_byte = hi_byte == 0xff ? 0xff : hi_byte - 4;
   // Which half of a BF16 pair (p, p) meets this lane's column.
   const uint32_t parity = kWide || j >= 8 ? 0xffff0000u : 0x0000ffffu;
 
@@ -386,13 +329,11 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
     f32x4 x[kTile];
 #pragma unroll
     for (int u = 0; u < kTile; ++u) {
-      i32x8 a = {};
-#pragma unroll
-      for (int e = 0; e < W; ++e) a[e] = (int)r.k[u][e];
-      const int ks = (int)(r.ks[u] >> ks_shift);  // the MFMA reads the lowest byte
+      const float ks = __uint_as_float(__builtin_amdgcn_alignbit(r.ks[u], r.ks[u], ks_turn));  // the converters read the exponent bits alone
       x[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      x[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[0], x[u], 4, 0, 0, ks, 0, hi_byte);
-      x[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q[1], x[u], 4, 0, 0, ks, 0, lo_byte);
+#pragma unroll
+      for (int n = 0; n < W; ++n)
+        x[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, mx_values(r.k[u][n], ks)), __builtin_bit_cast(bf16x8, q[n]), x[u], 0, 0, 0);
     }
     if constexpr (kPart) {
       // Tokens past the end: no score, and zeros for values that may be NaN.

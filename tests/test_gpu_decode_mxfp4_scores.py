@@ -1,0 +1,84 @@
+"""Scores of pbe_paged_decode_mxfp4 whose terms differ by many powers of two:
+queries with one dim far above the others. The bound is that of
+test_gpu_decode_mxfp4 (products of BF16 numbers are exact in FP32, sums take a
+rounding of 2^-24 per term); where the large dim meets zero codes, or keys as
+small as it is large, the terms' magnitudes, and the bound with them, stay what
+they are without it."""
+import numpy as np
+import pytest
+
+from oracle import mxfp4 as M
+from tests.conftest import say
+from tests.test_gpu_decode_mxfp4 import T, Case
+
+pytestmark = pytest.mark.gpu
+
+
+def set_code(c, dim, code):
+    """The code of one dim of every key."""
+    pool = c.views()[0]
+    at = M.code_at(np.arange(c.blocks * T), c.heads, c.dim, False)[..., dim].ravel()
+    pool[at] = (pool[at] & 0x0F) | (code << 4) if dim % 2 else (pool[at] & 0xF0) | code
+
+
+def key_scales(c):
+    """The scale bytes of all keys' groups: [slots][heads][groups], and where they lie."""
+    at = M.scale_at(np.arange(c.blocks * T), c.heads, c.dim)
+    return at, c.views()[2]
+
+
+def set_query(torch, c, dims, factor):
+    c.q[..., dims] = (c.q[..., dims].double() * factor).to(torch.bfloat16)
+    c.q_host = c.q.double().cpu().numpy()
+
+
+LENS = [2, 3, 2, 17, 200, 2, 700]
+
+
+@pytest.mark.parametrize("up", [14, 17, 20, 40, 100])
+@pytest.mark.parametrize("heads,group,dim", [(2, 7, 64), (2, 6, 128), (1, 12, 128), (1, 9, 64)])
+def test_a_large_query_dim_meets_zeros(torch_cuda, heads, group, dim, up):
+    torch = torch_cuda
+    say(f"decode mxfp4 scores: zeros at a dim 2^{up} above the others, H={heads}x{group} D={dim}")
+    c = Case(torch, LENS, heads, group, dim, seed=up)
+    set_code(c, dim - 3, 0)
+    c.upload()
+    set_query(torch, c, dim - 3, 2.0 ** up)
+    for splits in (1, 8):
+        c.call(splits)
+        c.check()
+
+
+@pytest.mark.parametrize("up", [14, 20, 60])
+@pytest.mark.parametrize("heads,group,dim", [(2, 7, 64), (2, 6, 128), (1, 12, 128)])
+def test_a_large_group_of_query_dims_meets_small_keys(torch_cuda, heads, group, dim, up):
+    torch = torch_cuda
+    say(f"decode mxfp4 scores: a group 2^{up} above the others, H={heads}x{group} D={dim}")
+    c = Case(torch, LENS, heads, group, dim, seed=up + 1)
+    at, scales = key_scales(c)
+    first = at[..., 0]
+    scales[first] = np.where(scales[first] == 255, 255, np.maximum(scales[first].astype(int) - up, 0))
+    c.upload()
+    set_query(torch, c, slice(0, 32), 2.0 ** up)
+    for splits in (1, 8):
+        c.call(splits)
+        c.check()
+
+
+@pytest.mark.parametrize("up", [8, 12, 16])
+@pytest.mark.parametrize("heads,group,dim", [(2, 7, 64), (2, 6, 128), (1, 12, 128)])
+def test_a_large_term_that_all_scores_share(torch_cuda, heads, group, dim, up):
+    """It leaves the weights as they are, up to its rounding in the scores."""
+    torch = torch_cuda
+    say(f"decode mxfp4 scores: 2^{up} in all of them, H={heads}x{group} D={dim}")
+    c = Case(torch, [2] * 40 + [5, 300], heads, group, dim, seed=up + 2)
+    set_code(c, 5, 2)   # 1.0
+    at, scales = key_scales(c)
+    first = at[..., 0]
+    scales[first] = np.where(scales[first] == 255, 255, 127)
+    c.upload()
+    c.q[..., 5] = 1.0
+    set_query(torch, c, 5, 2.0 ** up)
+    for splits in (1, 8):
+        c.call(splits)
+        c.check()
