@@ -16,6 +16,9 @@
 //    they are, wants the queries in eight bits or less and sums terms of unlike
 //    size within 2^-12 alone (measured). Lane (g, j) ends with tokens 4g..4g+3 of
 //    head j.
+//  - softmax: every weight is 2^((score - largest) * scale), of the difference, so the
+//    largest score's is 1 however large it is. (The score times the scale less the
+//    largest's, in one multiply-add, is off by the rounding of that product.)
 //  - values: lane (g, i) holds tokens 4g..4g+3 of column i, the D/16 dims
 //    [i*D/16, (i+1)*D/16). The scaled converters make a BF16 pair of a byte, an
 //    even and an odd dim of one token, exactly. Both count as terms of one
@@ -362,7 +365,6 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
       for (int i = 0; i < 4; ++i) top = fmaxf(top, x[u][i]);
     const float mn = fmaxf(m, group_max4(top));
     const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * p.scale);
-    const float base = -mn * p.scale;
     uint32_t pb[kTile][4];
 #pragma unroll
     for (int u = 0; u < kTile; ++u)
@@ -370,7 +372,7 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
       for (int i = 0; i < 4; ++i) {
         // a token past the end gets 0, or NaN where its head has no other score
         // than -infinity or NaN and is NaN whatever this token adds
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][i], p.scale, base));
+        const float e = __builtin_amdgcn_exp2f((x[u][i] - mn) * p.scale);
         pb[u][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{e, e}), mx_bf16x2));
       }
     m = mn;
@@ -414,7 +416,7 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
 
   // The waves' results into one. Lane (g, j) holds dims (4g + r)*D/16 + 2n + (its parity).
   if (g == 0) {  // lanes j and j + 8 hold the same
-    lds_m[w][head] = m * p.scale;
+    lds_m[w][head] = m;
     lds_l[w][head] = bad ? __builtin_nanf("") : l[0];
   }
 #pragma unroll
@@ -450,7 +452,7 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
-      const float li = lds_l[i][hj], wt = li > 0.f ? __builtin_amdgcn_exp2f(lds_m[i][hj] - top) : 0.f;
+      const float li = lds_l[i][hj], wt = li > 0.f ? __builtin_amdgcn_exp2f((lds_m[i][hj] - top) * p.scale) : 0.f;
       sum += li != li ? li : li * wt;
       if (wt > 0.f) o += *reinterpret_cast<const f32x4*>(&lds_o[i][hj][4 * col]) * wt;
     }
@@ -486,13 +488,13 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
         float mn = top;
 #pragma unroll
         for (int i = 0; i < kJoin; ++i) mn = fmaxf(mn, s0 + i < pieces ? ml[i][0] : -INFINITY);
-        const float keep = sum > 0.f ? __builtin_amdgcn_exp2f(top - mn) : 0.f;
+        const float keep = sum > 0.f ? __builtin_amdgcn_exp2f((top - mn) * p.scale) : 0.f;
         sum = sum != sum ? sum : sum * keep;
         o = keep > 0.f ? o * keep : f32x4{0.f, 0.f, 0.f, 0.f};
         top = mn;
 #pragma unroll
         for (int i = 0; i < kJoin; ++i) {  // a NaN sum stays; a result of weight 0 is left out whatever it holds
-          const float li = ml[i][1], wt = li > 0.f ? __builtin_amdgcn_exp2f(ml[i][0] - mn) : 0.f;
+          const float li = ml[i][1], wt = li > 0.f ? __builtin_amdgcn_exp2f((ml[i][0] - mn) * p.scale) : 0.f;
           sum += li != li ? li : li * wt;
           if (wt > 0.f) o += x[i] * wt;
         }

@@ -82,3 +82,28 @@ def test_a_large_term_that_all_scores_share(torch_cuda, heads, group, dim, up):
     for splits in (1, 8):
         c.call(splits)
         c.check()
+
+
+@pytest.mark.parametrize("up", [0, 30, 36, 60, 100])
+@pytest.mark.parametrize("heads,group,dim", [(2, 7, 64), (2, 6, 128), (1, 12, 128)])
+def test_equal_scores_of_any_size_give_the_mean(torch_cuda, heads, group, dim, up):
+    """Every key is the same, so all weights are: the output is the values' mean, off
+    by half a step of BF16 and (n / 32 + 64) roundings of 2^-23 of the sums."""
+    torch = torch_cuda
+    say(f"decode mxfp4 scores: equal ones of about 2^{up}, H={heads}x{group} D={dim}")
+    c = Case(torch, [1, 2, 17, 100, 500, 900], heads, group, dim, seed=up + 3)
+    for d in range(dim):
+        set_code(c, d, 1 + d % 7)
+    at, scales = key_scales(c)
+    scales[at] = np.where(scales[at] == 255, 255, 127)
+    c.upload()
+    set_query(torch, c, slice(0, dim), 2.0 ** up)
+    still = np.zeros_like(c.q_host)
+    o, _, size, _ = M.decode(still, c.views(), c.tables, c.lens, heads)
+    n = np.array(c.lens)[:, None, None]
+    bound = 2.0 ** -8 * np.abs(o) + (n / 32 + 64) * 2.0 ** -23 * size
+    for splits in (1, 8):
+        c.out.fill_(5.0)
+        c.call(splits)
+        torch.cuda.synchronize()
+        assert (np.abs(c.out.double().cpu().numpy() - o) <= bound).all()
