@@ -540,7 +540,9 @@ int pbe_gather_kv_mxfp4(const void* key_pool, uint64_t key_pool_bytes, const voi
  * sequence NaN; a NaN group in a token's K or V reaches the heads that read
  * it, as does a NaN or an infinity in the queries. Values of 2^128 and more
  * (scale bytes 253 and 254, which the writer does not store) count as
- * infinities: in V they give NaN, in K NaN or a weight of zero.
+ * infinities: in V they give NaN, in K NaN or a weight of zero. So does a q . k
+ * beyond FP32's range: -infinity takes a token's weight to zero, +infinity, or
+ * -infinity for all tokens, the head to NaN.
  * A batch's blocks are cut into pieces of one length, at most batch * splits of
  * them and 1,024 of a sequence, whatever the lengths (the kernel looks at
  * them); splits = 1 leaves every sequence whole. So the order of a sequence's

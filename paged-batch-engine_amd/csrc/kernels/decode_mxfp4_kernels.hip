@@ -364,15 +364,16 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, x[u][i]);
     const float mn = fmaxf(m, group_max4(top));
-    const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * p.scale);
+    // While all scores are -infinity (they may pass FP32's range) the weights are
+    // zeros, not 2^(infinity - infinity): a later tile, wave or piece can have others.
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f((m - base) * p.scale);
     uint32_t pb[kTile][4];
 #pragma unroll
     for (int u = 0; u < kTile; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        // a token past the end gets 0, or NaN where its head has no other score
-        // than -infinity or NaN and is NaN whatever this token adds
-        const float e = __builtin_amdgcn_exp2f((x[u][i] - mn) * p.scale);
+        const float e = __builtin_amdgcn_exp2f((x[u][i] - base) * p.scale);
         pb[u][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{e, e}), mx_bf16x2));
       }
     m = mn;
@@ -429,11 +430,12 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
   }
   __syncthreads();
   // From here on a thread holds four dims of a head, more than one after another
-  // where the heads have more dims than the workgroup threads.
+  // where the heads have more dims than the workgroup threads. Of tokens that all
+  // score -infinity there is no softmax.
   auto finish = [&](int hj, int col, const f32x4& o, float sum) {
     uint16_t e[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = to_bf16(sum != sum ? sum : sum > 0.f ? o[i] / sum : 0.f);
+    for (int i = 0; i < 4; ++i) e[i] = to_bf16(sum != sum ? sum : sum > 0.f ? o[i] / sum : seq > 0 ? __builtin_nanf("") : 0.f);
     *reinterpret_cast<u32x2*>(p.out + (row0 + hj) * D + 4 * col) = u32x2{e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16};
   };
   // The sequence's partial results [piece][query head]; a piece's bytes times

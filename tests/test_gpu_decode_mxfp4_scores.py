@@ -107,3 +107,59 @@ def test_equal_scores_of_any_size_give_the_mean(torch_cuda, heads, group, dim, u
         c.call(splits)
         torch.cuda.synchronize()
         assert (np.abs(c.out.double().cpu().numpy() - o) <= bound).all()
+
+
+BEYOND = [("first", lambda n: [0]), ("first tile", lambda n: range(0, 32)), ("first tiles of all waves", lambda n: range(0, 128)),
+          ("all but the last", lambda n: range(0, n - 1)), ("every other block", lambda n: [t for t in range(n) if t // T % 2 == 0]),
+          ("last", lambda n: [n - 1])]
+
+
+def beyond(torch, lens, heads, group, dim, tokens, sign=8):
+    """Queries and keys whose products pass FP32's range at some tokens, and are
+    zero at that dim for the others: what the oracle says of these, but for the
+    magnitudes of their scores."""
+    c = Case(torch, lens, heads, group, dim, seed=dim + len(lens))
+    set_code(c, 7, 0)
+    pool, scales = c.views()[0], c.views()[2]
+    for b, n in enumerate(lens):
+        t = np.array([x for x in tokens(n) if x < n], np.int64)
+        slots = c.tables[b, t // T].astype(np.int64) * T + t % T
+        at = M.code_at(slots, heads, dim, False)[..., :32]
+        pool[at] = 0
+        pool[at[..., 7]] = (6 | sign) << 4   # 4 or -4, an odd dim: the high half
+        scales[M.scale_at(slots, heads, dim)[..., 0]] = 252
+    c.upload()
+    c.q[..., 7] = 2.0 ** 20
+    c.q_host = c.q.double().cpu().numpy()
+    o, spread, size, _ = M.decode(c.q_host, c.views(), c.tables, lens, heads)
+    q = c.q_host.copy()
+    q[..., 7] = 0
+    return c, (o, spread, size, M.decode(q, c.views(), c.tables, lens, heads)[3])
+
+
+@pytest.mark.parametrize("which,tokens", BEYOND, ids=[w for w, _ in BEYOND])
+@pytest.mark.parametrize("heads,group,dim", [(2, 7, 64), (2, 6, 128), (1, 12, 128)])
+def test_scores_below_all_numbers_have_no_weight(torch_cuda, heads, group, dim, which, tokens):
+    torch = torch_cuda
+    say(f"decode mxfp4 scores: -infinity at {which}, H={heads}x{group} D={dim}")
+    c, want = beyond(torch, [2, 33, 150, 700, 1100], heads, group, dim, tokens)
+    for splits in (1, 2, 16):
+        c.out.fill_(5.0)
+        c.call(splits)
+        c.check(want=want, skip=[b for b, n in enumerate(c.lens) if len(set(tokens(n)) & set(range(n))) == n])
+
+
+def test_no_softmax_of_nothing_but_infinities(torch_cuda):
+    torch = torch_cuda
+    say("decode mxfp4 scores: all -infinity, or one +infinity")
+    for sign, tokens in ((8, lambda n: range(n)), (0, lambda n: [n // 2]), (0, lambda n: range(n))):
+        c, _ = beyond(torch, [1, 40, 700], 2, 6, 128, tokens, sign)
+        for splits in (1, 8):
+            c.out.fill_(5.0)
+            c.call(splits)
+            torch.cuda.synchronize()
+            assert torch.isnan(c.out.float()).all()
+    c, _ = beyond(torch, [0, 0], 2, 6, 128, lambda n: [])
+    c.call(1)
+    torch.cuda.synchronize()
+    assert (c.out == 0).all()
