@@ -526,8 +526,9 @@ int pbe_gather_kv_mxfp4(const void* key_pool, uint64_t key_pool_bytes, const voi
 
 /* Decode reader: paged attention for one query token per sequence over MXFP4
  * pages, as pbe_paged_decode_pools reads BF16 and FP8 ones: softmax(q . k /
- * sqrt(head_dim)) v, FP32 sums and softmax, probabilities rounded to BF16 for
- * the product with v and summed as rounded, BF16 outputs. pool_bytes and
+ * sqrt(head_dim)) v, exact products of BF16 queries and 4-bit keys, FP32 sums
+ * and softmax, probabilities within 2^-15 for the product with v (two BF16 parts
+ * each, as there), BF16 outputs. pool_bytes and
  * scale_pool_bytes are the bytes addressable from each pointer; q_heads a
  * multiple of kv_heads, at most 16 query heads per KV head.
  *

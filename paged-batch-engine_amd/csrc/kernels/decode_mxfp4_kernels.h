@@ -26,7 +26,7 @@ struct Mxfp4DecodeParams {
   // Set by launch_paged_decode_mxfp4.
   int32_t most;               // pieces there is room for; batch: every sequence whole
   uint32_t wanted;            // pieces that fill the chip
-  int32_t min_chunk;          // blocks of a piece, at least
+  int32_t min_chunk;          // blocks of a piece, at least, before a sequence's are made even
   FastDiv by_eight;           // workgroups of eight pieces
   float* part_acc;            // [most][q_heads][dim]: results of pieces
   float* part_ml;             // [most][q_heads][2]: maximum, sum

@@ -35,17 +35,20 @@
 //    finishes last joins their results, in their order; they are written and
 //    read at agent scope (written through, read past the XCD's own L2), so no
 //    L2 is written back: a workgroup waits for its stores, then takes a ticket.
-//  - probabilities are rounded to BF16 for that product, and the sum they are
-//    divided by is of the rounded ones: each weight is off by at most 2^-8 of
-//    itself, and they still add up to one.
+//  - a probability goes into that product as two BF16 numbers, its top eight bits
+//    and the next eight, within 2^-15 of the FP32 one; the sum they are divided by is
+//    of the FP32 ones. With one BF16 number each, the outputs of 64 x 5,040 tokens lay
+//    0.0014 of their norm from those of FP32 weights, now 0.0001 (rounding them to
+//    BF16 takes 0.0016).
 //
-// Bound by the pages' bytes and, for few of them, by the chain of dependent reads
-// (arguments, lengths, ids, pages, ticket, results). Calls back to back in a
-// graph, on pages that stay: 64 x 5,040 tokens of 2 x 128 18.3 us, 4.8 TB/s of the
-// bytes needed; 64 mixed up to 32,768 of 4 x 128 32.8 us, 4.9 TB/s; 1 x 5,040 of 2
-// x 64 7.9 us. Of the first, calls that end after each part take: launch 2.2, its
-// piece found 2.7, queries split 3.6, all but the tiles and the join 4.7, all but
-// the join 16.5.
+// Bound by the pages' bytes and the conversions and products of each block, side by
+// side, and for few blocks by the chain of dependent reads (arguments, lengths, ids,
+// pages, ticket, results). Calls back to back in a graph, on pages that stay and so
+// lie partly in the memory-side cache / on 2 GB of pages in turn: 64 x 5,040 tokens
+// of 2 x 128 19.4 / 22.6 us (4.5 / 3.9 TB/s of the bytes needed); 64 mixed up to
+// 32,768 of 4 x 128 34.1 / 41.0 us (4.7 / 3.9); 1 x 5,040 of 2 x 64 7.9 us either
+// way. Of the first, on pages that stay, calls that end after each part take: launch
+// 2.6, its piece found 2.6, all but the tiles and the join 4.4, all but the join 18.0.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -61,18 +64,20 @@ namespace pbe {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
-// Below, in us: A 64 x 5,040 tokens of 2 x 128, B 64 mixed up to 32,768 of 4 x 128,
-// C 150 mixed up to 3,000 of 2 x 64, D 256 mixed up to 600 of 4 x 128.
-// Blocks of a wave's tile. A / B / C / D with tiles of 1: 18.9 / 31.5 / 14.2 / 14.2,
-// of 2: 18.3 / 32.8 / 13.0 / 13.6, of 4 (14 registers spill): 20.0 / 34.9 / 12.6 /
-// 16.1. Half the workgroups of eight waves: 19.7 / 34.6 / 14.7 / 18.4.
+// Below, in us, on pages that stay: A 64 x 5,040 tokens of 2 x 128, B 64 mixed up to
+// 32,768 of 4 x 128, C 150 mixed up to 3,000 of 2 x 64, D 256 mixed up to 600 of 4 x
+// 128. As it is: 19.8 / 34.3 / 13.7 / 15.7.
+// Blocks of a wave's tile. A / B / C / D with tiles of 1: 21.3 / 37.5 / 14.4 / 16.9,
+// of 4 (registers spill): 20.7 / 36.3 / 13.6 / 17.9. Half the workgroups of eight
+// waves: 19.8 / 39.5 / 15.7 / 19.9.
 constexpr int kTile = 2;
 // Blocks of a piece that joining is worth: two tiles for every wave. With one, 64
-// mixed up to 250 of 2 x 128 took 6.6 us for 4.7, 8 mixed up to 2,000 of 8 x 128
-// 8.8 for 8.1, 1 x 600 of 2 x 128 6.7 for 7.3, A to D the same.
+// mixed up to 250 of 2 x 128 took 6.5 us for 4.9, 8 mixed up to 2,000 of 8 x 128
+// 8.9 for 8.1, 1 x 600 of 2 x 128 6.7 for 7.4, A to D the same. Pieces are made even
+// after that, so that those of a sequence little longer hold little more than half.
 constexpr int kMinChunk = 2 * kTile * kWaves;
-// Wanted workgroups per compute unit. A / B / C / D with 1: 18.7 / 32.9 / 15.0 /
-// 13.5, 2: 18.3 / 32.8 / 13.0 / 13.6, 3: 20.9 / 34.2 / 14.3 / 19.1.
+// Wanted workgroups per compute unit. A / B / C / D with 1: 21.1 / 39.7 / 15.7 /
+// 15.8, 3: 22.3 / 38.1 / 15.2 / 20.2.
 constexpr int kPiecesPerUnit = 2;
 constexpr int kAgent = 0x10;  // buffer access policy: agent scope
 static_assert(kMxDecodeMaxSplits < (1 << kTicketBits), "arrivals fit the ticket");
@@ -191,9 +196,8 @@ __device__ __forceinline__ void token_pairs(const uint32_t (&v)[D / 32], uint32_
 }
 
 // kWide: more than 8 query heads per KV head. The wide form holds for any number
-// of them, in 151 registers and three waves a SIMD for 119 and four; for up to
-// eight it takes, A / B / C / D above, 19.2 / 34.5 / 13.9 / 18.2 us, this one 18.3
-// / 32.8 / 13.0 / 13.6.
+// of them, in 156 registers and three waves a SIMD for 122 and four; for up to
+// eight it takes, A / B / C / D above, 22.8 / 40.6 / 15.1 / 20.5 us.
 template <int D, bool kWide>
 __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_kernel(const Mxfp4DecodeParams p) {
   constexpr int W = D / 32;                  // words of K (and of V) codes per lane and block
@@ -212,7 +216,7 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
   // A piece's KV heads go to one XCD, eight pieces side by side: two to four heads'
   // scales share a cache line, which several XCDs would read each for itself (64
   // x 5,040 tokens of 2 x 128 fetch 90.6 MB of the 88.2 that they need, in the order
-  // of the heads 96.0; 18.3 us and 18.9).
+  // of the heads 96.0; 19.4 us and 20.9).
   const int eight = (int)fast_div(blockIdx.x, p.by_eight), in_eight = (int)blockIdx.x - eight * (int)p.by_eight.d;
   const int z = eight * (int)kXcds + in_eight % (int)kXcds, h = in_eight / (int)kXcds;
   const Piece piece = find_piece(p, z, lane);
@@ -308,13 +312,12 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
 #pragma unroll
     for (int n = 0; n < W; ++n) q[n] = u32x4{0u, 0u, 0u, 0u};
   }
-  // Which half of a BF16 pair (p, p) meets this lane's column.
-  const uint32_t parity = kWide || j >= 8 ? 0xffff0000u : 0x0000ffffu;
+  // The upper bytes of a probability's part, in the half of a BF16 pair that meets
+  // this lane's column, and zeros in the other.
+  const uint32_t to_mine = kWide || j >= 8 ? 0x03020c0cu : 0x0c0c0302u;
 
-  float m = -INFINITY;  // of head j: its largest score
+  float m = -INFINITY, l = 0.f;  // of head j: its largest score, and the sum of this lane's probabilities
   f32x4 acc[PARTS][NT];
-  f32x4 l = {0.f, 0.f, 0.f, 0.f};  // its sum of probabilities, by the MFMA against ones (four times the same)
-  const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
 #pragma unroll
   for (int x = 0; x < PARTS; ++x)
 #pragma unroll
@@ -368,18 +371,17 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
     // zeros, not 2^(infinity - infinity): a later tile, wave or piece can have others.
     const float base = mn == -INFINITY ? 0.f : mn;
     const float alpha = __builtin_amdgcn_exp2f((m - base) * p.scale);
-    uint32_t pb[kTile][4];
+    float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < kTile; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float e = __builtin_amdgcn_exp2f((x[u][i] - base) * p.scale);
-        pb[u][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{e, e}), mx_bf16x2));
+        x[u][i] = __builtin_amdgcn_exp2f((x[u][i] - base) * p.scale);
+        sum += x[u][i];
       }
     m = mn;
+    l = l * alpha + sum;
     if (__ballot(alpha != 1.f) != 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) l[i] *= alpha;
 #pragma unroll
       for (int y = 0; y < PARTS; ++y)
 #pragma unroll
@@ -394,15 +396,27 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
       token_pairs<D, 1>(r.v[u], r.vs[u], c[1]);
       token_pairs<D, 2>(r.v[u], r.vs[u], c[2]);
       token_pairs<D, 3>(r.v[u], r.vs[u], c[3]);
-      const u32x4 even{pb[u][0] & 0xffffu, pb[u][1] & 0xffffu, pb[u][2] & 0xffffu, pb[u][3] & 0xffffu};
-      const u32x4 kept{pb[u][0] & parity, pb[u][1] & parity, pb[u][2] & parity, pb[u][3] & parity};
-      l = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(bf16x8, kept), l, 0, 0, 0);
+      // hi keeps a probability's top eight significant bits, lo the next eight.
+      u32x4 hi, lo, hi_even, lo_even;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const bf16x8 a = __builtin_bit_cast(bf16x8, u32x4{c[0][n], c[1][n], c[2][n], c[3][n]});
-        acc[0][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, kept), acc[0][n], 0, 0, 0);
-        if constexpr (kWide) acc[PARTS - 1][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, even), acc[PARTS - 1][n], 0, 0, 0);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t e = __float_as_uint(x[u][i]);
+        const uint32_t rest = __float_as_uint(x[u][i] - __uint_as_float(e & 0xffff0000u));
+        hi[i] = __builtin_amdgcn_perm(e, e, to_mine);
+        lo[i] = __builtin_amdgcn_perm(rest, rest, to_mine);
+        if constexpr (kWide) hi_even[i] = e >> 16, lo_even[i] = rest >> 16;
       }
+      // All products of hi before those of lo, so that none waits for the one before
+      // it (64 x 5,040 tokens of 2 x 128: 19.0 us, next to each other 20.6).
+#pragma unroll
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const bf16x8 a = __builtin_bit_cast(bf16x8, u32x4{c[0][n], c[1][n], c[2][n], c[3][n]});
+          acc[0][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, part ? lo : hi), acc[0][n], 0, 0, 0);
+          if constexpr (kWide)
+            acc[PARTS - 1][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, part ? lo_even : hi_even), acc[PARTS - 1][n], 0, 0, 0);
+        }
     }
     if constexpr (kNext) load_values(r);
   };
@@ -416,9 +430,10 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
   else if (tiles > 0) compute(tiles - 1, no, no);
 
   // The waves' results into one. Lane (g, j) holds dims (4g + r)*D/16 + 2n + (its parity).
+  l = group_sum4(l);
   if (g == 0) {  // lanes j and j + 8 hold the same
     lds_m[w][head] = m;
-    lds_l[w][head] = bad ? __builtin_nanf("") : l[0];
+    lds_l[w][head] = bad ? __builtin_nanf("") : l;
   }
 #pragma unroll
   for (int x = 0; x < PARTS; ++x) {
@@ -505,8 +520,8 @@ __global__ __launch_bounds__(kThreads, kWide ? 3 : 4) void paged_decode_mxfp4_ke
     }
   };
   // Few results want few loads, many want them together. Always 16: 64 x 5,040 of
-  // 2 x 128 19.2 us for 18.3, 1 x 600 7.4 for 6.7. Always 4: 1 x 32,768 of 4 x 128
-  // 16.3 us for 14.7, 1 x 5,040 of 2 x 64 8.7 for 7.9.
+  // 2 x 128 20.9 us for 19.8, 1 x 600 8.1 for 7.4. Always 4: 1 x 32,768 of 4 x 128
+  // 16.9 us for 15.4, 1 x 5,040 of 2 x 64 8.6 for 7.9.
   if (pieces <= 4) join(std::integral_constant<int, 4>{});
   else join(std::integral_constant<int, 16>{});
 }
@@ -531,8 +546,8 @@ int32_t mxfp4_decode_splits(int32_t batch, int32_t kv_heads, int32_t max_blocks,
   // unequal lengths can take; no sequence has more than its shortest pieces.
   // Many whole sequences fill the chip by themselves, with no piece to find and
   // none to join: 1,024 mixed sequences of 4 KV heads, the fewest that 256 compute
-  // units take whole, up to 600 tokens 32.1 us, in pieces 50.2; up to 4,000 191
-  // and 196.
+  // units take whole, up to 600 tokens 38.5 us, in pieces 54.7; up to 4,000 203
+  // and 214.
   if ((int64_t)batch * kv_heads >= 16 * compute_units) return 1;
   const int64_t pieces = wanted_pieces(kv_heads, compute_units) + batch, most = most_pieces(max_blocks);
   return (int32_t)std::max<int64_t>(1, std::min<int64_t>({(pieces + batch - 1) / batch, most, kMxDecodeMaxSplits}));
