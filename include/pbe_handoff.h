@@ -501,9 +501,10 @@ int pbe_scatter_kv_to_page(const void* keys, const void* values, int32_t in_dtyp
  * ties to the even code, and at most 6 in magnitude. A group that holds an
  * infinity or a NaN stores scale 255 and reads as NaN. A negative slot, or one
  * whose block would end beyond the pool or scale sizes given, writes nothing;
- * a slot that a call names twice ends as a mixture of the two rows. Pools and
- * scale pools 4-byte aligned. Asynchronous on `stream`; n_tokens = 0 queues
- * nothing. */
+ * a slot that a call names twice ends as a mixture of the two rows. Pools, scale
+ * pools and slots 4-byte aligned; the bytes given for the pools and scale pools
+ * may not overlap the rows or the slots. Asynchronous on `stream`; n_tokens = 0
+ * queues nothing. */
 int pbe_scatter_kv_mxfp4(const void* keys, const void* values, int32_t in_dtype, int32_t n_tokens,
                          const int32_t* slot_mapping, int32_t kv_heads, int32_t head_dim,
                          void* key_pool, uint64_t key_pool_bytes, void* value_pool,
@@ -516,7 +517,8 @@ int pbe_scatter_kv_mxfp4(const void* keys, const void* values, int32_t in_dtype,
  * exactly (under scale bytes 253 and 254, which the writer does not store,
  * those of 2^128 and more become infinite). A negative slot leaves its rows as they are; one whose block
  * would end beyond the pool or scale sizes given reads as NaN. The rest as
- * pbe_scatter_kv_mxfp4; a slot may be named any number of times. */
+ * pbe_scatter_kv_mxfp4 (nor may key rows overlap value rows); a slot may be named
+ * any number of times. */
 int pbe_gather_kv_mxfp4(const void* key_pool, uint64_t key_pool_bytes, const void* value_pool,
                         uint64_t value_pool_bytes, const uint8_t* key_scales,
                         uint64_t key_scale_bytes, const uint8_t* value_scales,
@@ -533,8 +535,10 @@ int pbe_gather_kv_mxfp4(const void* key_pool, uint64_t key_pool_bytes, const voi
  * multiple of kv_heads, at most 16 query heads per KV head.
  *
  * queries / outputs: bf16 [batch][q_heads][head_dim], 16-byte aligned; pools
- * 16-byte, scale pools 4-byte aligned. block_tables: int32
- * [batch][max_blocks_per_seq]; seq_lens: int32 [batch] (device memory). What
+ * 16-byte, scale pools 4-byte aligned. outputs may be queries itself; but for
+ * that, outputs and workspace may overlap neither each other nor anything read.
+ * block_tables: int32 [batch][max_blocks_per_seq]; seq_lens: int32 [batch]
+ * (device memory). What
  * lies behind a sequence's last token, in its page or in its table, is not
  * used. A length of 0 gives zeros; a negative one, one that needs more than
  * max_blocks_per_seq blocks, and a block id outside the pools give the
@@ -627,8 +631,8 @@ int pbe_build_step_tables(const int32_t* page_ids, int64_t n_page_ids, const int
  *     writes no page (its q_out row is written).
  *   kv_dtype: PBE_KV_BF16 or PBE_KV_FP8_E4M3 pages as pbe_scatter_kv lays them
  *     out (scales fp32), or PBE_KV_MXFP4 pages (block_size 16, scales bytes).
- *   q_out: bf16 [n_tokens][q_heads][head_dim], 16-byte aligned, apart from the
- *     inputs.
+ *   q_out: bf16 [n_tokens][q_heads][head_dim], 16-byte aligned. Inputs, q_out and
+ *     the bytes given for pools and scale pools may not overlap.
  * Arithmetic is FP32, rounded once, to BF16; FP8 and MXFP4 pages hold what
  * pbe_scatter_kv and pbe_scatter_kv_mxfp4 make of those BF16 rows, byte for
  * byte. Pools aligned to 16 bytes (BF16), 8 (FP8) or 4 (MXFP4), scale pools to

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <initializer_list>
 #include <mutex>
 #include <utility>
 #include <vector>
@@ -54,6 +55,22 @@ bool resolve(const pbe_arena_view& v, uint64_t offset, uint64_t len, uint64_t* a
 // source span (a copy must never race with itself).
 bool spans_disjoint(std::vector<std::pair<uint64_t, uint64_t>> dst,
                     std::vector<std::pair<uint64_t, uint64_t>> src);
+
+// A stretch of memory, and whether two share a byte (a null or empty one none).
+struct Span {
+  const void* at;
+  uint64_t bytes;
+};
+inline bool meet(const Span& a, const Span& b) {
+  const uint64_t x = reinterpret_cast<uint64_t>(a.at), y = reinterpret_cast<uint64_t>(b.at);
+  return a.at && b.at && a.bytes && b.bytes && (x < y ? y - x < a.bytes : x - y < b.bytes);
+}
+inline bool any_meet(std::initializer_list<Span> a, std::initializer_list<Span> b) {
+  for (const Span& x : a)
+    for (const Span& y : b)
+      if (meet(x, y)) return true;
+  return false;
+}
 
 // Checks on the host that [ptr, ptr+bytes) lies inside one allocation a kernel
 // on `device` may touch (device memory of that GPU, or pinned host memory), so

@@ -29,7 +29,7 @@ struct Pools {
 
 // Checks what writer and gather share, and fills `p` but for the rows.
 int rows_params(const Pools& pools, const int32_t* slots, int32_t n_tokens, int32_t kv_heads, int32_t head_dim, const void* keys,
-                const void* values, uint64_t elem, int device, pbe::Mxfp4RowsParams* p) {
+                const void* values, uint64_t elem, bool rows_written, int device, pbe::Mxfp4RowsParams* p) {
   if (head_dim != 64 && head_dim != 128) return fail(PBE_ERR_UNSUPPORTED, "MXFP4 pages hold heads of 64 or 128 dims");
   if (!slots || !keys || !values || !pools.key || !pools.value || !pools.key_scales || !pools.value_scales)
     return fail(PBE_ERR_INVALID, "null MXFP4 operand");
@@ -40,12 +40,18 @@ int rows_params(const Pools& pools, const int32_t* slots, int32_t n_tokens, int3
   if ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(values)) % 16)
     return fail(PBE_ERR_INVALID, "K/V rows must be 16-byte aligned");
   if ((reinterpret_cast<uintptr_t>(pools.key) | reinterpret_cast<uintptr_t>(pools.value) | reinterpret_cast<uintptr_t>(pools.key_scales) |
-       reinterpret_cast<uintptr_t>(pools.value_scales)) % 4)
-    return fail(PBE_ERR_INVALID, "MXFP4 pools and scale pools must be 4-byte aligned");
+       reinterpret_cast<uintptr_t>(pools.value_scales) | reinterpret_cast<uintptr_t>(slots)) % 4)
+    return fail(PBE_ERR_INVALID, "MXFP4 pools, scale pools and slots must be 4-byte aligned");
+  const uint64_t row_bytes = (uint64_t)n_tokens * kv_heads * head_dim * elem;
+  const Span k{keys, row_bytes}, v{values, row_bytes}, s{slots, (uint64_t)n_tokens * 4};
+  const std::initializer_list<Span> pages = {{pools.key, pools.key_bytes}, {pools.value, pools.value_bytes},
+                                             {pools.key_scales, pools.key_scale_bytes}, {pools.value_scales, pools.value_scale_bytes}};
+  // Workgroups read rows, pages and slots while others write.
+  if (any_meet({k, v}, pages) || (rows_written ? meet(k, v) || any_meet({k, v}, {s}) : any_meet({s}, pages)))
+    return fail(PBE_ERR_INVALID, "what is written must lie apart from what is read, and key rows from value rows");
   {
     PBE_DEVICE_SCOPE(device);
     std::vector<Range> known;
-    const uint64_t row_bytes = (uint64_t)n_tokens * kv_heads * head_dim * elem;
     auto ok = [&](const void* ptr, uint64_t bytes) { return bytes == 0 || accessible(ptr, bytes, device, &known); };
     if (!ok(keys, row_bytes) || !ok(values, row_bytes) || !ok(slots, (uint64_t)n_tokens * 4) || !ok(pools.key, pools.key_bytes) ||
         !ok(pools.value, pools.value_bytes) || !ok(pools.key_scales, pools.key_scale_bytes) ||
@@ -86,7 +92,7 @@ int pbe_scatter_kv_mxfp4(const void* keys, const void* values, int32_t in_dtype,
   const bool f32 = in_dtype == PBE_IN_F32;
   pbe::Mxfp4RowsParams p{};
   const int rc = rows_params({key_pool, key_pool_bytes, value_pool, value_pool_bytes, key_scales, key_scale_bytes, value_scales, value_scale_bytes},
-                             slot_mapping, n_tokens, kv_heads, head_dim, keys, values, f32 ? 4 : 2, device, &p);
+                             slot_mapping, n_tokens, kv_heads, head_dim, keys, values, f32 ? 4 : 2, false, device, &p);
   if (rc != PBE_OK) return rc;
   p.keys = static_cast<const uint8_t*>(keys);
   p.values = static_cast<const uint8_t*>(values);
@@ -106,7 +112,7 @@ int pbe_gather_kv_mxfp4(const void* key_pool, uint64_t key_pool_bytes, const voi
   if (n_tokens == 0) return PBE_OK;
   pbe::Mxfp4RowsParams p{};
   const int rc = rows_params({key_pool, key_pool_bytes, value_pool, value_pool_bytes, key_scales, key_scale_bytes, value_scales, value_scale_bytes},
-                             slot_mapping, n_tokens, kv_heads, head_dim, keys, values, 2, device, &p);
+                             slot_mapping, n_tokens, kv_heads, head_dim, keys, values, 2, true, device, &p);
   if (rc != PBE_OK) return rc;
   p.keys_out = static_cast<uint8_t*>(keys);
   p.values_out = static_cast<uint8_t*>(values);
@@ -160,11 +166,17 @@ int pbe_paged_decode_mxfp4(const void* key_pool, const void* value_pool, uint64_
   if (need && !workspace) return fail(PBE_ERR_INVALID, "more than one split needs a workspace");
   if (workspace_bytes < need)
     return fail(PBE_ERR_INVALID, "decode workspace holds %llu of %llu bytes", (unsigned long long)workspace_bytes, (unsigned long long)need);
+  const uint64_t rows = (uint64_t)batch * (uint64_t)q_heads * (uint64_t)head_dim * 2;
+  const Span q{queries, rows}, out{outputs, rows}, partials{workspace, need};
+  // The outputs may take the queries' place, row for row: a KV head's are written when all that read its queries have.
+  if (any_meet({out, partials}, {{key_pool, pool_bytes}, {value_pool, pool_bytes}, {key_scales, scale_pool_bytes}, {value_scales, scale_pool_bytes},
+                                 {block_tables, (uint64_t)batch * (uint64_t)max_blocks_per_seq * 4}, {seq_lens, (uint64_t)batch * 4}}) ||
+      meet(out, partials) || meet(q, partials) || (queries != outputs && meet(q, out)))
+    return fail(PBE_ERR_INVALID, "decode outputs and workspace must lie apart from each other and from what is read");
   {
     PBE_DEVICE_SCOPE(device);
     std::vector<Range> known;
     auto ok = [&](const void* ptr, uint64_t bytes) { return bytes == 0 || accessible(ptr, bytes, device, &known); };
-    const uint64_t rows = (uint64_t)batch * (uint64_t)q_heads * (uint64_t)head_dim * 2;
     if (!ok(key_pool, pool_bytes) || !ok(value_pool, pool_bytes) || !ok(key_scales, scale_pool_bytes) || !ok(value_scales, scale_pool_bytes) ||
         !ok(queries, rows) || !ok(outputs, rows) || !ok(block_tables, (uint64_t)batch * (uint64_t)max_blocks_per_seq * 4) ||
         !ok(seq_lens, (uint64_t)batch * 4) || !ok(workspace, need))

@@ -127,13 +127,16 @@ int pbe_qk_norm_rope_scatter(const void* q, int64_t q_stride, const void* k, int
   auto span = [&](int64_t stride, int64_t heads) { return (uint64_t)(((int64_t)n_tokens - 1) * stride + heads * dim) * (uint64_t)elem; };
   const uint64_t q_span = span(q_stride, q_heads), k_span = span(k_stride, kv_heads), v_span = span(v_stride, kv_heads);
   const uint64_t out_bytes = (uint64_t)n_tokens * (uint64_t)q_heads * (uint64_t)dim * 2;
-  auto meets = [&](const void* in, uint64_t bytes) { return at(in) < at(q_out) + out_bytes && at(q_out) < at(in) + bytes; };
   const uint64_t weight = (uint64_t)(dim * elem), table = rotary_dim ? (uint64_t)max_position * (uint64_t)rotary_dim * 4 : 0;
   const uint64_t ints = (uint64_t)n_tokens * 4;
-  if (meets(q, q_span) || meets(k, k_span) || meets(v, v_span) || (q_weight && meets(q_weight, weight)) ||
-      (k_weight && meets(k_weight, weight)) || (table && meets(cos_sin, table)) || (positions && meets(positions, ints)) ||
-      meets(slot_mapping, ints))
-    return fail(PBE_ERR_INVALID, "q_out must lie apart from the inputs");
+  const std::initializer_list<Span> inputs = {{q, q_span}, {k, k_span}, {v, v_span}, {q_weight, weight}, {k_weight, weight}, {cos_sin, table},
+                                              {positions, ints}, {slot_mapping, ints}};
+  const bool scaled = fp8 || mx;
+  const std::initializer_list<Span> pools = {{key_pool, key_pool_bytes}, {value_pool, value_pool_bytes},
+                                             {key_scales, scaled ? key_scale_bytes : 0}, {value_scales, scaled ? value_scale_bytes : 0}};
+  if (any_meet({{q_out, out_bytes}}, inputs)) return fail(PBE_ERR_INVALID, "q_out must lie apart from the inputs");
+  if (any_meet(pools, inputs) || any_meet(pools, {{q_out, out_bytes}}))
+    return fail(PBE_ERR_INVALID, "pools and scale pools must lie apart from the inputs and q_out");
   {
     PBE_DEVICE_SCOPE(device);
     std::vector<Range> known;

@@ -29,3 +29,19 @@ def test_a_sequence_in_the_widest_table(torch_cuda):
         c.out.fill_(5.0)
         c.call(splits, tables=wide)
         want = c.check(want=want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("splits", [1, 16])
+@pytest.mark.parametrize("heads,group,dim", [(2, 7, 64), (1, 12, 128)])
+def test_outputs_in_the_queries_place(torch_cuda, heads, group, dim, splits):
+    from tests.conftest import say
+    from tests.test_gpu_decode_mxfp4 import Case
+    torch = torch_cuda
+    say(f"decode mxfp4 in place H={heads}x{group} D={dim} splits={splits}")
+    c = Case(torch, [0, 1, 40, 900, 2000], heads, group, dim, seed=2)
+    c.call(splits)
+    torch.cuda.synchronize()
+    c.call(splits, out=c.q)
+    torch.cuda.synchronize()
+    assert torch.equal(c.q.view(torch.int16), c.out.view(torch.int16))
