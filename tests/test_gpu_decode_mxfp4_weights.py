@@ -56,3 +56,16 @@ def test_values_that_cancel_leave_what_the_weights_say(torch_cuda, heads, group,
     c.q_host = c.q.double().cpu().numpy()
     c.call(1)
     check(c)
+
+
+@pytest.mark.parametrize("group", [9, 12, 16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_sequences_of_many_query_heads(torch_cuda, dim, group):
+    """More pieces than are joined four at a time."""
+    say(f"decode mxfp4 5040 tokens H=1x{group} D={dim}")
+    c = Case(torch_cuda, [5040, 20, 3000], 1, group, dim, seed=group)
+    want = None
+    for splits in (0, 64, 1):
+        c.out.fill_(5.0)
+        c.call(splits)
+        want = check(c, want)
