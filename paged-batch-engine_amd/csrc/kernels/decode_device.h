@@ -1,5 +1,5 @@
-// Device helpers of the two decode readers (decode_kernels.hip,
-// decode_split_kernels.hip).
+// Device helpers of the decode readers (decode_kernels.hip,
+// decode_split_kernels.hip, decode_mxfp4_kernels.hip) and of the step tables.
 #pragma once
 #include "decode_kernels.h"
 #include "fp8_device.h"
@@ -91,6 +91,20 @@ __device__ __forceinline__ int wave_max_int(int x) {
   x = max_step<0x140>(x);
   return max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
              max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
+}
+
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int scan_step(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false);
+}
+// Inclusive prefix sum over the wave's lanes.
+__device__ __forceinline__ int wave_scan(int x) {
+  x = scan_step<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: within rows of 16
+  x = scan_step<0x112, 0xf>(x);
+  x = scan_step<0x114, 0xf>(x);
+  x = scan_step<0x118, 0xf>(x);
+  x = scan_step<0x142, 0xa>(x);     // row_bcast 15 into rows 1 and 3
+  return scan_step<0x143, 0xc>(x);  // row_bcast 31 into rows 2 and 3
 }
 
 // Blocks of a length; a bad one (negative, or beyond the table) has none.

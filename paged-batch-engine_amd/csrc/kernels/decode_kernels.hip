@@ -77,19 +77,6 @@ constexpr int kWhole = 24;
 constexpr int min_chunk(int row_bytes) { return row_bytes >= 256 ? 8 : 16; }
 
 // ---- which blocks a workgroup reads ---------------------------------------
-template <int kCtrl, int kRows>
-__device__ __forceinline__ int scan_step(int x) {
-  return x + __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false);
-}
-// Inclusive prefix sum over the wave's lanes.
-__device__ __forceinline__ int wave_scan(int x) {
-  x = scan_step<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: within rows of 16
-  x = scan_step<0x112, 0xf>(x);
-  x = scan_step<0x114, 0xf>(x);
-  x = scan_step<0x118, 0xf>(x);
-  x = scan_step<0x142, 0xa>(x);     // row_bcast 15 into rows 1 and 3
-  return scan_step<0x143, 0xc>(x);  // row_bcast 31 into rows 2 and 3
-}
 __device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 // Slots of a sequence of n blocks at c blocks per slot.
 __device__ __forceinline__ int slots_of(int n, uint32_t c) {

@@ -83,20 +83,6 @@ constexpr int kAgent = 0x10;  // buffer access policy: agent scope
 static_assert(kMxDecodeMaxSplits < (1 << kTicketBits), "arrivals fit the ticket");
 
 // ---- which blocks a workgroup reads ----
-template <int kCtrl, int kRows>
-__device__ __forceinline__ int scan_step(int x) {
-  return x + __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false);
-}
-// Inclusive prefix sum over the wave's lanes.
-__device__ __forceinline__ int wave_scan(int x) {
-  x = scan_step<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: within rows of 16
-  x = scan_step<0x112, 0xf>(x);
-  x = scan_step<0x114, 0xf>(x);
-  x = scan_step<0x118, 0xf>(x);
-  x = scan_step<0x142, 0xa>(x);     // row_bcast 15 into rows 1 and 3
-  return scan_step<0x143, 0xc>(x);  // row_bcast 31 into rows 2 and 3
-}
-
 struct Piece {
   int b = -1;       // sequence; -1: none for this workgroup
   int seq = 0;      // its length

@@ -29,20 +29,6 @@ namespace {
 constexpr int kThreads = 256, kPer = 4, kChunk = kThreads * kPer;  // requests summed at a time
 static_assert(kStepTokens == kThreads, "a token a thread");
 
-template <int kCtrl, int kRows>
-__device__ __forceinline__ int scan_step(int x) {
-  return x + __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false);
-}
-// Inclusive prefix sum over the wave's lanes.
-__device__ __forceinline__ int wave_scan(int x) {
-  x = scan_step<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: within rows of 16
-  x = scan_step<0x112, 0xf>(x);
-  x = scan_step<0x114, 0xf>(x);
-  x = scan_step<0x118, 0xf>(x);
-  x = scan_step<0x142, 0xa>(x);     // row_bcast 15 into rows 1 and 3
-  return scan_step<0x143, 0xc>(x);  // row_bcast 31 into rows 2 and 3
-}
-
 // Whether a request's lengths and pages make sense, and its length then.
 __device__ __forceinline__ bool fits(const StepTablesParams& p, int32_t cached, int32_t added, int32_t lo, int32_t hi) {
   if (lo < 0 || hi < lo || (uint32_t)hi > p.n_page_ids || cached < 0 || added < 0 || (int64_t)cached + added > 0x7fffffff) return false;
