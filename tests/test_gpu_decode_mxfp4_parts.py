@@ -12,16 +12,15 @@ T = 16
 
 
 def test_batches_beyond_one_launch(torch_cuda):
-    """262,140 sequences of 64 KV heads: 262,136 whole ones fill a launch, and 262,128
-    that may be cut, so that the last twelve are read by themselves, the long ones of
-    them in pieces.
-    Whole sequences give the bits that they give in smaller batches; in pieces, a sum
-    in another order moves an output by a step of BF16 at most, 2^-7 of it, and by
-    2^-15 of the values for the weights, and their 700 tokens' FP32 roundings, on
-    either side: below 2^-13 of the largest value."""
+    """65,532 sequences of 256 KV heads: 65,528 whole ones fill a launch, and 65,526
+    that may be cut, so that the last six are read by themselves, the long one of them
+    in pieces. Whole sequences give the bits that they give in smaller batches; in
+    pieces, a sum in another order moves an output by a step of BF16 at most, 2^-7 of
+    it, and by 2^-15 of the values for the weights, and their 700 tokens' FP32
+    roundings, on either side: below 2^-13 of the largest value."""
     torch = torch_cuda
-    say("decode mxfp4 of 262,140 sequences x 64 heads")
-    batch, heads, dim, blocks, longest = 262140, 64, 64, 50, 700
+    say("decode mxfp4 of 65,532 sequences x 256 heads")
+    batch, heads, dim, blocks, longest = 65532, 256, 64, 50, 700
     g = torch.Generator(device="cuda")
     g.manual_seed(1)
     half = T * heads * dim // 2
@@ -30,7 +29,7 @@ def test_batches_beyond_one_launch(torch_cuda):
     most = -(-longest // T)
     tables = torch.randint(0, blocks, (batch, most), generator=g, device="cuda", dtype=torch.int32)
     lens = torch.randint(0, 40, (batch,), generator=g, device="cuda", dtype=torch.int32)
-    for b, n in ((0, longest), (7, 0), (262127, 500), (262128, longest), (262129, 650), (262135, 600), (262136, longest), (262139, 333)):
+    for b, n in ((0, longest), (7, 0), (65524, 500), (65525, 333), (65530, longest)):
         lens[b] = n
     q = torch.randn((batch, heads, dim), generator=g, device="cuda", dtype=torch.bfloat16)
 
