@@ -9,8 +9,8 @@
 // head's stretch of that block from one compute unit.
 //
 // Both are bound by memory, and by the launch where there are few rows. 8,192
-// tokens of 4 x 128 BF16 (21 MB): writer 5.4 us, 3.9 TB/s, gather 5.9, 3.6; 64
-// tokens of 2 x 64: 2.5 and 2.4. The writer fetches and writes what it must (17.1
+// tokens of 4 x 128 BF16 (21 MB): writer 5.4 us, 3.9 TB/s, gather 5.9, 3.6 (FP32 rows,
+// 38 MB, on rows that stay: writer 7.8, and 4.6 of BF16); 64 tokens of 2 x 64: 2.5 and 2.4. The writer fetches and writes what it must (17.1
 // and 4.5 MB), so whole lines leave a compute unit although a lane stores four bytes.
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -15,7 +15,12 @@
 // What bounds it: the rows' bytes in large calls (8,191 tokens of (28 + 2 x 4) x
 // 128: BF16 28.7 us, 5.4 TB/s; FP32 in, half of the dims turned in pairs 40.5 us,
 // 5.6 TB/s), the launch and one chain of arguments, position, line of the table
-// and rows in small ones (one token 2.5 us in a graph). Halves of a whole head
+// and rows in small ones (one token 2.5 us in a graph). The pages' kind changes
+// little: 8,192 tokens as above into BF16, FP8 and MXFP4 pages 29.6 / 30.9 / 30.4 us,
+// 5,040 of (12 + 2 x 2) x 128 10.6 / 11.2 / 10.9, 64 of these 2.9 / 3.2 / 3.1; without
+// norms up to 0.6 less, or 0.9 more. A token's few bytes of an MXFP4 page leave a
+// compute unit by themselves, so that those pages' 4.5 MB (of 63.2 written) count as
+// 10.8. Halves of a whole head
 // change lanes by DPP; through LDS, as parts of a head's dims do, with kinds of
 // heads mixed in a run, the BF16 call took 33.4.
 #include <hip/hip_runtime.h>
@@ -239,7 +244,9 @@ hipError_t launch_qk_norm_rope(RopeParams p, int dim, bool f32_input, bool pairs
   // 36.7 / 31.9 / 28.7 (floor 23.5), 16,384 of (12 + 2 x 2) x 128 (64) 36.1 / 31.5 /
   // 28.9; 5,040 of these (20) 12.2 / 10.8 / 10.8, 5,040 of (14 + 2 x 2) x 64 (11) 7.8
   // / 6.9 / 7.6, 2,000 of (12 + 2 x 2) x 128 (8) 5.3 / 5.1 / 5.8; 512 (2) 3.3 / 3.5 /
-  // 4.2, 1 2.5 / 2.8 / 3.4.
+  // 4.2, 1 2.5 / 2.8 / 3.4. Other pages turn at the same places: 8,192 of (28 + 2 x 4)
+  // x 128, FP8 36.2 / 31.8 / 30.4, MXFP4 38.7 / 34.3 / 30.6; 5,040 of (12 + 2 x 2) x 128
+  // 12.2 / 11.1 / 12.5 and 12.6 / 10.9 / 11.5; 64 3.2 / 3.7 / 4.4 and 3.1 / 3.5 / 4.2.
   const uint64_t each = (uint64_t)p.n_tokens * (p.q_heads + 2 * p.kv_heads) * lanes / ((uint64_t)compute_units * kThreads);
   const int run = each >= 24 ? 4 : each >= 8 ? 2 : 1;
   p.q_runs = (p.q_heads + run - 1) / run;
