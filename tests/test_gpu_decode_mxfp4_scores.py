@@ -163,3 +163,28 @@ def test_no_softmax_of_nothing_but_infinities(torch_cuda):
     c.call(1)
     torch.cuda.synchronize()
     assert (c.out == 0).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_keys_of_two_to_the_128_count_as_infinities(torch_cuda, dim):
+    """Scale byte 254 and code 6, which the page writer does not store."""
+    torch = torch_cuda
+    say(f"decode mxfp4 scores: a key of 6 x 2^127, D={dim}")
+    c = Case(torch, [70], 1, 2, dim, seed=dim)
+    slot = int(c.tables[0, 1]) * T + 4
+    at = M.code_at([slot], 1, dim, False)[0, 0, :32]
+    c.views()[0][at] = 0
+    c.views()[0][at[9]] = 7 << 4
+    c.views()[2][M.scale_at([slot], 1, dim)[0, 0, 0]] = 254
+    c.upload()
+    c.q[0, 0, 9], c.q[0, 1, 9] = 1.0, -1.0
+    c.q_host = c.q.double().cpu().numpy()
+    o, spread, size, reach = M.decode(c.q_host, c.views(), c.tables, c.lens, 1)
+    c.views()[0][at[9]] = 0
+    reach = M.decode(c.q_host, c.views(), c.tables, c.lens, 1)[3]
+    c.call(1)
+    torch.cuda.synchronize()
+    assert torch.isnan(c.out[0, 0].float()).all()
+    got, o, spread, size = c.out[0, 1].double().cpu().numpy(), o[0, 1], spread[0, 1], size[0, 1]
+    e = 2 * (dim + 16) * 2.0 ** -24 * reach[0, 1] + 2.0 ** -20
+    assert (np.abs(got - o) <= 2.0 ** -8 * np.abs(o) + e * spread + (2.0 ** -15 + 70 * 2.0 ** -23) * size).all()
