@@ -651,6 +651,74 @@ int pbe_qk_norm_rope_scatter(const void* q, int64_t q_stride, const void* k, int
                              void* key_scales, uint64_t key_scale_bytes, void* value_scales,
                              uint64_t value_scale_bytes, int device, void* stream);
 
+/* ---- attention of prompts --------------------------------------------------
+ * What a prefill chunk's rows, or a request's drafted tokens, see: softmax(q . k /
+ * sqrt(head_dim)) v for many query tokens a sequence, causal. Query i of a
+ * sequence's n queries, which has `len` keys, sees keys 0 .. len - n + i; one that
+ * sees none gets zeros. BF16 queries and outputs, FP32 scores, softmax and sums;
+ * a softmax weight goes into its product with v as one BF16 number (within 2^-8).
+ * The sum that the outputs are divided by is that of the weights before the
+ * rounding. head_dim 64 or 128, q_heads any multiple of kv_heads.
+ *
+ * An infinity or a NaN in a key or value reaches the queries that see it, and no
+ * other. A score beyond FP32's range, or NaN: -infinity takes a key's weight to
+ * zero, +infinity, NaN, or -infinity for all keys that a query sees, its head to
+ * NaN. Query rows that belong to no sequence are left as they are. The order of a
+ * row's sums, and with it the last bits of its outputs, depends on the batch it is
+ * in and on the workspace's size; for one call they are the same every time.
+ *
+ * workspace: device memory, 16-byte aligned, used until the call completes and
+ * holding anything when it starts. With pbe_prompt_workspace_bytes() of it (of the
+ * current GPU) few rows over many keys are read in pieces that fill the GPU; with
+ * less, or NULL, in fewer or none. outputs may be the queries themselves (rows that
+ * lie one after another); but for that, outputs and workspace may overlap neither
+ * each other nor anything read. rows * q_heads at most INT32_MAX - 255. All
+ * arrays in memory of `device`; no rows are no work. Asynchronous on `stream`, one
+ * launch, or two where rows are read in pieces; the calls can be captured. */
+uint64_t pbe_prompt_workspace_bytes(int32_t n_rows, int32_t batch, int32_t q_heads,
+                                    int32_t kv_heads, int32_t head_dim);
+
+/* Over rows: bf16 q [n_queries] of q_heads heads, k and v [n_keys] of kv_heads heads,
+ * row t + 1 of q q_stride elements after row t (k_stride, v_stride likewise), so
+ * parts of one packed row work. 16-byte aligned, strides whole multiples of 16
+ * bytes. outputs: bf16 [n_queries][q_heads][head_dim], 16-byte aligned.
+ *   q_starts, k_starts: int32 [batch + 1] in device memory: sequence b has the
+ *     queries from q_starts[b] to q_starts[b + 1] and the keys from k_starts[b]
+ *     to k_starts[b + 1]. k_starts NULL: the same, and n_keys = n_queries.
+ * A sequence whose queries begin below 0, end before they begin or beyond
+ * n_queries, or whose keys do so beyond n_keys, gets NaN in those of its rows that
+ * there are. No counterpart in the reference's paged-KV runtime. */
+int pbe_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                         const void* v, int64_t v_stride, int32_t n_queries, int32_t n_keys,
+                         const int32_t* q_starts, const int32_t* k_starts, int32_t batch,
+                         int32_t q_heads, int32_t kv_heads, int32_t head_dim, void* outputs,
+                         void* workspace, uint64_t workspace_bytes, int device, void* stream);
+
+/* Over pages: the keys and values of a sequence, its new tokens' among them, lie
+ * in the pages of a layer as pbe_paged_decode_pools (PBE_KV_BF16, PBE_KV_FP8_E4M3:
+ * fp32 scales) and pbe_paged_decode_mxfp4 (PBE_KV_MXFP4: scale bytes) read them;
+ * pools and scale pools as there, 16 tokens a page.
+ *   queries / outputs: bf16 [n_rows][q_heads][head_dim], 16-byte aligned, as
+ *     pbe_qk_norm_rope_scatter writes them.
+ *   token_starts, seq_lens, block_tables: what pbe_build_step_tables makes, in
+ *     device memory: sequence b's queries are rows token_starts[b] ..
+ *     token_starts[b+1] - 1, the last of its seq_lens[b] tokens.
+ * A sequence whose rows begin below 0, end before they begin or beyond n_rows,
+ * whose length is negative, beyond 2^31 - 256 or needs more than
+ * max_blocks_per_seq blocks gets NaN in those of its rows that there are. A block
+ * id outside the pools gives NaN to the rows that see its tokens. What lies behind
+ * a sequence's last token, in its page or in its table, is not used. Takes the
+ * place of the reference's prefill attention (paged_kv_runtime.cpp) over pages. */
+int pbe_paged_prompt_attention(const void* key_pool, const void* value_pool, uint64_t pool_bytes,
+                               const void* key_scales, const void* value_scales,
+                               uint64_t scale_pool_bytes, int32_t kv_dtype, int32_t kv_heads,
+                               int32_t head_dim, const void* queries, void* outputs,
+                               int32_t n_rows, const int32_t* token_starts, int32_t batch,
+                               int32_t q_heads, const int32_t* block_tables,
+                               const int32_t* seq_lens, int32_t max_blocks_per_seq,
+                               void* workspace, uint64_t workspace_bytes, int device,
+                               void* stream);
+
 /* GPU UUID of `device` (16 bytes), as compared across processes. */
 int pbe_device_uuid(int device, uint8_t out[16]);
 /* The calling thread's current HIP device (the one a pool built without an

@@ -75,6 +75,7 @@ HIP_SOURCES = [
     "csrc/kernels/decode_mxfp4_kernels.hip",
     "csrc/kernels/step_kernels.hip",
     "csrc/kernels/rope_kernels.hip",
+    "csrc/kernels/prompt_kernels.hip",
     "csrc/capi/capi_core.hip",
     "csrc/capi/capi_arena.hip",
     "csrc/capi/capi_plan.hip",
@@ -83,6 +84,7 @@ HIP_SOURCES = [
     "csrc/capi/capi_scatter.hip",
     "csrc/capi/capi_mxfp4.hip",
     "csrc/capi/capi_step.hip",
+    "csrc/capi/capi_prompt.hip",
 ]
 CPU_TESTS = ["tests/cpp/test_drop_in_api.cpp"]
 GPU_TESTS = ["tests/cpp/test_gpu_backend.cpp"]

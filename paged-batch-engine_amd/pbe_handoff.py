@@ -156,6 +156,14 @@ _SIGNATURES = [
     ("pbe_paged_decode_mxfp4", C.c_int, [_P, _P, C.c_uint64, _P, _P, C.c_uint64, C.c_int32,
                                          C.c_int32, _P, _P, C.c_int32, C.c_int32, _P, _P,
                                          C.c_int32, C.c_int32, _P, C.c_uint64, C.c_int, _P]),
+    ("pbe_prompt_workspace_bytes", C.c_uint64, [C.c_int32] * 5),
+    ("pbe_prompt_attention", C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_int32,
+                                       C.c_int32, _P, _P, C.c_int32, C.c_int32, C.c_int32,
+                                       C.c_int32, _P, _P, C.c_uint64, C.c_int, _P]),
+    ("pbe_paged_prompt_attention", C.c_int, [_P, _P, C.c_uint64, _P, _P, C.c_uint64, C.c_int32,
+                                             C.c_int32, C.c_int32, _P, _P, C.c_int32, _P,
+                                             C.c_int32, C.c_int32, _P, _P, C.c_int32, _P,
+                                             C.c_uint64, C.c_int, _P]),
     ("pbe_build_step_tables", C.c_int, [_P, C.c_int64, _P, _P, _P, C.c_int32, C.c_int32, _P,
                                         C.c_int32, _P, _P, _P, _P, C.c_int32, C.c_int, _P]),
     ("pbe_qk_norm_rope_scatter", C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_int32,
@@ -707,3 +715,38 @@ def qk_norm_rope_scatter(q: int, q_stride: int, k: int, k_stride: int, v: int, v
                                          key_scales or None, key_scale_bytes,
                                          value_scales or None, value_scale_bytes, device,
                                          stream or None))
+
+
+def prompt_workspace_bytes(n_rows: int, batch: int, q_heads: int, kv_heads: int,
+                           head_dim: int) -> int:
+    return int(lib().pbe_prompt_workspace_bytes(n_rows, batch, q_heads, kv_heads, head_dim))
+
+
+def prompt_attention(q: int, q_stride: int, k: int, k_stride: int, v: int, v_stride: int,
+                     n_queries: int, n_keys: int, q_starts: int, k_starts: int, batch: int,
+                     q_heads: int, kv_heads: int, head_dim: int, outputs: int,
+                     workspace: int = 0, workspace_bytes: int = 0, stream: int = 0,
+                     device: int = 0) -> None:
+    """Causal attention of packed prompts over rows (pbe_prompt_attention);
+    strides in elements, k_starts 0: the queries' own tokens."""
+    check(lib().pbe_prompt_attention(q or None, q_stride, k or None, k_stride, v or None, v_stride,
+                                     n_queries, n_keys, q_starts or None, k_starts or None, batch,
+                                     q_heads, kv_heads, head_dim, outputs or None,
+                                     workspace or None, workspace_bytes, device, stream or None))
+
+
+def paged_prompt_attention(key_pool: int, value_pool: int, pool_bytes: int, key_scales: int,
+                           value_scales: int, scale_pool_bytes: int, kv_dtype: int,
+                           kv_heads: int, head_dim: int, queries: int, outputs: int, n_rows: int,
+                           token_starts: int, batch: int, q_heads: int, tables: int,
+                           seq_lens: int, max_blocks: int, workspace: int = 0,
+                           workspace_bytes: int = 0, stream: int = 0, device: int = 0) -> None:
+    """Causal attention of a step's new tokens over pages
+    (pbe_paged_prompt_attention)."""
+    check(lib().pbe_paged_prompt_attention(key_pool or None, value_pool or None, pool_bytes,
+                                           key_scales or None, value_scales or None,
+                                           scale_pool_bytes, kv_dtype, kv_heads, head_dim,
+                                           queries or None, outputs or None, n_rows,
+                                           token_starts or None, batch, q_heads, tables or None,
+                                           seq_lens or None, max_blocks, workspace or None,
+                                           workspace_bytes, device, stream or None))
