@@ -719,6 +719,80 @@ int pbe_paged_prompt_attention(const void* key_pool, const void* value_pool, uin
                                void* workspace, uint64_t workspace_bytes, int device,
                                void* stream);
 
+/* ---- page movers -------------------------------------------------------------
+ * Requests that share a cache, and the pages they leave behind, from one step to the
+ * next on the GPU: the tables alone say which pages are held, so nothing is counted
+ * between calls, and a captured step can fork by what it sampled. No counterpart in
+ * the reference on the GPU (its KVCacheManager forks on the host).
+ *
+ * A pool has n_pages pages, in one plane or more (a page-major arena: one plane of
+ * pages of 2*layers*half bytes; local pools: a plane each for every layer's K, V and
+ * scales). Page i lies at byte i * page_bytes of each plane; table entries name it
+ * as i * id_stride (2*layers over a page-major arena, 1 over local pools).
+ * page_bytes: a multiple of 16, at most 1 GiB; planes 16-byte aligned, segments of
+ * whole pages, planes apart from each other; at most 112 planes and 224 segments
+ * a call, and 2^20 pages.
+ *   reserved: int32 [n_pages], or NULL: a page whose word is not 0 is held by others
+ *     as well (a prefill under way, say): it is neither taken nor moved.
+ *   workspace: as many bytes as the functions beside say, used until the call
+ *     completes and holding anything when it starts.
+ * Arrays 4-byte aligned and in memory of `device`; outputs and workspace may
+ * overlap nothing else of a call, nor any array the planes. Rows *
+ * max_blocks_per_seq and n_pages * id_stride at most INT32_MAX. Asynchronous on
+ * `stream`, two launches; the calls can be captured. */
+typedef struct pbe_page_plane {
+  pbe_arena_view memory;
+  uint64_t page_bytes;
+} pbe_page_plane;
+
+/* The next step's requests from the last one's: row i of the new tables goes on
+ * from row parents[i] of the old ones, so a request goes on, forks (a parent named
+ * more than once), ends (one not named) and changes its row in one call, and gets
+ * the pages for its next tokens.
+ *   tables_in: int32 [rows_in][max_blocks_per_seq]; lens_in: int32 [rows_in], tokens of
+ *     each row; the pages of those tokens are held, entries behind them are not.
+ *   parents: int32 [rows_out]; negative: no request. new_lens: int32 [rows_out],
+ *     tokens that are to fit behind a row's own, or NULL for one each.
+ *   tables_out: int32 [rows_out][max_blocks_per_seq]: the parent's pages, then fresh
+ *     ones for the tokens to come, then -1. Whole pages are shared. The last page,
+ *     where it is not full, stays the parent's first child's (the lowest row); every
+ *     other child gets a fresh page with a copy of it in all planes. What tables_in
+ *     shares already must be whole pages.
+ *   lens_out: int32 [rows_out]: the parent's length; 0 without one.
+ *   counts: int32 [2]: fresh pages wanted, and those that there were.
+ * Fresh pages are the lowest ones that neither a new row's parent nor `reserved`
+ * holds, in the order of rows and entries. Where they run out, rows whose pages, in
+ * that order, lie beyond the last one get lens_out -1 and a row of -1; their parents'
+ * pages still count as held. So does a row whose parent is not below rows_in, whose
+ * lengths are negative or add up to more than INT32_MAX or than its table holds, or
+ * which would copy a page that is not in the pool. Other entries of tables_in that
+ * name no page of the pool are passed on as they are. */
+uint64_t pbe_fork_pages_workspace_bytes(int32_t n_pages, int32_t rows_in, int32_t rows_out);
+int pbe_fork_pages(const pbe_page_plane* planes, int32_t n_planes, int32_t n_pages,
+                   int32_t id_stride, int32_t block_size, const int32_t* tables_in,
+                   const int32_t* lens_in, int32_t rows_in, const int32_t* parents,
+                   const int32_t* new_lens, int32_t rows_out, int32_t max_blocks_per_seq,
+                   const int32_t* reserved, int32_t* tables_out, int32_t* lens_out,
+                   int32_t* counts, void* workspace, uint64_t workspace_bytes, int device,
+                   void* stream);
+
+/* Pages moved to the front of their pool, so that what is handed over or given back
+ * is one stretch: the M pages that table entries name and nobody else holds take the
+ * first M places that nobody else holds. Those among them stay; the others, in their
+ * order, move to the places left, in theirs. The places they leave keep their bytes.
+ *   tables_in: int32 [rows][max_blocks_per_seq]; every entry that names a page of the
+ *     pool counts. tables_out: the same with the pages' new names; other entries
+ *     as they are.
+ *   moved_to: int32 [n_pages], or NULL: a page's new place, its own if it stays,
+ *     -1 if no entry names it.
+ *   counts: int32 [2]: M, and the pages moved. */
+uint64_t pbe_compact_pages_workspace_bytes(int32_t n_pages);
+int pbe_compact_pages(const pbe_page_plane* planes, int32_t n_planes, int32_t n_pages,
+                      int32_t id_stride, const int32_t* tables_in, int32_t rows,
+                      int32_t max_blocks_per_seq, const int32_t* reserved, int32_t* tables_out,
+                      int32_t* moved_to, int32_t* counts, void* workspace,
+                      uint64_t workspace_bytes, int device, void* stream);
+
 /* GPU UUID of `device` (16 bytes), as compared across processes. */
 int pbe_device_uuid(int device, uint8_t out[16]);
 /* The calling thread's current HIP device (the one a pool built without an

@@ -76,6 +76,7 @@ HIP_SOURCES = [
     "csrc/kernels/step_kernels.hip",
     "csrc/kernels/rope_kernels.hip",
     "csrc/kernels/prompt_kernels.hip",
+    "csrc/kernels/page_kernels.hip",
     "csrc/capi/capi_core.hip",
     "csrc/capi/capi_arena.hip",
     "csrc/capi/capi_plan.hip",
@@ -85,6 +86,7 @@ HIP_SOURCES = [
     "csrc/capi/capi_mxfp4.hip",
     "csrc/capi/capi_step.hip",
     "csrc/capi/capi_prompt.hip",
+    "csrc/capi/capi_pages.hip",
 ]
 CPU_TESTS = ["tests/cpp/test_drop_in_api.cpp"]
 GPU_TESTS = ["tests/cpp/test_gpu_backend.cpp"]

@@ -49,6 +49,10 @@ class ArenaView(C.Structure):
                 ("reserved", C.c_uint32), ("base", C.c_void_p * PBE_MAX_SEGMENTS)]
 
 
+class PagePlane(C.Structure):
+    _fields_ = [("memory", ArenaView), ("page_bytes", C.c_uint64)]
+
+
 class ArenaIpc(C.Structure):
     _fields_ = [("version", C.c_uint32), ("nseg", C.c_uint32), ("bytes", C.c_uint64),
                 ("segment_bytes", C.c_uint64), ("epoch", C.c_uint64),
@@ -164,6 +168,13 @@ _SIGNATURES = [
                                              C.c_int32, C.c_int32, _P, _P, C.c_int32, _P,
                                              C.c_int32, C.c_int32, _P, _P, C.c_int32, _P,
                                              C.c_uint64, C.c_int, _P]),
+    ("pbe_fork_pages_workspace_bytes", C.c_uint64, [C.c_int32] * 3),
+    ("pbe_fork_pages", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, C.c_int32,
+                                 _P, _P, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, C.c_uint64,
+                                 C.c_int, _P]),
+    ("pbe_compact_pages_workspace_bytes", C.c_uint64, [C.c_int32]),
+    ("pbe_compact_pages", C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int32, C.c_int32,
+                                    _P, _P, _P, _P, _P, C.c_uint64, C.c_int, _P]),
     ("pbe_build_step_tables", C.c_int, [_P, C.c_int64, _P, _P, _P, C.c_int32, C.c_int32, _P,
                                         C.c_int32, _P, _P, _P, _P, C.c_int32, C.c_int, _P]),
     ("pbe_qk_norm_rope_scatter", C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_int32,
@@ -750,3 +761,41 @@ def paged_prompt_attention(key_pool: int, value_pool: int, pool_bytes: int, key_
                                            token_starts or None, batch, q_heads, tables or None,
                                            seq_lens or None, max_blocks, workspace or None,
                                            workspace_bytes, device, stream or None))
+
+
+def page_planes(planes) -> C.Array:
+    """The planes of a page pool, of (ArenaView, bytes of a page) pairs."""
+    planes = list(planes)
+    return (PagePlane * len(planes))(*(PagePlane(view, page) for view, page in planes))
+
+
+def fork_pages_workspace_bytes(n_pages: int, rows_in: int, rows_out: int) -> int:
+    return int(lib().pbe_fork_pages_workspace_bytes(n_pages, rows_in, rows_out))
+
+
+def fork_pages(planes, n_pages: int, id_stride: int, block_size: int, tables_in: int,
+               lens_in: int, rows_in: int, parents: int, new_lens: int, rows_out: int,
+               max_blocks: int, reserved: int, tables_out: int, lens_out: int, counts: int,
+               workspace: int, workspace_bytes: int, stream: int = 0, device: int = 0) -> None:
+    """The next step's requests from the last one's, on the GPU (pbe_fork_pages);
+    planes from page_planes(), new_lens 0: one new token each, reserved 0: none."""
+    check(lib().pbe_fork_pages(planes, len(planes), n_pages, id_stride, block_size,
+                               tables_in or None, lens_in or None, rows_in, parents or None,
+                               new_lens or None, rows_out, max_blocks, reserved or None,
+                               tables_out or None, lens_out or None, counts or None,
+                               workspace or None, workspace_bytes, device, stream or None))
+
+
+def compact_pages_workspace_bytes(n_pages: int) -> int:
+    return int(lib().pbe_compact_pages_workspace_bytes(n_pages))
+
+
+def compact_pages(planes, n_pages: int, id_stride: int, tables_in: int, rows: int,
+                  max_blocks: int, reserved: int, tables_out: int, moved_to: int, counts: int,
+                  workspace: int, workspace_bytes: int, stream: int = 0, device: int = 0) -> None:
+    """Pages in use moved to the front of their pool (pbe_compact_pages);
+    moved_to 0: not wanted."""
+    check(lib().pbe_compact_pages(planes, len(planes), n_pages, id_stride, tables_in or None, rows,
+                                  max_blocks, reserved or None, tables_out or None,
+                                  moved_to or None, counts or None, workspace or None,
+                                  workspace_bytes, device, stream or None))
