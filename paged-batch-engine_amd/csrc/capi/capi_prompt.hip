@@ -14,13 +14,7 @@ using namespace pbe_capi;
 namespace {
 
 constexpr uint64_t kTokens = 16;
-constexpr int64_t kWorkgroups = 2;    // of a compute unit, that tiles are cut for
 constexpr int32_t kMostTokens = INT32_MAX - 255;  // so that a tile's end fits 31 bits
-
-// Pieces per KV head that fill the GPU beside one for each of `tiles`.
-int64_t wanted_pieces(int64_t tiles, int32_t kv_heads, int64_t units) {
-  return std::max<int64_t>(0, kWorkgroups * units / kv_heads - tiles);
-}
 
 struct Call {
   const void* queries;
@@ -48,21 +42,16 @@ int check(const Call& c, int device) {
   return PBE_OK;
 }
 
-// Tiles, pieces and workspace; *need: the bytes of it that the launch uses.
-int plan(const Call& c, int device, pbe::PromptParams* p, int* rows, uint64_t* need) {
+// Tiles, parts and workspace; *need: the bytes of it that the launch uses.
+int plan(const Call& c, pbe::KeyKind kind, int64_t most_keys, int device, pbe::PromptParams* p, pbe::PromptPlan* plan, uint64_t* need) {
   p->group = c.q_heads / c.kv_heads;
-  *rows = pbe::prompt_tile_rows(c.n_rows, c.batch, p->group);
-  const int64_t tiles = pbe::prompt_units(c.n_rows, c.batch, p->group, *rows, 0);
-  const uint64_t each = pbe::prompt_workspace_bytes(1, c.kv_heads, c.head_dim, *rows);
-  const int64_t held = c.workspace ? (int64_t)std::min<uint64_t>(c.workspace_bytes / each, INT32_MAX) - tiles : 0;
-  const int64_t wanted = std::max<int64_t>(0, std::min(wanted_pieces(tiles, c.kv_heads, compute_units(device)), held));
-  const int64_t units = tiles + wanted;
-  if (units * c.kv_heads >= 0xffffffffll / (2 * *rows)) return fail(PBE_ERR_INVALID, "too many rows and heads for one launch");
-  *need = wanted ? (uint64_t)units * each : 0;
-  p->units = (int32_t)units;
-  p->wanted = (int32_t)wanted;
+  *plan = pbe::plan_prompt(c.n_rows, c.batch, p->group, c.kv_heads, kind, most_keys, compute_units(device), c.workspace ? c.workspace_bytes : 0, c.head_dim);
+  // fewer than 2^32 threads in a launch: eight workgroups more than are needed, the join's of 1,024
+  if ((std::max<int64_t>(plan->tiles, plan->parts) + 8) * c.kv_heads >= 0xffffffffll / (plan->parts ? 1024 : 2 * plan->rows))
+    return fail(PBE_ERR_INVALID, "too many rows and heads for one launch");
+  *need = (uint64_t)plan->parts * plan->each;
   p->part_acc = static_cast<float*>(c.workspace);
-  p->part_ml = p->part_acc + (uint64_t)units * (uint64_t)c.kv_heads * (uint64_t)*rows * (uint64_t)c.head_dim;
+  p->part_ml = p->part_acc + 2ull * (uint64_t)plan->parts * (uint64_t)c.kv_heads * (uint64_t)plan->rows * (uint64_t)c.head_dim;
   p->q = static_cast<const uint8_t*>(c.queries);
   p->out = static_cast<uint8_t*>(c.outputs);
   p->q_starts = c.starts;
@@ -80,11 +69,12 @@ extern "C" {
 
 uint64_t pbe_prompt_workspace_bytes(int32_t n_rows, int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim) {
   if (n_rows <= 0 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_heads % kv_heads) return 0;
-  const int32_t group = q_heads / kv_heads;
-  const int rows = pbe::prompt_tile_rows(n_rows, batch, group);
-  const int64_t tiles = pbe::prompt_units(n_rows, batch, group, rows, 0);
-  const int64_t wanted = wanted_pieces(tiles, kv_heads, compute_units());
-  return wanted ? pbe::prompt_workspace_bytes(tiles + wanted, kv_heads, head_dim, rows) : 0;
+  uint64_t most = 0;  // over the kinds of keys and values
+  for (const pbe::KeyKind kind : {pbe::KeyKind::kRows, pbe::KeyKind::kBf16, pbe::KeyKind::kFp8, pbe::KeyKind::kMxfp4}) {
+    const pbe::PromptPlan r = pbe::plan_prompt(n_rows, batch, q_heads / kv_heads, kv_heads, kind, INT32_MAX, compute_units(), ~0ull, head_dim);
+    most = std::max(most, (uint64_t)r.parts * r.each);
+  }
+  return most;
 }
 
 int pbe_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
@@ -113,9 +103,9 @@ int pbe_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t
     spans[i] = r.count ? (uint64_t)((r.count - 1) * r.stride + r.row) * 2 : 0;
   }
   pbe::PromptParams p{};
-  int rows = 0;
+  pbe::PromptPlan laid;
   uint64_t need = 0;
-  rc = plan(c, device, &p, &rows, &need);
+  rc = plan(c, pbe::KeyKind::kRows, n_keys, device, &p, &laid, &need);
   if (rc != PBE_OK) return rc;
   const uint64_t out_bytes = (uint64_t)n_queries * (uint64_t)q_heads * (uint64_t)dim * 2, starts = ((uint64_t)batch + 1) * 4;
   const Span out{outputs, out_bytes}, partials{workspace, need}, queries{q, spans[0]};
@@ -139,7 +129,7 @@ int pbe_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t
   p.lens = k_starts;
   p.n_k = n_keys;
   PBE_DEVICE_SCOPE(device);
-  PBE_HIP(pbe::launch_prompt_attention(p, head_dim, pbe::KeyKind::kRows, rows, static_cast<hipStream_t>(stream)));
+  PBE_HIP(pbe::launch_prompt_attention(p, laid, head_dim, pbe::KeyKind::kRows, static_cast<hipStream_t>(stream)));
   return PBE_OK;
 }
 
@@ -172,9 +162,10 @@ int pbe_paged_prompt_attention(const void* key_pool, const void* value_pool, uin
   if (pool_bytes < half || (scaled && scale_pool_bytes < block_scales))
     return fail(PBE_ERR_INVALID, "pools and scale pools must hold at least one block");
   pbe::PromptParams p{};
-  int rows = 0;
+  pbe::PromptPlan laid;
   uint64_t need = 0;
-  rc = plan(c, device, &p, &rows, &need);
+  const pbe::KeyKind kind = mx ? pbe::KeyKind::kMxfp4 : fp8 ? pbe::KeyKind::kFp8 : pbe::KeyKind::kBf16;
+  rc = plan(c, kind, (int64_t)max_blocks_per_seq * (int64_t)kTokens, device, &p, &laid, &need);
   if (rc != PBE_OK) return rc;
   const uint64_t row_bytes = (uint64_t)n_rows * (uint64_t)q_heads * (uint64_t)head_dim * 2;
   const uint64_t starts = ((uint64_t)batch + 1) * 4, lens = (uint64_t)batch * 4, tables = (uint64_t)batch * (uint64_t)max_blocks_per_seq * 4;
@@ -207,8 +198,7 @@ int pbe_paged_prompt_attention(const void* key_pool, const void* value_pool, uin
   if (scaled) blocks = std::min(blocks, scale_pool_bytes / block_scales);
   p.blocks = (int32_t)std::min<uint64_t>(blocks, INT32_MAX);
   PBE_DEVICE_SCOPE(device);
-  PBE_HIP(pbe::launch_prompt_attention(p, head_dim, mx ? pbe::KeyKind::kMxfp4 : fp8 ? pbe::KeyKind::kFp8 : pbe::KeyKind::kBf16, rows,
-                                       static_cast<hipStream_t>(stream)));
+  PBE_HIP(pbe::launch_prompt_attention(p, laid, head_dim, kind, static_cast<hipStream_t>(stream)));
   return PBE_OK;
 }
 

@@ -20,26 +20,33 @@ struct PromptParams {
   const int32_t* q_starts;  // [batch + 1]
   const int32_t* lens;      // pages: [batch] lengths; rows: [batch + 1] first rows
   const int32_t* tables;    // pages: [batch][max_blocks]
-  float* part_acc;          // [unit][kv_heads][rows of a tile][head_dim]
-  float* part_ml;           // [unit][kv_heads][rows of a tile][2]: maximum, sum
+  float* part_acc;          // [part][2][kv_heads][rows of a tile][head_dim]
+  float* part_ml;           // [part][2][kv_heads][rows of a tile][2]: maximum, sum
   uint64_t q_stride, k_stride, v_stride;  // bytes between rows (k, v: of rows, or of a page's tokens)
   uint64_t half;            // pages: bytes of one block of one pool
   int32_t n_q, n_k;         // rows there are (n_k: of rows)
   int32_t batch, kv_heads, group;
   int32_t max_blocks, blocks;  // pages: of a table, of the pools
-  int32_t units;            // pieces of tiles that the launch has workgroups for, per KV head
-  int32_t wanted;           // pieces that fill the GPU, per KV head; 0: no tile is cut
+  int32_t parts;            // per KV head that the work is cut into; 0: a workgroup a tile
+  int32_t step;             // what a tile costs more than the one before (sixteenths of a key)
+  double a_part;            // 1 / parts
   float scale;              // log2(e) / sqrt(head_dim): scores in base 2
   FastDiv by_group;
 };
 
-// Rows (tokens times query heads of a KV head) of a workgroup's tile.
-int prompt_tile_rows(int64_t n_q, int64_t batch, int32_t group);
-// Most pieces per KV head of tiles of `rows`: as many as are wanted and one a tile.
-int64_t prompt_units(int64_t n_q, int64_t batch, int32_t group, int rows, int64_t wanted);
-// Bytes of partial results of `units` pieces, 16-byte multiples.
-uint64_t prompt_workspace_bytes(int64_t units, int32_t kv_heads, int32_t head_dim, int rows);
+// How a call is cut up: tiles of `rows` rows (tokens times query heads of a KV
+// head), at most `tiles` of them; `parts` equal parts of all their work per KV head,
+// with `each` bytes of partial results, or 0.
+struct PromptPlan {
+  int rows = 0;
+  int64_t tiles = 0;
+  int32_t parts = 0;
+  uint64_t each = 0;
+};
+// most_keys: that a sequence may have; units: compute units.
+PromptPlan plan_prompt(int64_t n_q, int64_t batch, int32_t group, int32_t kv_heads, KeyKind kind, int64_t most_keys, int64_t units, uint64_t workspace,
+                       int32_t head_dim);
 
-hipError_t launch_prompt_attention(const PromptParams& p, int dim, KeyKind kind, int rows, hipStream_t stream);
+hipError_t launch_prompt_attention(PromptParams p, const PromptPlan& plan, int dim, KeyKind kind, hipStream_t stream);
 
 }  // namespace pbe

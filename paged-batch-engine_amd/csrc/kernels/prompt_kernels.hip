@@ -3,6 +3,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "decode_device.h"
 #include "mxfp4_device.h"
@@ -13,36 +14,41 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 #define PBE_LDS __attribute__((address_space(3)))
 
-constexpr int kKeys = 64;        // keys of a tile
-constexpr int kMinPiece = 8;     // key tiles of a piece that joining is worth
-constexpr int kMaxPieces = 256;  // of a tile
-constexpr float kLazy = 8.f;     // how far (in base 2) scores may pass the maximum that weights refer to
+constexpr int kKeys = 64;         // keys of a tile
+constexpr int kPiece = 8;          // key tiles between the cuts of a tile
+constexpr int kMaxCuts = 4096;    // of a tile
+constexpr float kLazy = 8.f;      // how far (in base 2) scores may pass the maximum that weights refer to
+constexpr float kFar = 1024.f;    // maxima (in base 2) beyond which weights come from the scores' differences
+constexpr int kXcds = 8;
+static_assert(kBlockTokens == 16, "a key tile is four blocks");
 
 // ---- which rows and keys a workgroup has ----
-struct Unit {
-  int b = -1;              // sequence; -1: none for this workgroup
-  int tile = 0;            // of its rows
-  int s = 0, k = 1;        // which piece of the tile's keys, of how many
-  int begin = 0, rows = 0; // first row of q, tokens
-  int shown = 0;           // of those, the ones within n_q
-  int first = 0;           // first row of k (rows)
-  int len = 0;             // keys
-  bool bad = false;        // starts or length make no sense
+struct Seq {
+  int begin = 0, rows = 0;  // first row of q, tokens (those within n_q)
+  int first = 0, len = 0;   // first row of k (rows), keys
+  int tiles = 0;
+  bool bad = false;         // starts or length make no sense
+  // What tile t costs, in sixteenths of a key: base + step * (t + 1). A model: it
+  // only has to be the same for all workgroups.
+  int64_t base = 0, step = 0;
+  __device__ __forceinline__ int64_t cost(int t) const { return base + step * (t + 1); }
+  __device__ __forceinline__ int64_t before(int64_t t) const { return base * t + step * (t * (t + 1) / 2); }
 };
 
-template <KeyKind kKind>
-__device__ __forceinline__ Unit unit_of(const PromptParams& p, int b) {
-  Unit u;
-  u.b = b;
+constexpr int64_t kTileCost = 16 * 2 * kKeys;  // of a tile's start and end
+
+template <KeyKind kKind, int kRows>
+__device__ __forceinline__ Seq seq_of(const PromptParams& p, int b) {
+  Seq u;
   const int lo = p.q_starts[b], hi = p.q_starts[b + 1];
   u.begin = min(max(lo, 0), p.n_q);
   u.bad = lo < 0 || hi < lo || hi > p.n_q;
-  u.shown = max(0, min(hi, p.n_q) - u.begin);
-  u.rows = u.shown;
+  u.rows = max(0, min(hi, p.n_q) - u.begin);
   if constexpr (kKind == KeyKind::kRows) {
     const int from = p.lens[b], to = p.lens[b + 1];
     u.bad |= from < 0 || to < from || to > p.n_k;
@@ -53,65 +59,170 @@ __device__ __forceinline__ Unit unit_of(const PromptParams& p, int b) {
     u.bad |= len < 0 || len > 0x7fffff00 || (uint32_t)len > (uint32_t)p.max_blocks * (uint64_t)kBlockTokens;
     u.len = u.bad ? 0 : len;
   }
+  u.tiles = (int)(((uint32_t)u.rows * (uint32_t)p.group + kRows - 1) / kRows);
+  u.base = kTileCost + 16 * (int64_t)max(0, u.len - u.rows);
+  u.step = u.len ? p.step : 0;
   return u;
 }
 
 __device__ __forceinline__ int key_tiles(int len) { return (int)(((uint32_t)len + kKeys - 1) / kKeys); }
 
-// Unit z of the batch. Every tile of a sequence is cut into as many pieces as its
-// whole length gives.
-template <KeyKind kKind, int kRows>
-__device__ __forceinline__ Unit find_unit(const PromptParams& p, int z, int lane) {
-  int c = 0x7fffffff;
-  auto tiles_of = [&](const Unit& u) { return (int)(((uint32_t)u.shown * (uint32_t)p.group + kRows - 1) / kRows); };
-  if (p.wanted) {
-    int64_t sum = 0;
-    for (int i = lane; i < p.batch; i += 64) {
-      const Unit u = unit_of<kKind>(p, i);
-      sum += (int64_t)tiles_of(u) * key_tiles(u.len);
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d, 64);
-    c = (int)min((int64_t)0x7fffffff, max((int64_t)kMinPiece, (sum + p.wanted - 1) / p.wanted));
-  }
-  int before = 0;
-  for (int i = 0; i < p.batch; i += 64) {
-    Unit u;
-    int n = 0, k = 1;
-    if (i + lane < p.batch) {
-      u = unit_of<kKind>(p, i + lane);
-      const int kt = key_tiles(u.len);
-      k = p.wanted ? min(kMaxPieces, max(1, (kt + c - 1) / c)) : 1;
-      n = tiles_of(u) * k;
-    }
-    const int upto = wave_scan(n) + before;
-    const uint64_t past = __ballot(upto > z);
+// Row r of a sequence's, tokens times query heads of a KV head: its token (rows
+// behind the last: the last one's), and the keys that a token sees.
+__device__ __forceinline__ int token_of(const PromptParams& p, const Seq& u, int r) {
+  return (int)fast_div((uint32_t)min(r, u.rows * p.group - 1), p.by_group);
+}
+__device__ __forceinline__ int seen_by(const Seq& u, int token) { return max(0, u.len - u.rows + token + 1); }
+template <int kRows>
+__device__ __forceinline__ int tiles_seen(const PromptParams& p, const Seq& u, int t) {
+  return key_tiles(seen_by(u, token_of(p, u, t * kRows + kRows - 1)));
+}
+
+__device__ __forceinline__ int64_t of_lane(int64_t x, int lane) {
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, lane) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32);
+}
+// Inclusive prefix sum over the wave's lanes of numbers below 2^62: 32-bit scans of
+// 21 bits each.
+__device__ __forceinline__ int64_t wave_scan64(int64_t x) {
+  const int64_t a = wave_scan((int)(x & 0x1fffff)), b = wave_scan((int)(x >> 21 & 0x1fffff)), c = wave_scan((int)(x >> 42));
+  return a + (b << 21) + (c << 42);
+}
+
+// The sequence in which place x of a running sum over the sequences lies, `of` being
+// what a sequence adds to it, and the sum before it; b = batch behind the last.
+struct Found {
+  int b;
+  int64_t before;
+};
+template <typename Of>
+__device__ __forceinline__ Found find_seq(int batch, int64_t x, int lane, Of of) {
+  int64_t before = 0;
+  for (int i = 0; i < batch; i += 64) {
+    const int64_t mine = i + lane < batch ? of(i + lane) : 0, upto = before + wave_scan64(mine);
+    const uint64_t past = __ballot(upto > x);
     if (past) {
       const int at = __builtin_ctzll(past);
-      Unit r;
-      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
-      r.b = i + at;
-      r.k = of(k);
-      r.begin = of(u.begin);
-      r.rows = r.shown = of(u.shown);
-      r.first = of(u.first);
-      r.len = of(u.len);
-      r.bad = of(u.bad);
-      const int w = z - of(upto - n), tiles = of(n) / r.k;
-      r.tile = tiles - 1 - w / r.k;  // those that see the most keys first
-      r.s = w % r.k;
-      return r;
+      return {i + at, of_lane(upto - mine, at)};
     }
-    before = __builtin_amdgcn_readlane(upto, 63);
+    before = of_lane(upto, 63);
   }
-  return Unit{};
+  return {batch, before};
+}
+
+// All the work of the batch, and where part w of it begins.
+template <KeyKind kKind, int kRows>
+__device__ __forceinline__ int64_t work_of(const PromptParams& p, int b) {
+  const Seq u = seq_of<kKind, kRows>(p, b);
+  return u.before(u.tiles);
+}
+template <KeyKind kKind, int kRows>
+__device__ __forceinline__ int64_t total_work(const PromptParams& p, int lane) {
+  int64_t sum = 0;
+  for (int b = lane; b < p.batch; b += 64) sum += work_of<kKind, kRows>(p, b);
+  return of_lane(wave_scan64(sum), 63);
+}
+__device__ __forceinline__ int64_t part_at(const PromptParams& p, int64_t total, int w) {
+  const int64_t each = (int64_t)((double)total * p.a_part) + 1 + (total >> 50);  // at least a parts-th
+  return min(total, each * w);
+}
+
+// Key tile k of tile t of sequence b; the work before the tile.
+struct Place {
+  int b, t, k;
+  int64_t start;
+};
+
+// The key tile at which a part that begins at y of a tile's `cost` cuts its n key
+// tiles: cuts lie kPiece tiles apart, and as far from the end.
+__device__ __forceinline__ int cut_at(int64_t y, int64_t cost, int n) {
+  const int k = min((int)((double)y * (double)n / (double)cost), n - kPiece);
+  return k <= 0 ? 0 : k - k % kPiece;
+}
+
+// Place x of the work, which is sequence f's.
+template <KeyKind kKind, int kRows>
+__device__ __forceinline__ Place place_at(const PromptParams& p, const Found& f, int64_t x) {
+  if (f.b >= p.batch) return {p.batch, 0, 0, f.before};
+  const Seq u = seq_of<kKind, kRows>(p, f.b);
+  const int64_t y = x - f.before;
+  // before(t) <= y < before(t + 1), from the root of its quadratic
+  const float half = (float)u.base + 0.5f * (float)u.step, root = __builtin_amdgcn_sqrtf(half * half + 2.f * (float)u.step * (float)y);
+  int t = min(max((int)(2.f * (float)y / (half + root)), 0), u.tiles - 1);
+  while (t > 0 && u.before(t) > y) --t;
+  while (t + 1 < u.tiles && u.before(t + 1) <= y) ++t;
+  t = __builtin_amdgcn_readfirstlane(t);
+  const int64_t before = u.before(t);
+  return {f.b, t, __builtin_amdgcn_readfirstlane(cut_at(y - before, u.cost(t), tiles_seen<kRows>(p, u, t))), f.before + before};
+}
+
+// Where part w begins and ends. Returns all the work.
+template <KeyKind kKind, int kRows>
+__device__ __forceinline__ int64_t find_part(const PromptParams& p, int w, int lane, Place* at, Place* end) {
+  if (p.batch <= 64) {
+    const int64_t mine = lane < p.batch ? work_of<kKind, kRows>(p, lane) : 0, upto = wave_scan64(mine), total = of_lane(upto, 63);
+    auto place = [&](int64_t x) {
+      const uint64_t past = __ballot(upto > x);
+      const int b = past ? __builtin_ctzll(past) : p.batch;
+      return place_at<kKind, kRows>(p, Found{b, past ? of_lane(upto - mine, b) : total}, x);
+    };
+    *at = place(part_at(p, total, w));
+    if (end) *end = place(part_at(p, total, w + 1));
+    return total;
+  }
+  const int64_t total = total_work<kKind, kRows>(p, lane);
+  auto place = [&](int64_t x) { return place_at<kKind, kRows>(p, find_seq(p.batch, x, lane, [&](int b) { return work_of<kKind, kRows>(p, b); }), x); };
+  *at = place(part_at(p, total, w));
+  if (end) *end = place(part_at(p, total, w + 1));
+  return total;
+}
+
+// The w-th tile of the batch, those that cost the most first (so that none of them is
+// among the last to begin). Returns whether there is one.
+template <KeyKind kKind, int kRows>
+__device__ __forceinline__ bool find_tile(const PromptParams& p, int w, int lane, Place* at) {
+  if (p.batch == 1) {
+    const Seq u = seq_of<kKind, kRows>(p, 0);
+    *at = {0, u.tiles - 1 - w, 0, 0};
+    return w < u.tiles;
+  }
+  if (p.batch > 64) {  // too many to rank: a sequence's last tile first
+    const Found f = find_seq(p.batch, w, lane, [&](int b) { return (int64_t)seq_of<kKind, kRows>(p, b).tiles; });
+    if (f.b >= p.batch) return false;
+    *at = {f.b, seq_of<kKind, kRows>(p, f.b).tiles - 1 - (int)(w - f.before), 0, 0};
+    return true;
+  }
+  const Seq u = lane < p.batch ? seq_of<kKind, kRows>(p, lane) : Seq{};
+  if (w >= __builtin_amdgcn_readlane(wave_scan(u.tiles), 63)) return false;
+  // Tiles of this lane's sequence that cost more than c: those from t on with base +
+  // step * (t + 1) > c.
+  const float base = (float)u.base, step = (float)u.step, a_step = u.step ? 1.f / step : 0.f;
+  auto above = [&](float c) {
+    const int below = u.step ? min(u.tiles, max(0, (int)floorf((c - base) * a_step))) : base > c ? 0 : u.tiles;
+    return u.tiles - below;
+  };
+  // The largest cost (of some float grid) that at most w tiles pass: then those that
+  // pass it are before tile w, and what is left is taken in the sequences' order.
+  float low = 0.f, high = (float)wave_max_int((int)min((int64_t)0x7fffff00, u.cost(u.tiles) / 16 + 1)) * 16.f;
+  for (int i = 0; i < 14; ++i) {
+    const float mid = 0.5f * (low + high);
+    const bool few = __builtin_amdgcn_readlane(wave_scan(above(mid)), 63) <= w;
+    high = few ? mid : high;
+    low = few ? low : mid;
+  }
+  // `high` is passed by at most w tiles, `low` by more: tile w is among those between.
+  const int over = above(high), between = above(low) - over;
+  const int rank = w - __builtin_amdgcn_readlane(wave_scan(over), 63);
+  const int upto = wave_scan(between);
+  const int b = __builtin_ctzll(__ballot(upto > rank));
+  auto of = [&](int x) { return __builtin_amdgcn_readlane(x, b); };
+  *at = {b, of(u.tiles) - 1 - of(over) - (rank - of(upto - between)), 0, 0};
+  return true;
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   const f32x2 v{a, b};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
 }
-
 __device__ __forceinline__ float halves_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -120,189 +231,211 @@ __device__ __forceinline__ float halves_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-
 // The sum of a word's two BF16 values and c, in FP32.
-typedef short s16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float sum_bf16(uint32_t x, float c) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(s16x2, x), s16x2{0x3f80, 0x3f80}, c, false);
 }
 
-// Where the 16-byte chunk c of row r of a K or V tile lies in LDS (in bytes): the
+// Where the 16-byte chunk c of row r of a tile of K or V lies in LDS (in bytes): the
 // chunks of a row change places so that the lanes of a read hit different banks.
 template <int D>
-__device__ __forceinline__ uint32_t k_at(uint32_t r, uint32_t c) {
-  return r * (2 * D) + ((c ^ (r & (D / 8 - 1))) * 16);
-}
+__device__ __forceinline__ uint32_t k_flip(uint32_t r) { return r & (D / 8 - 1); }
 template <int D>
-__device__ __forceinline__ uint32_t v_at(uint32_t r, uint32_t c) {
-  return r * (2 * D) + ((c ^ ((2 * r) & (D / 8 - 1))) * 16);
-}
+__device__ __forceinline__ uint32_t v_flip(uint32_t r) { return (2 * r) & (D / 8 - 1); }
+template <int D>
+__device__ __forceinline__ uint32_t code_flip(uint32_t r) { return (r / (256 / D)) & (D / 16 - 1); }
+template <int D>
+__device__ __forceinline__ uint32_t k_at(uint32_t r, uint32_t c) { return r * (2 * D) + ((c ^ k_flip<D>(r)) * 16); }
+template <int D>
+__device__ __forceinline__ uint32_t v_at(uint32_t r, uint32_t c) { return r * (2 * D) + ((c ^ v_flip<D>(r)) * 16); }
+template <int D>
+__device__ __forceinline__ uint32_t code_at(uint32_t r, uint32_t c) { return r * D + ((c ^ code_flip<D>(r)) * 16); }
 
 // ---- keys and values into LDS ----
-// 16 bytes a lane from `from` to LDS, lane after lane from `to` on, past the
-// registers. Written as an instruction because the compiler would wait for the
-// builtin's result before any read of LDS; here arrived() says when it is there.
-// It writes no register but m0, which nothing else here uses.
+// A lane's 16 (or 4) bytes to LDS, lane after lane from `to` on, past the registers.
+// Written as instructions because the compiler would wait for the builtin's result
+// before any read of LDS; here arrived() says when it is there. They write no
+// register but m0, which nothing else here uses.
 __device__ __forceinline__ void load_to_lds(const uint8_t* from, PBE_LDS uint8_t* to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"((uint32_t)(uintptr_t)to) : "memory");
 }
-// Waits for all that this wave has asked global memory for (vmcnt 0, no other counter).
+__device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t lane_at, PBE_LDS uint8_t* to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_at), "s"(base), "s"((uint32_t)(uintptr_t)to) : "memory");
+}
+__device__ __forceinline__ void load_word_to_lds(const uint8_t* from, PBE_LDS uint8_t* to) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"((uint32_t)(uintptr_t)to) : "memory");
+}
+// Waits until at most kLeft of what this wave has asked global memory for is on its way.
+template <int kLeft>
 __device__ __forceinline__ void arrived() {
+  static_assert(kLeft < 64, "six bits");
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0f70);
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (kLeft & 15) | (kLeft >> 4) << 14);
   asm volatile("" ::: "memory");
 }
 
+// Key tiles in LDS, loaded there directly, in turns: while one is used, the next
+// kTurns - 1 are on their way.
+//  - rows and BF16 pages: as they are. FP8 pages: as they are too; reads convert.
+//  - MXFP4 pages: codes as they are, in two turns; each thread makes BF16 rows of what
+//    it asked for before a tile is used (the values' codes cannot be transposed).
 template <int D, KeyKind kKind, int kWaves>
 struct Stage {
-  static constexpr int T = 64 * kWaves;
-  static constexpr int kTileBytes = kKeys * D * 2;
-  static constexpr int kRowsAnInstr = 1024 / (2 * D), kInstrs = kKeys / kRowsAnInstr / kWaves;
-  static constexpr int kFp8Units = kKeys * D / 16, kFp8Each = (kFp8Units + T - 1) / T;
-  static constexpr int kMxEach = (256 + T - 1) / T;
-  static constexpr bool kDirect = kKind == KeyKind::kRows || kKind == KeyKind::kBf16;
+  static constexpr bool kMx = kKind == KeyKind::kMxfp4, kFp8 = kKind == KeyKind::kFp8, kScaled = kMx || kFp8;
+  static constexpr int kTile = kKeys * D * (kFp8 ? 1 : 2);                 // bytes of K (or V) as they are read
+  static constexpr int kRaw = kMx ? kKeys * D / 2 : kTile;                 // as they are loaded
+  static constexpr int kTurns = kFp8 ? 3 : 2;
+  static constexpr int kInstr = kRaw / 1024;                               // loads for K (or V)
+  static constexpr int kLoads = (2 * kInstr + kWaves - 1) / kWaves;        // of a wave
+  static constexpr int kScaleBytes = kScaled ? 512 : 0;                    // K's and V's of a tile
+  static constexpr int kAll = kTurns * 2 * kRaw + (kMx ? 2 * kTile : 0) + 3 * kScaleBytes;
+  static constexpr int kPerTile = kLoads + kScaled * (kWaves == 1 ? 2 : 1);                        // loads of a wave and tile
+  static constexpr int kRowBytes = kFp8 ? D : 2 * D, kChunks = kRowBytes / 16, kRowsALoad = 64 / kChunks;  // rows, FP8, BF16
 
   const PromptParams& p;
-  const Unit& u;
-  int head, lane, wave, nblocks;
-  int32_t ids = 0, next_ids = 0;  // of 64 blocks from `chunk` on, a lane each, and of the next 64
-  uint64_t bad = 0, next_bad = 0;
+  const Seq& u;
+  PBE_LDS uint8_t* const mem;
+  int b, head, lane, wave, nblocks;
+  int32_t ids = 0, next = 0;  // of 64 blocks from `chunk` on, a lane each; the next 64's entries
+  uint64_t bad = 0;           // those of the 64 that are not in the pools (their id is 0 here)
   int chunk = -1;
-  // FP8, MXFP4: what waits in registers to be converted
-  u32x4 kr[kKind == KeyKind::kFp8 ? kFp8Each : kMxEach], vr[kKind == KeyKind::kFp8 ? kFp8Each : kMxEach];
-  uint32_t sk[kMxEach], sv[kMxEach];
 
-  __device__ __forceinline__ Stage(const PromptParams& p_, const Unit& u_, int head_, int lane_, int wave_)
-      : p(p_), u(u_), head(head_), lane(lane_), wave(wave_), nblocks((int)(((uint32_t)u_.len + kBlockTokens - 1) / kBlockTokens)) {}
+  __device__ __forceinline__ Stage(const PromptParams& p_, const Seq& u_, PBE_LDS uint8_t* mem_, int b_, int head_, int lane_, int wave_)
+      : p(p_), u(u_), mem(mem_), b(b_), head(head_), lane(lane_), wave(wave_), nblocks((int)(((uint32_t)u_.len + kBlockTokens - 1) / kBlockTokens)) {}
 
-  __device__ __forceinline__ void load_ids(int first, int32_t* to, uint64_t* wrong) {
-    const int i = min(first + lane, nblocks - 1);
-    int32_t id = p.tables[(int64_t)u.b * p.max_blocks + i];
-    const bool off = id < 0 || id >= p.blocks;
-    *wrong = __ballot(off);
-    *to = off ? 0 : id;
-  }
-  // Makes the ids of key tile kt's blocks (kt counts up by one) ready.
-  __device__ __forceinline__ void ids_for(int kt) {
+  __device__ __forceinline__ PBE_LDS uint8_t* raw(int turn) const { return mem + turn % kTurns * (2 * kRaw); }
+  __device__ __forceinline__ PBE_LDS uint8_t* keys(int turn) const { return kMx ? mem + kTurns * 2 * kRaw : raw(turn); }
+  __device__ __forceinline__ PBE_LDS uint8_t* values(int turn) const { return keys(turn) + kTile; }
+  __device__ __forceinline__ PBE_LDS uint8_t* scales(int turn) const { return mem + kAll - 3 * kScaleBytes + turn % 3 * kScaleBytes; }
+
+  __device__ __forceinline__ int32_t entry(int first) const { return p.tables[(int64_t)b * p.max_blocks + min(first + lane, nblocks - 1)]; }
+  // Makes the ids of key tile kt's blocks (kt counts up by one) ready. Returns which
+  // of its four are not in the pools.
+  __device__ __forceinline__ uint32_t ids_for(int kt) {
     if constexpr (kKind != KeyKind::kRows) {
       const int c = kt / 16 * 64;
-      if (c == chunk) return;
-      if (chunk < 0) {
-        load_ids(c, &ids, &bad);
+      if (c != chunk) {
+        const int32_t id = chunk < 0 ? entry(c) : next;
+        const bool off = id < 0 || id >= p.blocks;
+        bad = __ballot(off);
+        ids = off ? 0 : id;
+        chunk = c;
+        next = entry(c + 64);
+      }
+      return (uint32_t)(bad >> (kt % 16 * 4)) & 15u;
+    }
+    return 0;
+  }
+  // A block's id, of the same block for all lanes, or each lane's own.
+  __device__ __forceinline__ uint64_t id_of(int block) const { return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(ids, min(block, nblocks - 1) & 63); }
+  __device__ __forceinline__ uint64_t own_id_of(int block) const { return (uint64_t)(uint32_t)__shfl(ids, min(block, nblocks - 1) & 63, 64); }
+
+  // Load i of this wave: K's or V's, and the place of its first byte among them.
+  __device__ __forceinline__ int load_of(int i) const {
+    // neighbouring ones of both in turn
+    return kLoads % 2 ? (wave + i * kWaves) % (2 * kInstr) : i % 2 * kInstr + wave * (kLoads / 2) + i / 2;
+  }
+
+  // Asks for key tile kt, the turn-th of this workgroup's. Returns which of its
+  // blocks are not in the pools. What lies behind the last key, in its block, is
+  // loaded with it; rows behind it are the last one again.
+  __device__ __forceinline__ uint32_t load(int kt, int turn) {
+    if (kKind == KeyKind::kRows && kt * kKeys + kKeys <= u.len && max(p.k_stride, p.v_stride) < (1u << 28)) return load_tile<true>(kt, turn);
+    return load_tile<false>(kt, turn);
+  }
+  // kFast (rows): the whole tile is there, and the distances within it fit 32 bits.
+  template <bool kFast>
+  __device__ __forceinline__ uint32_t load_tile(int kt, int turn) {
+    const uint32_t wrong = ids_for(kt);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int n = load_of(i);
+      const bool value = n >= kInstr;
+      const int at = (value ? n - kInstr : n) * 64;  // in 16 bytes, among K's (or V's)
+      const uint8_t* const from = value ? p.v : p.k;
+      PBE_LDS uint8_t* const to = raw(turn) + n * 1024;
+      if constexpr (!kMx) {
+        const uint64_t stride = value ? p.v_stride : p.k_stride;
+        const uint32_t r0 = (uint32_t)at / kChunks, r = (uint32_t)lane / kChunks, c = (uint32_t)lane % kChunks;
+        const uint32_t flip = kFp8 ? code_flip<D>(r0 + r) : value ? v_flip<D>(r0 + r) : k_flip<D>(r0 + r);
+        const uint64_t in_row = (uint64_t)head * kRowBytes;
+        if constexpr (kKind == KeyKind::kRows && kFast) {
+          load_to_lds(from + (uint64_t)(u.first + kt * kKeys + (int)r0) * stride + in_row, r * (uint32_t)stride + (c ^ flip) * 16, to);
+        } else if constexpr (kKind == KeyKind::kRows) {
+          load_to_lds(from + (uint64_t)(u.first + min(kt * kKeys + (int)(r0 + r), u.len - 1)) * stride + in_row + (c ^ flip) * 16, to);
+        } else {
+          load_to_lds(from + id_of(kt * 4 + (int)(r0 / kBlockTokens)) * p.half + r0 % kBlockTokens * stride + in_row,
+                      r * (uint32_t)stride + (c ^ flip) * 16, to);
+        }
       } else {
-        ids = next_ids;
-        bad = next_bad;
-      }
-      chunk = c;
-      load_ids(c + 64, &next_ids, &next_bad);
-    }
-  }
-  // Which of a key tile's four blocks are not in the pools.
-  __device__ __forceinline__ uint32_t wrong_blocks(int kt) const { return (uint32_t)(bad >> (kt % 16 * 4)) & 15u; }
-
-  // Byte offset of the K (or V) row of key j, of this head.
-  __device__ __forceinline__ uint64_t row_at(int j, uint64_t stride) const {
-    if constexpr (kKind == KeyKind::kRows) {
-      return (uint64_t)(u.first + j) * stride;
-    } else {
-      const uint32_t id = (uint32_t)__shfl(ids, (j / kBlockTokens) & 63, 64);
-      return (uint64_t)id * p.half + (uint64_t)(j % kBlockTokens) * stride;
-    }
-  }
-
-  // Asks for key tile kt.
-  __device__ __forceinline__ void load(int kt, PBE_LDS uint8_t* ks, PBE_LDS uint8_t* vs) {
-    ids_for(kt);
-    const int last = u.len - 1;
-    if constexpr (kDirect) {
-#pragma unroll
-      for (int i = 0; i < kInstrs; ++i) {
-        const int r0 = (wave * kInstrs + i) * kRowsAnInstr;
-        const uint32_t r = (uint32_t)r0 + (uint32_t)lane / (D / 8), c = (uint32_t)lane % (D / 8);
-        const int j = min(kt * kKeys + (int)r, last);
-        const uint64_t at = (uint64_t)head * (2 * D);
-        const uint8_t* kp = p.k + row_at(j, p.k_stride) + at + (c ^ (r & (D / 8 - 1))) * 16;
-        const uint8_t* vp = p.v + row_at(j, p.v_stride) + at + (c ^ ((2 * r) & (D / 8 - 1))) * 16;
-        load_to_lds(kp, ks + r0 * (2 * D));
-        load_to_lds(vp, vs + r0 * (2 * D));
-      }
-    } else if constexpr (kKind == KeyKind::kFp8) {
-#pragma unroll
-      for (int i = 0; i < kFp8Each; ++i) {
-        const int unit = min((int)threadIdx.x + i * T, kFp8Units - 1);
-        const int j = min(kt * kKeys + unit / (D / 16), last);
-        const uint64_t at = row_at(j, p.k_stride) + (uint64_t)head * D + (uint64_t)(unit % (D / 16)) * 16;
-        kr[i] = *(PBE_GLOBAL const u32x4*)(uintptr_t)(p.k + at);
-        vr[i] = *(PBE_GLOBAL const u32x4*)(uintptr_t)(p.v + at);
-      }
-      const int j = min(kt * kKeys + lane, last);
-      const uint32_t id = (uint32_t)__shfl(ids, (j / kBlockTokens) & 63, 64);
-      const uint64_t at = (((uint64_t)id * kBlockTokens + (uint64_t)(j % kBlockTokens)) * (uint64_t)p.kv_heads + (uint64_t)head) * 4;
-      if (wave == 0) sk[0] = *(PBE_GLOBAL const uint32_t*)(uintptr_t)(p.k_scales + at);
-      if (wave == 1) sk[0] = *(PBE_GLOBAL const uint32_t*)(uintptr_t)(p.v_scales + at);
-    } else {
-      const int last_block = nblocks - 1;
-#pragma unroll
-      for (int i = 0; i < kMxEach; ++i) {
-        const int unit = min((int)threadIdx.x + i * T, 255);
-        {  // K: 64 tokens, four quarters of the dims each
-          const int tok = unit / 4, quarter = unit % 4, block = min(kt * 4 + tok / kBlockTokens, last_block);
-          const uint64_t id = (uint64_t)(uint32_t)__shfl(ids, block & 63, 64);
-          const uint64_t at = id * p.half + (uint64_t)head * mx_head_bytes(D) + (uint64_t)(quarter * kBlockTokens + tok % kBlockTokens) * (D / 8);
-          if constexpr (D == 128) kr[i] = *(PBE_GLOBAL const u32x4*)(uintptr_t)(p.k + at);
-          else kr[i].xy = *(PBE_GLOBAL const u32x2*)(uintptr_t)(p.k + at);
-          sk[i] = *(PBE_GLOBAL const uint8_t*)(uintptr_t)(p.k_scales + id * (p.half / 16) + (uint64_t)head * mx_head_scales(D) +
-                                                          (D == 128 ? quarter : quarter / 2) * kBlockTokens + tok % kBlockTokens);
-        }
-        {  // V: 16 quads of tokens, 16 columns of dims each
-          const int quad = unit / 16, column = unit % 16, block = min(kt * 4 + quad / 4, last_block);
-          const uint64_t id = (uint64_t)(uint32_t)__shfl(ids, block & 63, 64);
-          const uint64_t at = id * p.half + (uint64_t)head * mx_head_bytes(D) + (uint64_t)(quad % 4) * (2 * D) + (uint64_t)column * (D / 8);
-          if constexpr (D == 128) vr[i] = *(PBE_GLOBAL const u32x4*)(uintptr_t)(p.v + at);
-          else vr[i].xy = *(PBE_GLOBAL const u32x2*)(uintptr_t)(p.v + at);
-          sv[i] = *(PBE_GLOBAL const uint32_t*)(uintptr_t)(p.v_scales + id * (p.half / 16) + (uint64_t)head * mx_head_scales(D) +
-                                                           (D == 128 ? column / 4 : column / 8) * kBlockTokens + quad % 4 * 4);
-        }
+        // K: [4 quarters][16 tokens][D/8 bytes] a block, V: [4 quads][16 columns][D/8]
+        constexpr int kBlock = D / 2;  // of 16 bytes, in a block
+        const uint64_t in_block = (uint64_t)head * mx_head_bytes(D);
+        if constexpr (D == 128) load_to_lds(from + id_of(kt * 4 + at / kBlock) * p.half + in_block, (uint32_t)lane * 16, to);
+        else load_to_lds(from + own_id_of(kt * 4 + (at + lane) / kBlock) * p.half + in_block + (uint32_t)(lane % kBlock) * 16, to);
       }
     }
+    if constexpr (kScaled) {
+      // K's by even waves, V's by odd ones; a wave alone asks for both
+#pragma unroll
+      for (int i = 0; i < (kWaves == 1 ? 2 : 1); ++i) {
+        const bool value = kWaves == 1 ? i : wave & 1;
+        const uint8_t* from = value ? p.v_scales : p.k_scales;
+        if constexpr (kMx) {  // [D/32 groups][16 tokens] a block
+          constexpr int kWords = D / 8;
+          from += own_id_of(kt * 4 + (lane / kWords) % 4) * (p.half / 16) + (uint64_t)head * mx_head_scales(D) + lane % kWords * 4;
+        } else {
+          from += ((own_id_of(kt * 4 + lane / kBlockTokens) * kBlockTokens + (uint64_t)(lane % kBlockTokens)) * (uint64_t)p.kv_heads + (uint64_t)head) * 4;
+        }
+        load_word_to_lds(from, scales(turn) + value * 256);
+      }
+    }
+    return wrong;
   }
 
-  // Puts what load() asked for into the tiles (a direct load does so by itself).
-  __device__ __forceinline__ void store(PBE_LDS uint8_t* ks, PBE_LDS uint8_t* vs, PBE_LDS float* scales) {
-    if constexpr (kKind == KeyKind::kFp8) {
+  // What this wave asked for of a tile is there; `after`: tiles asked for since.
+  __device__ __forceinline__ void wait(int after) const {
+    if (kMx ? after >= 1 : after >= kTurns - 2) arrived<(kMx ? 1 : kTurns - 2) * kPerTile>();
+    else arrived<0>();
+  }
+
+  // MXFP4: BF16 rows of the turn-th tile from its codes.
+  __device__ __forceinline__ void convert(int turn) const {
+    PBE_LDS uint8_t* const ks = keys(0);
+    PBE_LDS uint8_t* const vs = values(0);
+    PBE_LDS const uint8_t* const sc = scales(turn);
 #pragma unroll
-      for (int i = 0; i < kFp8Each; ++i) {
-        const int unit = (int)threadIdx.x + i * T;
-        if (kFp8Units % T && unit >= kFp8Units) break;
-        const uint32_t r = (uint32_t)unit / (D / 16), c = 2 * ((uint32_t)unit % (D / 16));
+    for (int i = 0; i < kLoads; ++i) {
+      if (kLoads % 2 && wave + i * kWaves >= 2 * kInstr) break;
+      const int n = load_of(i);
+      const bool value = n >= kInstr;
+      const uint32_t at = (uint32_t)((value ? n - kInstr : n) * 64 + lane);
+      const u32x4 x = *(PBE_LDS const u32x4*)(raw(turn) + n * 1024 + lane * 16);
+      const uint32_t block = at / (D / 2), o = at % (D / 2), groups = block * mx_head_scales(D);
+      if (!value) {
+        // 16 bytes: a token's quarter of the dims (D 128), or that of two tokens
+        constexpr uint32_t kTok = 128 / D, kEach = 4 / kTok;  // tokens; chunks of each
+        const uint32_t quarter = o / (kBlockTokens / kTok), tok = o % (kBlockTokens / kTok) * kTok, group = D == 128 ? quarter : quarter / 2;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const u32x2 a = e4m3x4_to_bf16x4_cvt(kr[i][2 * e]), b = e4m3x4_to_bf16x4_cvt(kr[i][2 * e + 1]);
-          *(PBE_LDS u32x4*)(ks + k_at<D>(r, c + e)) = u32x4{a.x, a.y, b.x, b.y};
-          const u32x2 x = e4m3x4_to_bf16x4_cvt(vr[i][2 * e]), y = e4m3x4_to_bf16x4_cvt(vr[i][2 * e + 1]);
-          *(PBE_LDS u32x4*)(vs + v_at<D>(r, c + e)) = u32x4{x.x, x.y, y.x, y.y};
+        for (uint32_t e = 0; e < 4; ++e) {
+          const uint32_t t = tok + e / kEach;
+          const float f = mx_scale(sc[groups + group * kBlockTokens + t]);
+          *(PBE_LDS u32x4*)(ks + k_at<D>(block * kBlockTokens + t, quarter * (D / 32) + e % kEach)) = mx_values(x[e], f);
         }
-      }
-      if (wave == 0) scales[lane] = __uint_as_float(sk[0]);
-      if (wave == 1) scales[kKeys + lane] = __uint_as_float(sk[0]);
-    } else if constexpr (kKind == KeyKind::kMxfp4) {
-#pragma unroll
-      for (int i = 0; i < kMxEach; ++i) {
-        const int unit = (int)threadIdx.x + i * T;
-        if (256 % T && unit >= 256) break;
-        const uint32_t tok = (uint32_t)unit / 4, quarter = (uint32_t)unit % 4;
-        const float scale = mx_scale(sk[i]);
-#pragma unroll
-        for (uint32_t e = 0; e < D / 32; ++e) *(PBE_LDS u32x4*)(ks + k_at<D>(tok, quarter * (D / 32) + e)) = mx_values(kr[i][e], scale);
-        const uint32_t quad = (uint32_t)unit / 16, column = (uint32_t)unit % 16;
+      } else {
+        // four tokens' dims of a column (D 128: eight), or of two columns (four each)
+        constexpr uint32_t kCols = 128 / D;
+        const uint32_t quad = o / (16 / kCols), column = o % (16 / kCols) * kCols, group = D == 128 ? column / 4 : column / 8;
+        const uint32_t four = *(PBE_LDS const uint32_t*)(sc + 256 + groups + group * kBlockTokens + quad * 4);
 #pragma unroll
         for (uint32_t t = 0; t < 4; ++t) {
-          const float s = mx_scale((sv[i] >> (8 * t)) & 255u);
+          const float f = mx_scale((four >> (8 * t)) & 255u);
+          const uint32_t row = block * kBlockTokens + quad * 4 + t;
           if constexpr (D == 128) {
-            *(PBE_LDS u32x4*)(vs + v_at<D>(4 * quad + t, column)) = mx_values(vr[i][t], s);
+            *(PBE_LDS u32x4*)(vs + v_at<D>(row, column)) = mx_values(x[t], f);
           } else {
-            const uint32_t codes = vr[i][t / 2] >> (16 * (t % 2));
-            *(PBE_LDS u32x2*)(vs + v_at<D>(4 * quad + t, column / 2) + 8 * (column % 2)) = u32x2{mx_pair<0>(codes, s), mx_pair<1>(codes, s)};
+            const uint32_t a = x[t / 2] >> (16 * (t % 2)), c = x[2 + t / 2] >> (16 * (t % 2));
+            *(PBE_LDS u32x4*)(vs + v_at<D>(row, column / 2)) = u32x4{mx_pair<0>(a, f), mx_pair<1>(a, f), mx_pair<0>(c, f), mx_pair<1>(c, f)};
           }
         }
       }
@@ -310,336 +443,507 @@ struct Stage {
   }
 };
 
-// Non-zero where one of a word's two BF16 values is an infinity or a NaN.
-__device__ __forceinline__ uint32_t special(uint32_t x) { return ((x & 0x7fff7fffu) + 0x00800080u) & 0x80008000u; }
+__device__ __forceinline__ u32x4 e4m3x8_to_bf16x8(u32x2 x) {
+  const u32x2 lo = e4m3x4_to_bf16x4_cvt(x.x), hi = e4m3x4_to_bf16x4_cvt(x.y);
+  return u32x4{lo.x, lo.y, hi.x, hi.y};
+}
+
+// Non-zero where one of a word's BF16 values is an infinity or a NaN, or one of its
+// E4M3 codes a NaN; and the word with zeros in their place.
+template <bool kFp8>
+__device__ __forceinline__ uint32_t special(uint32_t x) {
+  return kFp8 ? ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u : ((x & 0x7fff7fffu) + 0x00800080u) & 0x80008000u;
+}
+template <bool kFp8>
+__device__ __forceinline__ uint32_t without_special(uint32_t x) {
+  const uint32_t s = special<kFp8>(x);
+  return kFp8 ? x & ~(s | (s - (s >> 7))) : x & ~(s | (s - (s >> 15)));
+}
+
+// Which part (or tile) and head a workgroup has. Pages whose lines several heads
+// share have their heads on one XCD, others (nearly) each head on its own.
+template <KeyKind kKind>
+__device__ __forceinline__ void workgroup_of(const PromptParams& p, int* w, int* head) {
+  const int x = blockIdx.x;
+  if constexpr (kKind == KeyKind::kFp8 || kKind == KeyKind::kMxfp4) {
+    const int q = x / kXcds;
+    *w = q / p.kv_heads * kXcds + x % kXcds;
+    *head = q % p.kv_heads;
+  } else {
+    *w = x / p.kv_heads;
+    *head = x - *w * p.kv_heads;
+  }
+}
 
 template <int D, KeyKind kKind, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, kWaves / 2) void prompt_attention_kernel(const PromptParams p) {
-  constexpr int kRows = 32 * kWaves, kTile = kKeys * D * 2, kDims = D / 32;
+__global__ __launch_bounds__(64 * kWaves, kWaves > 2 ? 2 : 1) void prompt_attention_kernel(const PromptParams p) {
   using S = Stage<D, kKind, kWaves>;
-  // two turns of a tile's keys and values; of FP8 ones, their scales
-  __shared__ __align__(1024) uint8_t tile_mem[4 * kTile];
-  __shared__ __align__(16) float scale_mem[kKind == KeyKind::kFp8 ? 4 * kKeys : 4];
+  constexpr int kRows = 32 * kWaves, kDims = D / 32;
+  constexpr bool kFp8 = S::kFp8;
+  __shared__ __align__(1024) uint8_t tile_mem[S::kAll];
   __shared__ uint32_t special_mem[kWaves];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int z = blockIdx.x / p.kv_heads, head = blockIdx.x - z * p.kv_heads;
-  const Unit u = find_unit<kKind, kRows>(p, z, lane);
-  if (u.b < 0) return;
+  int w, head;
+  workgroup_of<kKind>(p, &w, &head);
   const int h = lane >> 5, col = lane & 31;
-  const int stacked = u.rows * p.group;                       // rows of the sequence and this head
-  const int row0 = u.tile * kRows + wave * 32;                // of the wave
-  auto token_of = [&](int r) { return (int)fast_div((uint32_t)min(r, stacked - 1), p.by_group); };
-  const int token = token_of(row0 + col), g = min(row0 + col, stacked - 1) - token * p.group;
-  const int q_heads = p.kv_heads * p.group;
-  const int64_t q_row = (int64_t)u.begin + token;
-  const int q_head = head * p.group + g;
-  auto seen_by = [&](int tok) { return max(0, u.len - u.rows + tok + 1); };
-  const int seen = seen_by(token);
-  const int wave_least = seen_by(token_of(row0)), wave_most = row0 < stacked ? seen_by(token_of(row0 + 31)) : 0;
-  const int tile_least = seen_by(token_of(u.tile * kRows)), tile_most = seen_by(token_of(u.tile * kRows + kRows - 1));
-  const int all = key_tiles(tile_most);
-  const int kt0 = (int)((int64_t)all * u.s / u.k), kt1 = (int)((int64_t)all * (u.s + 1) / u.k);
-
-  bf16x8 q[D / 16];
-  {
-    const uint8_t* at = p.q + (uint64_t)q_row * p.q_stride + (uint64_t)q_head * (2 * D) + h * 16;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) q[i] = *(PBE_GLOBAL const bf16x8*)(uintptr_t)(at + i * 32);
+  Place at, end;
+  if (p.parts) {
+    if (w >= p.parts) return;
+    find_part<kKind, kRows>(p, w, lane, &at, &end);
+  } else {
+    if (!find_tile<kKind, kRows>(p, w, lane, &at)) return;
+    end = {at.b, at.t + 1, 0, 0};
   }
-  f32x16 o[kDims];
-#pragma unroll
-  for (int i = 0; i < kDims; ++i) o[i] = f32x16{};
-  float m = -INFINITY, l = 0.f;
+  bool opened = false;  // a tile was worked on before
+  for (int b = at.b; b < p.batch && b <= end.b; ++b) {
+    const Seq u = seq_of<kKind, kRows>(p, b);
+    const int t1 = b == end.b ? min(u.tiles, end.t + (end.k > 0)) : u.tiles;
+    for (int t = b == at.b ? at.t : 0; t < t1; ++t) {
+      const int row0 = t * kRows + wave * 32;                     // of the wave
+      const int stacked = u.rows * p.group;                       // rows of the sequence and this head
+      const int token = token_of(p, u, row0 + col), g = min(row0 + col, stacked - 1) - token * p.group;
+      const int q_heads = p.kv_heads * p.group, q_head = head * p.group + g;
+      const int64_t q_row = (int64_t)u.begin + token;
+      const int seen = seen_by(u, token);
+      const int wave_least = seen_by(u, token_of(p, u, row0)), wave_most = row0 < stacked ? seen_by(u, token_of(p, u, row0 + 31)) : 0;
+      const int tile_least = seen_by(u, token_of(p, u, t * kRows));
+      const int all = tiles_seen<kRows>(p, u, t);
+      const bool opens = b == at.b && t == at.t, ends = b == end.b && t == end.t;
+      const int kt0 = opens ? at.k : 0, kt1 = ends ? end.k : all;
+      if (kt0 == kt1 && all > 0) continue;
 
-  S stage(p, u, head, lane, wave);
-  PBE_LDS uint8_t* const tiles = (PBE_LDS uint8_t*)tile_mem;
-  PBE_LDS float* const tile_scales = (PBE_LDS float*)scale_mem;
-  auto keys_at = [&](int turn) { return tiles + turn * (2 * kTile); };
-  auto values_at = [&](int turn) { return tiles + turn * (2 * kTile) + kTile; };
-  uint32_t wrong = 0, next_wrong = 0;
-  if (kt0 < kt1) {
-    stage.load(kt0, keys_at(0), values_at(0));
-    stage.store(keys_at(0), values_at(0), tile_scales);
-    next_wrong = stage.wrong_blocks(kt0);
-  }
-  for (int kt = kt0; kt < kt1; ++kt) {
-    const int turn = (kt - kt0) & 1;
-    const int first = kt * kKeys;
-    if constexpr (S::kDirect) arrived();
-    __syncthreads();
-    wrong = next_wrong;
-    PBE_LDS const uint8_t* kb = keys_at(turn);
-    PBE_LDS const uint8_t* vb = values_at(turn);
-    const bool more = kt + 1 < kt1;
-    if (more) {
-      stage.load(kt + 1, keys_at(turn ^ 1), values_at(turn ^ 1));
-      if constexpr (kKind != KeyKind::kRows) next_wrong = stage.wrong_blocks(kt + 1);
-    }
-    // Values that some of the tile's rows do not see may be anything: an infinity
-    // or a NaN times a weight of zero would reach those rows.
-    bool odd = false;
-    if (first + kKeys > tile_least) {
-      uint32_t some = 0;
+      f32x16 o[kDims];
 #pragma unroll
-      for (int i = 0; i < kTile / (64 * kWaves * 16); ++i) {
-        const u32x4 x = *(PBE_LDS const u32x4*)(vb + (i * 64 * kWaves + threadIdx.x) * 16);
-        some |= special(x.x) | special(x.y) | special(x.z) | special(x.w);
+      for (int i = 0; i < kDims; ++i) o[i] = f32x16{};
+      float m = -INFINITY, l = 0.f;
+      bool far = false;
+
+      S stage(p, u, (PBE_LDS uint8_t*)tile_mem, b, head, lane, wave);
+      if (opened) __syncthreads();  // the tile before has been read
+      opened = true;
+      // Blocks not in the pools: of this key tile and those asked for.
+      constexpr int kAhead = S::kMx ? 2 : S::kTurns - 1;  // tiles asked for before one is used
+      uint32_t wrong = 0, wrongs[kAhead] = {};
+      if (kt0 < kt1) wrongs[0] = stage.load(kt0, 0);
+      bf16x8 q[D / 16];
+      {
+        const uint8_t* from = p.q + (uint64_t)q_row * p.q_stride + (uint64_t)q_head * (2 * D) + h * 16;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) q[i] = *(PBE_GLOBAL const bf16x8*)(uintptr_t)(from + i * 32);
       }
-      const bool any = __ballot(some != 0) != 0;
-      if (lane == 0) special_mem[wave] = any;
-      __syncthreads();
+      arrived<0>();  // here, so that no wait for q stands in the loop
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) odd |= special_mem[i] != 0;
-    }
-    if (first < wave_most) {
-      f32x16 s[2];
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        s[sub] = f32x16{};
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const bf16x8 a = *(PBE_LDS const bf16x8*)(kb + k_at<D>(sub * 32 + col, 2 * i + h));
-          s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[i], s[sub], 0, 0, 0);
+      for (int i = 1; i < kAhead; ++i)
+        if (kt0 + i < kt1) wrongs[i] = stage.load(kt0 + i, i);
+      for (int kt = kt0; kt < kt1; ++kt) {
+        const int turn = kt - kt0, first = kt * kKeys;
+        stage.wait(kt1 - 1 - kt);
+        __syncthreads();
+        if constexpr (S::kMx) {
+          stage.convert(turn);
+          __syncthreads();
         }
-      }
-      auto key_of = [&](int sub, int i) { return first + sub * 32 + 8 * (i / 4) + 4 * h + i % 4; };
-      PBE_LDS const float* scales = tile_scales + turn * (2 * kKeys);
-      if constexpr (kKind == KeyKind::kFp8) {
+        wrong = wrongs[0];
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const f32x4 f = *(PBE_LDS const f32x4*)(scales + sub * 32 + 8 * i + 4 * h);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[sub][4 * i + e] *= f[e];
+        for (int i = 0; i + 1 < kAhead; ++i) wrongs[i] = wrongs[i + 1];
+        if (kt + kAhead < kt1) wrongs[kAhead - 1] = stage.load(kt + kAhead, turn + kAhead);
+        PBE_LDS const uint8_t* const kb = stage.keys(turn);
+        PBE_LDS uint8_t* const vb = stage.values(turn);
+        PBE_LDS const float* const scales = (PBE_LDS const float*)stage.scales(turn);
+        auto key_of = [&](int sub, int i) { return first + sub * 32 + 8 * (i / 4) + 4 * h + i % 4; };
+        // A operand of keys 32 sub.. and dims 16 i..: a key's eight dims a lane.
+        auto keys = [&](int sub, int i) {
+          if constexpr (kFp8) return e4m3x8_to_bf16x8(*(PBE_LDS const u32x2*)(kb + code_at<D>(sub * 32 + col, i) + 8 * h));
+          else return *(PBE_LDS const u32x4*)(kb + k_at<D>(sub * 32 + col, 2 * i + h));
+        };
+        // A operand of dims 32 d.. and keys 16 n..: a dim's eight keys a lane, those that
+        // the scores' registers have: 4h.. and 8 + 4h... Transposing reads: of 16 lanes each
+        // asks for a part of a key's 16 dims and gets one dim of four (or eight) keys.
+        auto values = [&](int d, int n) {
+          const uint32_t i = lane & 15, half = (lane >> 4) & 1;
+          if constexpr (kFp8) {
+            const uint32_t r = 16 * n + 4 * h + i / 2 + (i >= 8 ? 4 : 0);
+            const auto x = __builtin_amdgcn_ds_read_tr8_b64_v2i32((PBE_LDS i32x2*)(vb + code_at<D>(r, 2 * d + half) + 8 * (i % 2)));
+            return e4m3x8_to_bf16x8(__builtin_bit_cast(u32x2, x));
+          } else {
+            const uint32_t chunk = 4 * d + 2 * half + (i % 4) / 2, r = 16 * n + 4 * h + i / 4;
+            const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((PBE_LDS s16x4*)(vb + v_at<D>(r, chunk) + 8 * (i % 2))));
+            const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((PBE_LDS s16x4*)(vb + v_at<D>(r + 8, chunk) + 8 * (i % 2))));
+            return u32x4{x.x, x.y, y.x, y.y};
           }
-      }
-      if (kKind != KeyKind::kRows && wrong) {
+        };
+        // Values that some of the tile's rows do not see may be anything: an infinity or a
+        // NaN times a weight of zero would reach those rows. Where there are any, rows that
+        // see them get them here, and the product below finds zeros in their place.
+        if (first + kKeys > tile_least) {
+          // 16 bytes a thread at a time
+          constexpr int kStep = 64 * kWaves * 16, kEach = (S::kTile + kStep - 1) / kStep;
+          const bool has = kStep <= S::kTile || (int)threadIdx.x * 16 < S::kTile;
+          uint32_t some = 0;
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
+          for (int i = 0; i < kEach; ++i) {
+            if (!has) break;
+            const u32x4 x = *(PBE_LDS const u32x4*)(vb + i * kStep + threadIdx.x * 16);
+            some |= special<kFp8>(x.x) | special<kFp8>(x.y) | special<kFp8>(x.z) | special<kFp8>(x.w);
+          }
+          const bool any = __ballot(some != 0) != 0;
+          if (lane == 0) special_mem[wave] = any;
+          __syncthreads();
+          bool odd = false;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (wrong >> (2 * sub + i / 8) & 1) s[sub][i] = NAN;
-      }
-      const bool masked = first + kKeys > wave_least;
-      if (masked) {
+          for (int i = 0; i < kWaves; ++i) odd |= special_mem[i] != 0;
+          if (odd) {
+            if (first < wave_most) {
+              bf16x8 sees[4];
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
+              for (int n = 0; n < 4; ++n) {
+                u32x4 x;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[sub][i] = key_of(sub, i) < seen ? s[sub][i] : -INFINITY;
-      }
-      float top = s[0][0];
+                for (int e = 0; e < 4; ++e)
+                  x[e] = (key_of(n / 2, 8 * (n % 2) + 2 * e) < seen ? 0x3f80u : 0u) | (key_of(n / 2, 8 * (n % 2) + 2 * e + 1) < seen ? 0x3f800000u : 0u);
+                sees[n] = __builtin_bit_cast(bf16x8, x);
+              }
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[0][i]);
+              for (int d = 0; d < kDims; ++d) {
+                f32x16 up = {}, down = {};  // how many a row sees; a NaN counts as both
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[1][i]);
-      top = halves_max(top);
-      // The maximum that weights refer to follows the largest score only when that
-      // has passed it by 2^kLazy: sums then need no scaling for most tiles.
-      if (__any((top - m) * p.scale > kLazy || (m == -INFINITY && top > m))) {
-        const float now = fmaxf(m, top);
-        const float fade = m == now ? 1.f : __builtin_amdgcn_exp2f((m - now) * p.scale);
-        m = now;
-        l *= fade;
+                for (int n = 0; n < 4; ++n) {
+                  const u32x4 x = values(d, n);
+                  u32x4 plus, minus;
 #pragma unroll
-        for (int d = 0; d < kDims; ++d)
+                  for (int e = 0; e < 4; ++e) {
+                    const uint32_t lo = x[e] & 0xffffu, hi = x[e] >> 16;
+                    const bool lo_off = (lo & 0x7f80u) == 0x7f80u, hi_off = (hi & 0x7f80u) == 0x7f80u;
+                    plus[e] = (lo_off && lo != 0xff80u ? 0x3f80u : 0u) | (hi_off && hi != 0xff80u ? 0x3f800000u : 0u);
+                    minus[e] = (lo_off && lo != 0x7f80u ? 0x3f80u : 0u) | (hi_off && hi != 0x7f80u ? 0x3f800000u : 0u);
+                  }
+                  up = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, plus), sees[n], up, 0, 0, 0);
+                  down = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, minus), sees[n], down, 0, 0, 0);
+                }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[d][i] *= fade;
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      bf16x8 w[4];
-      float sum = 0.f;
+                for (int i = 0; i < 16; ++i) o[d][i] += (up[i] > 0.f ? INFINITY : 0.f) - (down[i] > 0.f ? INFINITY : 0.f);
+              }
+            }
+            __syncthreads();
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
+            for (int i = 0; i < kEach; ++i) {
+              if (!has) break;
+              PBE_LDS u32x4* const to = (PBE_LDS u32x4*)(vb + i * kStep + threadIdx.x * 16);
+              u32x4 x = *to;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[sub][i] = __builtin_amdgcn_exp2f((s[sub][i] - base) * p.scale);
-          if constexpr (kKind == KeyKind::kFp8) sum += s[sub][i];
+              for (int e = 0; e < 4; ++e) x[e] = without_special<kFp8>(x[e]);
+              *to = x;
+            }
+            __syncthreads();
+          }
         }
-      if constexpr (kKind == KeyKind::kFp8) {
+        if (first < wave_most) {
+          f32x16 s[2];
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
+          for (int sub = 0; sub < 2; ++sub) s[sub] = f32x16{};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const f32x4 f = *(PBE_LDS const f32x4*)(scales + kKeys + sub * 32 + 8 * i + 4 * h);
+          for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[sub][4 * i + e] *= f[e];
+            for (int sub = 0; sub < 2; ++sub) {
+              const bf16x8 a = __builtin_bit_cast(bf16x8, keys(sub, i));
+              s[sub] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[i], s[sub], 0, 0, 0);
+            }
+          // six reads ahead of the products
+          constexpr int kProducts = D / 8, kFirst = 6;
+          __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
+#pragma unroll
+          for (int i = 0; i < kProducts - kFirst; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
           }
-        if (masked) {
+          __builtin_amdgcn_sched_group_barrier(0x8, kFirst, 0);
+          if constexpr (kKind == KeyKind::kFp8) {
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const f32x4 f = *(PBE_LDS const f32x4*)(scales + sub * 32 + 8 * i + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[sub][4 * i + e] *= f[e];
+              }
+          }
+          if (kKind != KeyKind::kRows && wrong) {
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (wrong >> (2 * sub + i / 8) & 1) s[sub][i] = NAN;
+          }
+          const bool masked = first + kKeys > wave_least;
+          if (masked) {
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) s[sub][i] = key_of(sub, i) < seen ? s[sub][i] : -INFINITY;
+          }
+          float top = s[0][0];
 #pragma unroll
           for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[sub][i] = key_of(sub, i) < seen ? s[sub][i] : 0.f;
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[sub][i]);
+          top = halves_max(top);
+          // The maximum that weights refer to follows the largest score only when that
+          // has passed it by 2^kLazy: sums then need no scaling for most tiles.
+          if (__any((top - m) * p.scale > kLazy)) {
+            const float now = fmaxf(m, top);
+            const float fade = m == now || m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - now) * p.scale);
+            m = now;
+            far = __any(m != -INFINITY && fabsf(m * p.scale) > kFar);
+            l *= fade;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[d][i] *= fade;
+          }
+          // 2^((score - maximum) * scale), by one multiply-add: its rounding of maximum *
+          // scale is in all weights of a row alike, and below kFar far below their own.
+          const float base = m == -INFINITY ? 0.f : m;
+          float scaled = base * p.scale;
+          if (far) {
+            scaled = 0.f;
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) s[sub][i] -= base;
+          }
+          float sum = 0.f;
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              s[sub][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[sub][i], p.scale, -scaled));
+              if constexpr (kKind == KeyKind::kFp8) sum += s[sub][i];
+            }
+          if constexpr (kKind == KeyKind::kFp8) {
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const f32x4 f = *(PBE_LDS const f32x4*)(scales + kKeys + sub * 32 + 8 * i + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[sub][4 * i + e] *= f[e];
+              }
+            if (masked) {  // a scale that the row does not see may be an infinity or a NaN
+#pragma unroll
+              for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[sub][i] = key_of(sub, i) < seen ? s[sub][i] : 0.f;
+            }
+          }
+          bf16x8 weights[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            u32x4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = pack_bf16(s[n / 2][8 * (n % 2) + 2 * e], s[n / 2][8 * (n % 2) + 2 * e + 1]);
+            weights[n] = __builtin_bit_cast(bf16x8, x);
+            if constexpr (kKind != KeyKind::kFp8) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sum = sum_bf16(x[e], sum);
+            }
+          }
+          l += sum;
+#pragma unroll
+          for (int d = 0; d < kDims; ++d)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values(d, n)), weights[n], o[d], 0, 0, 0);
+          // four products' reads ahead
+          constexpr int kMore = kDims * 4 - 4, kReads = kFp8 ? 1 : 2;
+          __builtin_amdgcn_sched_group_barrier(0x100, 4 * kReads, 1);
+#pragma unroll
+          for (int i = 0; i < kMore; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 1);
+            __builtin_amdgcn_sched_group_barrier(0x100, kReads, 1);
+          }
+          __builtin_amdgcn_sched_group_barrier(0x8, 4, 1);
         }
       }
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        u32x4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = pack_bf16(s[n / 2][8 * (n % 2) + 2 * e], s[n / 2][8 * (n % 2) + 2 * e + 1]);
-        w[n] = __builtin_bit_cast(bf16x8, x);
-        if constexpr (kKind != KeyKind::kFp8) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum = sum_bf16(x[e], sum);
-        }
-      }
-      l += sum;
-      // lane l of 16: four dims of key l / 4; it gets dim l of four keys
-      auto values = [&](int d, int n) {
-        const uint32_t i = lane & 15, chunk = 4 * d + 2 * ((lane >> 4) & 1) + (i % 4) / 2;
-        s16x4 a, b;
-        const uint32_t r = 16 * n + 4 * h + i / 4;
-        a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((PBE_LDS s16x4*)(vb + v_at<D>(r, chunk) + 8 * (i % 2)));
-        b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((PBE_LDS s16x4*)(vb + v_at<D>(r + 8, chunk) + 8 * (i % 2)));
-        const u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
-        return u32x4{x.x, x.y, y.x, y.y};
-      };
-      if (!odd) {
+
+      l = halves_sum(l);
+      if (row0 + col >= stacked) continue;
+      if (kt0 == 0 && kt1 == all) {
+        const float over = u.bad ? NAN : seen > 0 ? 1.f / l : 0.f;
+        uint8_t* to = p.out + ((uint64_t)q_row * (uint64_t)q_heads + (uint64_t)q_head) * (2 * D) + h * 8;
 #pragma unroll
         for (int d = 0; d < kDims; ++d)
 #pragma unroll
-          for (int n = 0; n < 4; ++n)
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, values(d, n)), w[n], o[d], 0, 0, 0);
+          for (int i = 0; i < 4; ++i)
+            *(PBE_GLOBAL u32x2*)(uintptr_t)(to + d * 64 + i * 16) =
+                u32x2{pack_bf16(o[d][4 * i] * over, o[d][4 * i + 1] * over), pack_bf16(o[d][4 * i + 2] * over, o[d][4 * i + 3] * over)};
       } else {
-        // Infinities and NaN are counted apart, for the rows that see them.
-        bf16x8 sees[4];
+        const uint64_t slot = ((uint64_t)w * 2 + !opens) * (uint64_t)p.kv_heads + (uint64_t)head;
+        const uint64_t row = slot * kRows + (uint64_t)(row0 - t * kRows + col);
+        float* acc = p.part_acc + row * D + 4 * h;
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          u32x4 x;
+        for (int d = 0; d < kDims; ++d)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[e] = (key_of(n / 2, 8 * (n % 2) + 2 * e) < seen ? 0x3f80u : 0u) | (key_of(n / 2, 8 * (n % 2) + 2 * e + 1) < seen ? 0x3f800000u : 0u);
-          sees[n] = __builtin_bit_cast(bf16x8, x);
-        }
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) {
-          f32x16 up = {}, down = {};
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const u32x4 x = values(d, n);
-            u32x4 fine, plus, minus;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t lo = x[e] & 0xffffu, hi = x[e] >> 16;
-              const bool lo_off = (lo & 0x7f80u) == 0x7f80u, hi_off = (hi & 0x7f80u) == 0x7f80u;
-              fine[e] = (lo_off ? 0u : lo) | (hi_off ? 0u : hi << 16);
-              // a NaN counts as both infinities
-              plus[e] = (lo_off && lo != 0xff80u ? 0x3f80u : 0u) | (hi_off && hi != 0xff80u ? 0x3f800000u : 0u);
-              minus[e] = (lo_off && lo != 0x7f80u ? 0x3f80u : 0u) | (hi_off && hi != 0x7f80u ? 0x3f800000u : 0u);
-            }
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fine), w[n], o[d], 0, 0, 0);
-            up = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, plus), sees[n], up, 0, 0, 0);
-            down = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, minus), sees[n], down, 0, 0, 0);
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (up[i] > 0.f) o[d][i] += INFINITY;
-            if (down[i] > 0.f) o[d][i] -= INFINITY;
-          }
-        }
+          for (int i = 0; i < 4; ++i)
+            *(PBE_GLOBAL f32x4*)(uintptr_t)(acc + d * 32 + i * 8) = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+        if (h == 0) *(PBE_GLOBAL f32x2*)(uintptr_t)(p.part_ml + row * 2) = f32x2{m, l};
       }
     }
-    if (more) stage.store(keys_at(turn ^ 1), values_at(turn ^ 1), tile_scales + (turn ^ 1) * (2 * kKeys));
-  }
-
-  l = halves_sum(l);
-  if (row0 + col >= stacked) return;
-  if (u.k == 1) {
-    const float over = u.bad ? NAN : seen > 0 ? 1.f / l : 0.f;
-    uint8_t* at = p.out + ((uint64_t)q_row * (uint64_t)q_heads + (uint64_t)q_head) * (2 * D) + h * 8;
-#pragma unroll
-    for (int d = 0; d < kDims; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *(PBE_GLOBAL u32x2*)(uintptr_t)(at + d * 64 + i * 16) =
-            u32x2{pack_bf16(o[d][4 * i] * over, o[d][4 * i + 1] * over), pack_bf16(o[d][4 * i + 2] * over, o[d][4 * i + 3] * over)};
-  } else {
-    const uint64_t row = ((uint64_t)z * (uint64_t)p.kv_heads + (uint64_t)head) * kRows + (uint64_t)(wave * 32 + col);
-    float* acc = p.part_acc + row * D + 4 * h;
-#pragma unroll
-    for (int d = 0; d < kDims; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) *(PBE_GLOBAL f32x4*)(uintptr_t)(acc + d * 32 + i * 8) = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-    if (h == 0) *(PBE_GLOBAL f32x2*)(uintptr_t)(p.part_ml + row * 2) = f32x2{m, l};
   }
 }
 
-// Joins the pieces of the tiles that were cut: piece s of k takes the s-th part of
-// the tile's rows.
-template <int D, KeyKind kKind, int kWaves>
-__global__ __launch_bounds__(256) void prompt_join_kernel(const PromptParams p) {
-  constexpr int kRows = 32 * kWaves, kLanes = D / 4;
+// Joins the tiles that were cut. Of a tile's n + 1 parts, each of the n that do not
+// begin it has a workgroup here, which takes its share of the tile's rows.
+constexpr int kJoinThreads = 1024;
+template <int D, KeyKind kKind, int kRows>
+__global__ __launch_bounds__(kJoinThreads) void prompt_join_kernel(const PromptParams p) {
+  constexpr int kLanes = D / 4;
+  __shared__ int cuts[kMaxCuts + 2];  // the key tiles at which the tile's parts begin
   const int lane = threadIdx.x & 63;
-  const int z = blockIdx.x / p.kv_heads, head = blockIdx.x - z * p.kv_heads;
-  const Unit u = find_unit<kKind, kRows>(p, z, lane);
-  if (u.b < 0 || u.k == 1) return;
-  const int stacked = u.rows * p.group;
-  const int from = kRows * u.s / u.k, to = kRows * (u.s + 1) / u.k;
+  int w, head;
+  workgroup_of<kKind>(p, &w, &head);
+  if (w >= p.parts) return;
+  Place at;
+  const int64_t total = find_part<kKind, kRows>(p, w, lane, &at, nullptr);
+  if (at.b >= p.batch || at.k == 0) return;
+  const Seq u = seq_of<kKind, kRows>(p, at.b);
+  const int64_t cost = u.cost(at.t);
+  const int all = tiles_seen<kRows>(p, u, at.t);
+  // Part i's start: its cut of this tile, -1 before the tile, `all` behind it.
+  auto cut_of = [&](int i) {
+    const int64_t y = part_at(p, total, i) - at.start;
+    return y < 0 ? -1 : y >= cost ? all : cut_at(y, cost, all);
+  };
+  // the last part that begins at or before the tile's start
+  int w0 = w;
+  for (;;) {
+    const uint64_t inside = __ballot(w0 - 1 - lane >= 0 && cut_of(w0 - 1 - lane) > 0);
+    const int n = ~inside ? __builtin_ctzll(~inside) : 64;
+    w0 -= n;
+    if (n < 64) break;
+  }
+  --w0;  // w0 + 1 is the first that begins inside; part 0 begins at no tile's inside
+  int n = 0;  // parts that begin inside
+  for (int i = w0;; i += 64) {
+    const int c = i + lane <= p.parts ? cut_of(i + lane) : all;
+    const uint64_t past = __ballot(c >= all);
+    const int many = past ? __builtin_ctzll(past) : 64;
+    if (threadIdx.x < 64 && lane <= many && i - w0 + lane < kMaxCuts + 2) cuts[i - w0 + lane] = c;
+    n = i - w0 + many - 1;
+    if (past) break;
+  }
+  __syncthreads();
+  const int share = w - w0 - 1, rows = min(kRows, u.rows * p.group - at.t * kRows);
+  const int from = (int)((int64_t)rows * share / n), to = (int)((int64_t)rows * (share + 1) / n);
   const int q_heads = p.kv_heads * p.group;
-  const uint64_t z0 = (uint64_t)(z - u.s);
-  for (int r = from + (int)threadIdx.x / kLanes; r < to; r += 256 / kLanes) {
-    const int row = u.tile * kRows + r;
-    if (row >= stacked) break;
-    const int token = (int)fast_div((uint32_t)row, p.by_group), g = row - token * p.group, d = 4 * (threadIdx.x % kLanes);
-    const int seen = max(0, u.len - u.rows + token + 1);
-    auto place = [&](int s) { return ((z0 + (uint64_t)s) * (uint64_t)p.kv_heads + (uint64_t)head) * kRows + (uint64_t)r; };
-    float m = -INFINITY;
-    for (int s = 0; s < u.k; ++s) m = fmaxf(m, p.part_ml[place(s) * 2]);
-    const float base = m == -INFINITY ? 0.f : m;
-    f32x4 acc = {};
-    float l = 0.f;
-    for (int s = 0; s < u.k; ++s) {
-      const uint64_t at = place(s);
-      const float f = __builtin_amdgcn_exp2f((p.part_ml[at * 2] - base) * p.scale);
-      l += p.part_ml[at * 2 + 1] * f;
-      const f32x4 x = *(PBE_GLOBAL const f32x4*)(uintptr_t)(p.part_acc + at * D + d);
+  const bool begins = cuts[0] == 0;  // else its first tile was another one
+  // kTogether rows of a thread at once, so that their loads are on their way together
+  constexpr int kStep = kJoinThreads / kLanes, kTogether = 4;
+  const int d = 4 * ((int)threadIdx.x % kLanes);
+  for (int r0 = from + (int)threadIdx.x / kLanes; r0 < to; r0 += kTogether * kStep) {
+    float m[kTogether], l[kTogether];
+    f32x4 acc[kTogether];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += x[e] * f;
+    for (int e = 0; e < kTogether; ++e) m[e] = -INFINITY, l[e] = 0.f, acc[e] = f32x4{};
+    for (int i = 0; i <= n; ++i) {
+      if (max(cuts[i], 0) == cuts[i + 1]) continue;  // nothing between two cuts
+      const uint64_t place = (((uint64_t)(w0 + i) * 2 + (i == 0 && !begins)) * (uint64_t)p.kv_heads + (uint64_t)head) * kRows;
+      f32x2 ml[kTogether];
+      f32x4 x[kTogether];
+#pragma unroll
+      for (int e = 0; e < kTogether; ++e) {
+        const uint64_t at_row = place + (uint64_t)min(r0 + e * kStep, to - 1);
+        ml[e] = *(PBE_GLOBAL const f32x2*)(uintptr_t)(p.part_ml + at_row * 2);
+        x[e] = *(PBE_GLOBAL const f32x4*)(uintptr_t)(p.part_acc + at_row * D + d);
+      }
+#pragma unroll
+      for (int e = 0; e < kTogether; ++e) {
+        const float now = fmaxf(m[e], ml[e].x), base = now == -INFINITY ? 0.f : now;
+        const float old = m[e] == now ? 1.f : __builtin_amdgcn_exp2f((m[e] - base) * p.scale);
+        const float add = ml[e].x == now ? 1.f : __builtin_amdgcn_exp2f((ml[e].x - base) * p.scale);
+        m[e] = now;
+        l[e] = l[e] * old + ml[e].y * add;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[e][c] = acc[e][c] * old + x[e][c] * add;
+      }
     }
-    const float over = seen > 0 ? 1.f / l : 0.f;
-    *(PBE_GLOBAL u32x2*)(uintptr_t)(p.out + (((uint64_t)u.begin + token) * (uint64_t)q_heads + (uint64_t)(head * p.group + g)) * (2 * D) + 2 * d) =
-        u32x2{pack_bf16(acc[0] * over, acc[1] * over), pack_bf16(acc[2] * over, acc[3] * over)};
+#pragma unroll
+    for (int e = 0; e < kTogether; ++e) {
+      const int row = at.t * kRows + r0 + e * kStep;
+      if (r0 + e * kStep >= to) break;
+      const int token = (int)fast_div((uint32_t)row, p.by_group), g = row - token * p.group;
+      const float over = seen_by(u, token) > 0 ? 1.f / l[e] : 0.f;
+      *(PBE_GLOBAL u32x2*)(uintptr_t)(p.out + (((uint64_t)u.begin + token) * (uint64_t)q_heads + (uint64_t)(head * p.group + g)) * (2 * D) + 2 * d) =
+          u32x2{pack_bf16(acc[e][0] * over, acc[e][1] * over), pack_bf16(acc[e][2] * over, acc[e][3] * over)};
+    }
   }
 }
 
 template <int D, KeyKind kKind, int kWaves>
-hipError_t launch(const PromptParams& p, hipStream_t stream) {
-  const dim3 grid((uint32_t)(p.units * p.kv_heads));
+hipError_t launch(const PromptParams& p, int64_t workgroups, hipStream_t stream) {
+  const int64_t rounded = (workgroups + kXcds - 1) / kXcds * kXcds;
+  const dim3 grid((uint32_t)(rounded * p.kv_heads));
   hipLaunchKernelGGL((prompt_attention_kernel<D, kKind, kWaves>), grid, dim3(64 * kWaves), 0, stream, p);
-  if (p.wanted) hipLaunchKernelGGL((prompt_join_kernel<D, kKind, kWaves>), grid, dim3(256), 0, stream, p);
+  if (p.parts) hipLaunchKernelGGL((prompt_join_kernel<D, kKind, 32 * kWaves>), grid, dim3(kJoinThreads), 0, stream, p);
   return hipGetLastError();
 }
 
 template <int D, KeyKind kKind>
-hipError_t launch_rows(const PromptParams& p, int rows, hipStream_t stream) {
-  return rows == 64 ? launch<D, kKind, 2>(p, stream) : launch<D, kKind, 4>(p, stream);
+hipError_t launch_rows(const PromptParams& p, int rows, int64_t workgroups, hipStream_t stream) {
+  switch (rows) {
+    case 32: return launch<D, kKind, 1>(p, workgroups, stream);
+    case 64: return launch<D, kKind, 2>(p, workgroups, stream);
+    case 128: return launch<D, kKind, 4>(p, workgroups, stream);
+    default: return launch<D, kKind, 8>(p, workgroups, stream);
+  }
 }
 
 template <int D>
-hipError_t launch_kind(const PromptParams& p, KeyKind kind, int rows, hipStream_t stream) {
+hipError_t launch_kind(const PromptParams& p, KeyKind kind, int rows, int64_t workgroups, hipStream_t stream) {
   switch (kind) {
-    case KeyKind::kRows: return launch_rows<D, KeyKind::kRows>(p, rows, stream);
-    case KeyKind::kBf16: return launch_rows<D, KeyKind::kBf16>(p, rows, stream);
-    case KeyKind::kFp8: return launch_rows<D, KeyKind::kFp8>(p, rows, stream);
-    default: return launch_rows<D, KeyKind::kMxfp4>(p, rows, stream);
+    case KeyKind::kRows: return launch_rows<D, KeyKind::kRows>(p, rows, workgroups, stream);
+    case KeyKind::kBf16: return launch_rows<D, KeyKind::kBf16>(p, rows, workgroups, stream);
+    case KeyKind::kFp8: return launch_rows<D, KeyKind::kFp8>(p, rows, workgroups, stream);
+    default: return launch_rows<D, KeyKind::kMxfp4>(p, rows, workgroups, stream);
   }
 }
 
 }  // namespace
 
-int prompt_tile_rows(int64_t n_q, int64_t batch, int32_t group) { return n_q * group <= 64 * batch ? 64 : 128; }
-
-int64_t prompt_units(int64_t n_q, int64_t batch, int32_t group, int rows, int64_t wanted) {
-  return n_q * group / rows + std::min(batch, n_q) + wanted;
+// Bytes of LDS of a workgroup.
+static int64_t lds_bytes(KeyKind kind, int dim) {
+  auto of = [&](auto stage64, auto stage128) { return dim == 64 ? decltype(stage64)::value : decltype(stage128)::value; };
+  switch (kind) {
+    case KeyKind::kFp8: return of(std::integral_constant<int, Stage<64, KeyKind::kFp8, 1>::kAll>(), std::integral_constant<int, Stage<128, KeyKind::kFp8, 1>::kAll>());
+    case KeyKind::kMxfp4:
+      return of(std::integral_constant<int, Stage<64, KeyKind::kMxfp4, 1>::kAll>(), std::integral_constant<int, Stage<128, KeyKind::kMxfp4, 1>::kAll>());
+    default: return of(std::integral_constant<int, Stage<64, KeyKind::kRows, 1>::kAll>(), std::integral_constant<int, Stage<128, KeyKind::kRows, 1>::kAll>());
+  }
 }
 
-uint64_t prompt_workspace_bytes(int64_t units, int32_t kv_heads, int32_t head_dim, int rows) {
-  return (uint64_t)units * (uint64_t)kv_heads * (uint64_t)rows * (uint64_t)(head_dim + 2) * 4;
+PromptPlan plan_prompt(int64_t n_q, int64_t batch, int32_t group, int32_t kv_heads, KeyKind kind, int64_t most_keys, int64_t units, uint64_t workspace,
+                       int32_t head_dim) {
+  PromptPlan r;
+  const int64_t rows = n_q * group;
+  r.rows = rows <= 32 * batch ? 32 : rows <= 64 * batch ? 64 : rows <= 128 * batch ? 128 : 256;
+  r.tiles = rows / r.rows + std::min(batch, n_q);
+  // workgroups that a compute unit holds: eight waves' registers, 160 KiB of LDS
+  const int64_t held = std::min<int64_t>(256 / r.rows, 160 * 1024 / (lds_bytes(kind, head_dim) + 64));
+  const int64_t slots = std::max<int64_t>(1, held * units / kv_heads);
+  r.each = 2ull * (uint64_t)kv_heads * (uint64_t)r.rows * (uint64_t)(head_dim + 2) * 4;
+  const int64_t parts = std::min<int64_t>(slots, (int64_t)std::min<uint64_t>(workspace / r.each, 1 << 20));
+  // a tile is only cut where both pieces have kPiece key tiles
+  const bool cut = parts > 1 && most_keys >= 2 * kPiece * kKeys && r.tiles < 2 * slots && (8 * parts >= 7 * slots || parts >= r.tiles);
+  r.parts = cut ? (int32_t)parts : 0;
+  return r;
 }
 
-hipError_t launch_prompt_attention(const PromptParams& p, int dim, KeyKind kind, int rows, hipStream_t stream) {
-  if (dim == 128) return launch_kind<128>(p, kind, rows, stream);
-  if (dim == 64) return launch_kind<64>(p, kind, rows, stream);
+hipError_t launch_prompt_attention(PromptParams p, const PromptPlan& plan, int dim, KeyKind kind, hipStream_t stream) {
+  p.parts = plan.parts;
+  p.a_part = plan.parts ? 1.0 / plan.parts : 0;
+  p.step = 16 * plan.rows / p.group;
+  const int64_t workgroups = plan.parts ? plan.parts : plan.tiles;
+  if (dim == 128) return launch_kind<128>(p, kind, plan.rows, workgroups, stream);
+  if (dim == 64) return launch_kind<64>(p, kind, plan.rows, workgroups, stream);
   return hipErrorInvalidValue;
 }
 
