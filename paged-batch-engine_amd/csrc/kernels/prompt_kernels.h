@@ -29,7 +29,6 @@ struct PromptParams {
   int32_t max_blocks, blocks;  // pages: of a table, of the pools
   int32_t parts;            // per KV head that the work is cut into; 0: a workgroup a tile
   int32_t step;             // what a tile costs more than the one before (sixteenths of a key)
-  double a_part;            // 1 / parts
   float scale;              // log2(e) / sqrt(head_dim): scores in base 2
   FastDiv by_group;
 };

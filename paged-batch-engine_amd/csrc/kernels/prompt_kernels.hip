@@ -20,7 +20,8 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 #define PBE_LDS __attribute__((address_space(3)))
 
 constexpr int kKeys = 64;         // keys of a tile
-constexpr int kPiece = 8;          // key tiles between the cuts of a tile
+constexpr int kPiece = 8;          // key tiles that a part has at least, on the average
+constexpr int kEdge = 4;           // key tiles of a tile that is cut before and behind the cuts
 constexpr int kMaxCuts = 4096;    // of a tile
 constexpr float kLazy = 8.f;      // how far (in base 2) scores may pass the maximum that weights refer to
 constexpr float kFar = 1024.f;    // maxima (in base 2) beyond which weights come from the scores' differences
@@ -109,21 +110,25 @@ __device__ __forceinline__ Found find_seq(int batch, int64_t x, int lane, Of of)
   return {batch, before};
 }
 
-// All the work of the batch, and where part w of it begins.
+// The batch's work, cut into `parts` of `each`: as many as there are workgroups for,
+// but none that is less than a tile or kPiece key tiles on the average.
+struct Work {
+  int64_t total, each;
+  int parts;
+  __device__ __forceinline__ int64_t begin(int w) const { return min(total, each * w); }
+};
+__device__ __forceinline__ Work work_in(const PromptParams& p, int64_t total, int tiles) {
+  Work r;
+  r.total = total;
+  r.parts = (int)min((int64_t)p.parts, max((int64_t)tiles, total / (kPiece * 16 * kKeys)));
+  r.parts = max(1, __builtin_amdgcn_readfirstlane(r.parts));
+  r.each = (int64_t)((double)total / (double)r.parts) + 1 + (total >> 50);  // at least a parts-th
+  return r;
+}
 template <KeyKind kKind, int kRows>
 __device__ __forceinline__ int64_t work_of(const PromptParams& p, int b) {
   const Seq u = seq_of<kKind, kRows>(p, b);
   return u.before(u.tiles);
-}
-template <KeyKind kKind, int kRows>
-__device__ __forceinline__ int64_t total_work(const PromptParams& p, int lane) {
-  int64_t sum = 0;
-  for (int b = lane; b < p.batch; b += 64) sum += work_of<kKind, kRows>(p, b);
-  return of_lane(wave_scan64(sum), 63);
-}
-__device__ __forceinline__ int64_t part_at(const PromptParams& p, int64_t total, int w) {
-  const int64_t each = (int64_t)((double)total * p.a_part) + 1 + (total >> 50);  // at least a parts-th
-  return min(total, each * w);
 }
 
 // Key tile k of tile t of sequence b; the work before the tile.
@@ -133,10 +138,10 @@ struct Place {
 };
 
 // The key tile at which a part that begins at y of a tile's `cost` cuts its n key
-// tiles: cuts lie kPiece tiles apart, and as far from the end.
+// tiles: kEdge at least from both of its ends, or not at all.
 __device__ __forceinline__ int cut_at(int64_t y, int64_t cost, int n) {
-  const int k = min((int)((double)y * (double)n / (double)cost), n - kPiece);
-  return k <= 0 ? 0 : k - k % kPiece;
+  const int k = min((int)((double)y * (double)n / (double)cost), n - kEdge);
+  return k < kEdge ? 0 : k;
 }
 
 // Place x of the work, which is sequence f's.
@@ -155,25 +160,34 @@ __device__ __forceinline__ Place place_at(const PromptParams& p, const Found& f,
   return {f.b, t, __builtin_amdgcn_readfirstlane(cut_at(y - before, u.cost(t), tiles_seen<kRows>(p, u, t))), f.before + before};
 }
 
-// Where part w begins and ends. Returns all the work.
+// Where part w begins and ends.
 template <KeyKind kKind, int kRows>
-__device__ __forceinline__ int64_t find_part(const PromptParams& p, int w, int lane, Place* at, Place* end) {
+__device__ __forceinline__ Work find_part(const PromptParams& p, int w, int lane, Place* at, Place* end) {
   if (p.batch <= 64) {
-    const int64_t mine = lane < p.batch ? work_of<kKind, kRows>(p, lane) : 0, upto = wave_scan64(mine), total = of_lane(upto, 63);
+    const Seq u = lane < p.batch ? seq_of<kKind, kRows>(p, lane) : Seq{};
+    const int64_t mine = u.before(u.tiles), upto = wave_scan64(mine);
+    const Work work = work_in(p, of_lane(upto, 63), __builtin_amdgcn_readlane(wave_scan(u.tiles), 63));
     auto place = [&](int64_t x) {
       const uint64_t past = __ballot(upto > x);
       const int b = past ? __builtin_ctzll(past) : p.batch;
-      return place_at<kKind, kRows>(p, Found{b, past ? of_lane(upto - mine, b) : total}, x);
+      return place_at<kKind, kRows>(p, Found{b, past ? of_lane(upto - mine, b) : work.total}, x);
     };
-    *at = place(part_at(p, total, w));
-    if (end) *end = place(part_at(p, total, w + 1));
-    return total;
+    *at = place(work.begin(w));
+    if (end) *end = place(work.begin(w + 1));
+    return work;
   }
-  const int64_t total = total_work<kKind, kRows>(p, lane);
+  int64_t sum = 0;
+  int tiles = 0;
+  for (int b = lane; b < p.batch; b += 64) {
+    const Seq u = seq_of<kKind, kRows>(p, b);
+    sum += u.before(u.tiles);
+    tiles += u.tiles;
+  }
+  const Work work = work_in(p, of_lane(wave_scan64(sum), 63), __builtin_amdgcn_readlane(wave_scan(tiles), 63));
   auto place = [&](int64_t x) { return place_at<kKind, kRows>(p, find_seq(p.batch, x, lane, [&](int b) { return work_of<kKind, kRows>(p, b); }), x); };
-  *at = place(part_at(p, total, w));
-  if (end) *end = place(part_at(p, total, w + 1));
-  return total;
+  *at = place(work.begin(w));
+  if (end) *end = place(work.begin(w + 1));
+  return work;
 }
 
 // The w-th tile of the batch, those that cost the most first (so that none of them is
@@ -489,7 +503,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 2 ? 2 : 1) void prompt_attent
   Place at, end;
   if (p.parts) {
     if (w >= p.parts) return;
-    find_part<kKind, kRows>(p, w, lane, &at, &end);
+    if (w >= find_part<kKind, kRows>(p, w, lane, &at, &end).parts) return;
   } else {
     if (!find_tile<kKind, kRows>(p, w, lane, &at)) return;
     end = {at.b, at.t + 1, 0, 0};
@@ -793,9 +807,13 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 2 ? 2 : 1) void prompt_attent
 
 // Joins the tiles that were cut. Of a tile's n + 1 parts, each of the n that do not
 // begin it has a workgroup here, which takes its share of the tile's rows.
-constexpr int kJoinThreads = 1024;
+constexpr int kJoinRows = 4;  // of a thread at once, so that their loads are on their way together
+template <int D, int kRows>
+constexpr int join_threads() {
+  return D / 4 * kRows / kJoinRows < 1024 ? D / 4 * kRows / kJoinRows : 1024;
+}
 template <int D, KeyKind kKind, int kRows>
-__global__ __launch_bounds__(kJoinThreads) void prompt_join_kernel(const PromptParams p) {
+__global__ __launch_bounds__((join_threads<D, kRows>())) void prompt_join_kernel(const PromptParams p) {
   constexpr int kLanes = D / 4;
   __shared__ int cuts[kMaxCuts + 2];  // the key tiles at which the tile's parts begin
   const int lane = threadIdx.x & 63;
@@ -803,14 +821,14 @@ __global__ __launch_bounds__(kJoinThreads) void prompt_join_kernel(const PromptP
   workgroup_of<kKind>(p, &w, &head);
   if (w >= p.parts) return;
   Place at;
-  const int64_t total = find_part<kKind, kRows>(p, w, lane, &at, nullptr);
-  if (at.b >= p.batch || at.k == 0) return;
+  const Work work = find_part<kKind, kRows>(p, w, lane, &at, nullptr);
+  if (w >= work.parts || at.b >= p.batch || at.k == 0) return;
   const Seq u = seq_of<kKind, kRows>(p, at.b);
   const int64_t cost = u.cost(at.t);
   const int all = tiles_seen<kRows>(p, u, at.t);
   // Part i's start: its cut of this tile, -1 before the tile, `all` behind it.
   auto cut_of = [&](int i) {
-    const int64_t y = part_at(p, total, i) - at.start;
+    const int64_t y = work.begin(i) - at.start;
     return y < 0 ? -1 : y >= cost ? all : cut_at(y, cost, all);
   };
   // the last part that begins at or before the tile's start
@@ -824,7 +842,7 @@ __global__ __launch_bounds__(kJoinThreads) void prompt_join_kernel(const PromptP
   --w0;  // w0 + 1 is the first that begins inside; part 0 begins at no tile's inside
   int n = 0;  // parts that begin inside
   for (int i = w0;; i += 64) {
-    const int c = i + lane <= p.parts ? cut_of(i + lane) : all;
+    const int c = i + lane <= work.parts ? cut_of(i + lane) : all;
     const uint64_t past = __ballot(c >= all);
     const int many = past ? __builtin_ctzll(past) : 64;
     if (threadIdx.x < 64 && lane <= many && i - w0 + lane < kMaxCuts + 2) cuts[i - w0 + lane] = c;
@@ -836,8 +854,7 @@ __global__ __launch_bounds__(kJoinThreads) void prompt_join_kernel(const PromptP
   const int from = (int)((int64_t)rows * share / n), to = (int)((int64_t)rows * (share + 1) / n);
   const int q_heads = p.kv_heads * p.group;
   const bool begins = cuts[0] == 0;  // else its first tile was another one
-  // kTogether rows of a thread at once, so that their loads are on their way together
-  constexpr int kStep = kJoinThreads / kLanes, kTogether = 4;
+  constexpr int kStep = join_threads<D, kRows>() / kLanes, kTogether = kJoinRows;
   const int d = 4 * ((int)threadIdx.x % kLanes);
   for (int r0 = from + (int)threadIdx.x / kLanes; r0 < to; r0 += kTogether * kStep) {
     float m[kTogether], l[kTogether];
@@ -883,7 +900,7 @@ hipError_t launch(const PromptParams& p, int64_t workgroups, hipStream_t stream)
   const int64_t rounded = (workgroups + kXcds - 1) / kXcds * kXcds;
   const dim3 grid((uint32_t)(rounded * p.kv_heads));
   hipLaunchKernelGGL((prompt_attention_kernel<D, kKind, kWaves>), grid, dim3(64 * kWaves), 0, stream, p);
-  if (p.parts) hipLaunchKernelGGL((prompt_join_kernel<D, kKind, 32 * kWaves>), grid, dim3(kJoinThreads), 0, stream, p);
+  if (p.parts) hipLaunchKernelGGL((prompt_join_kernel<D, kKind, 32 * kWaves>), grid, dim3(join_threads<D, 32 * kWaves>()), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -931,15 +948,14 @@ PromptPlan plan_prompt(int64_t n_q, int64_t batch, int32_t group, int32_t kv_hea
   const int64_t slots = std::max<int64_t>(1, held * units / kv_heads);
   r.each = 2ull * (uint64_t)kv_heads * (uint64_t)r.rows * (uint64_t)(head_dim + 2) * 4;
   const int64_t parts = std::min<int64_t>(slots, (int64_t)std::min<uint64_t>(workspace / r.each, 1 << 20));
-  // a tile is only cut where both pieces have kPiece key tiles
-  const bool cut = parts > 1 && most_keys >= 2 * kPiece * kKeys && r.tiles < 2 * slots && (8 * parts >= 7 * slots || parts >= r.tiles);
+  // below, no tile can be cut
+  const bool cut = parts > 1 && most_keys >= 2 * kEdge * kKeys && r.tiles < 2 * slots && (8 * parts >= 7 * slots || parts >= r.tiles);
   r.parts = cut ? (int32_t)parts : 0;
   return r;
 }
 
 hipError_t launch_prompt_attention(PromptParams p, const PromptPlan& plan, int dim, KeyKind kind, hipStream_t stream) {
   p.parts = plan.parts;
-  p.a_part = plan.parts ? 1.0 / plan.parts : 0;
   p.step = 16 * plan.rows / p.group;
   const int64_t workgroups = plan.parts ? plan.parts : plan.tiles;
   if (dim == 128) return launch_kind<128>(p, kind, plan.rows, workgroups, stream);
