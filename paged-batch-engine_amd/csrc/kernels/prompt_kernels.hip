@@ -20,7 +20,7 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 #define PBE_LDS __attribute__((address_space(3)))
 
 constexpr int kKeys = 64;         // keys of a tile
-constexpr int kPiece = 8;          // key tiles that a part has at least, on the average
+constexpr int kPiece = 4;          // key tiles that a part has at least, on the average
 constexpr int kEdge = 4;           // key tiles of a tile that is cut before and behind the cuts
 constexpr int kMaxCuts = 4096;    // of a tile
 constexpr float kLazy = 8.f;      // how far (in base 2) scores may pass the maximum that weights refer to
@@ -298,7 +298,7 @@ struct Stage {
   static constexpr bool kMx = kKind == KeyKind::kMxfp4, kFp8 = kKind == KeyKind::kFp8, kScaled = kMx || kFp8;
   static constexpr int kTile = kKeys * D * (kFp8 ? 1 : 2);                 // bytes of K (or V) as they are read
   static constexpr int kRaw = kMx ? kKeys * D / 2 : kTile;                 // as they are loaded
-  static constexpr int kTurns = kFp8 ? 3 : 2;
+  static constexpr int kTurns = 2;
   static constexpr int kInstr = kRaw / 1024;                               // loads for K (or V)
   static constexpr int kLoads = (2 * kInstr + kWaves - 1) / kWaves;        // of a wave
   static constexpr int kScaleBytes = kScaled ? 512 : 0;                    // K's and V's of a tile
