@@ -12,12 +12,15 @@
 
 #include "decode_device.h"
 #include "page_kernels.h"
+#include "xcd_order.h"
 
 namespace pbe {
 namespace {
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
 constexpr int kWords = kMostPages / 32;
+constexpr int kForkRows = 3584;  // whose first children fit LDS beside the map; more take the workspace
+constexpr uint32_t kCopyGroup = 384 * 1024 / kPageSlice;  // slices that an XCD takes one after another
 constexpr int kCopyThreads = 256, kCopyEach = kPageSlice / (16 * kCopyThreads);
 
 // Page of an entry, or -1 where it names none of the pool's.
@@ -75,10 +78,6 @@ __device__ __forceinline__ Child child_of(const ForkParams& p, int i) {
   return c;
 }
 
-__device__ __forceinline__ int first_of(const ForkParams& p, int parent) {
-  return __hip_atomic_load(p.firsts + parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
 // Bits of pages that others hold, and of those that there are not.
 __device__ __forceinline__ uint64_t held_elsewhere(const int32_t* reserved, int n_pages, int first, int lane) {
   const int i = first + lane;
@@ -87,54 +86,81 @@ __device__ __forceinline__ uint64_t held_elsewhere(const int32_t* reserved, int 
 
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(const ForkParams p) {
   __shared__ uint32_t held[kWords];
+  __shared__ int32_t firsts[kForkRows];                     // a row's first child
+  __shared__ int32_t row_of[kPlanThreads], kept_of[kPlanThreads];  // of the children whose parents are marked
   __shared__ uint32_t sums[kPlanWaves];
+  __shared__ int marked;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int words = (p.n_pages + 63) / 64 * 2;
+  const bool few = p.rows_in <= kForkRows;
+  Child mine = t < p.rows_out ? child_of(p, t) : Child();   // the first kPlanThreads children's
   for (int w = wave; w < words / 2; w += kPlanWaves) {
     const uint64_t bits = held_elsewhere(p.reserved, p.n_pages, w * 64, lane);
     if (lane == 0) held[2 * w] = (uint32_t)bits;
     if (lane == 1) held[2 * w + 1] = (uint32_t)(bits >> 32);
   }
-  for (int i = t; i < p.rows_in; i += kPlanThreads) p.firsts[i] = 0x7fffffff;
-  __threadfence();
+  for (int i = t; i < p.rows_in; i += kPlanThreads) {
+    if (few) firsts[i] = 0x7fffffff;
+    else p.firsts[i] = 0x7fffffff;
+  }
+  if (!few) __threadfence();
   __syncthreads();
+  auto child = [&](int i) { return i < kPlanThreads ? mine : i < p.rows_out ? child_of(p, i) : Child(); };
   for (int i = t; i < p.rows_out; i += kPlanThreads) {
-    const Child c = child_of(p, i);
-    if (c.parent >= 0) atomicMin(p.firsts + c.parent, i);
+    const Child c = child(i);
+    if (c.parent < 0) continue;
+    if (few) atomicMin(&firsts[c.parent], i);
+    else atomicMin(p.firsts + c.parent, i);
   }
-  __threadfence();
+  if (!few) __threadfence();
   __syncthreads();
-  // what the children's parents hold, each parent once
-  for (int i = wave; i < p.rows_out; i += kPlanWaves) {
-    const Child c = child_of(p, i);
-    if (c.parent < 0 || first_of(p, c.parent) != i) continue;
-    const int32_t* row = p.tables_in + (int64_t)c.parent * p.max_blocks;
-    for (int j = lane; j < c.kept; j += 64) {
-      const int page = page_of(row[j], p.n_pages, p.stride, p.by_stride);
-      if (page >= 0) atomicOr(&held[page / 32], 1u << (page % 32));
+  auto first_of = [&](int parent) {
+    return few ? firsts[parent] : __hip_atomic_load(p.firsts + parent, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  // What the children's parents hold, each parent once: kPlanThreads children at a
+  // time are listed, then waves mark the rows listed, kMarks of them together.
+  for (int i0 = 0; i0 < p.rows_out; i0 += kPlanThreads) {
+    if (t == 0) marked = 0;
+    __syncthreads();
+    const Child c = child(i0 + t);
+    if (c.parent >= 0 && first_of(c.parent) == i0 + t) {
+      const int at = atomicAdd(&marked, 1);  // in any order: bits are set
+      row_of[at] = c.parent;
+      kept_of[at] = c.kept;
     }
+    __syncthreads();
+    constexpr int kMarks = 4;
+    for (int r = wave * kMarks; r < marked; r += kPlanWaves * kMarks) {
+      int most = 0;
+#pragma unroll
+      for (int e = 0; e < kMarks; ++e) most = max(most, r + e < marked ? kept_of[r + e] : 0);
+      for (int k = lane; k < most; k += 64) {
+        int id[kMarks];
+#pragma unroll
+        for (int e = 0; e < kMarks; ++e) id[e] = r + e < marked && k < kept_of[r + e] ? p.tables_in[(int64_t)row_of[r + e] * p.max_blocks + k] : -1;
+#pragma unroll
+        for (int e = 0; e < kMarks; ++e) {
+          const int page = page_of(id[e], p.n_pages, p.stride, p.by_stride);
+          if (page >= 0) atomicOr(&held[page / 32], 1u << (page % 32));
+        }
+      }
+    }
+    __syncthreads();
   }
-  __syncthreads();
   const int each = (words + kPlanThreads - 1) / kPlanThreads, from = min(words, t * each), to = min(words, from + each);
-  uint32_t mine = 0;
-  for (int w = from; w < to; ++w) mine += 32 - __popc(held[w]);
+  uint32_t open = 0;
+  for (int w = from; w < to; ++w) open += 32 - __popc(held[w]);
   uint32_t available;
-  uint32_t rank = plan_scan(mine, sums, &available);
+  uint32_t rank = plan_scan(open, sums, &available);
   // needs in the children's order
   uint32_t needed = 0, copied = 0;
   for (int i0 = 0; i0 < p.rows_out; i0 += kPlanThreads) {
     const int i = i0 + t;
-    Child c;
-    bool copy = false;
-    if (i < p.rows_out) {
-      c = child_of(p, i);
-      if (c.parent >= 0) {
-        copy = c.kept * (int64_t)p.block_size != c.len && first_of(p, c.parent) != i;
-        // a copy needs a page to copy from
-        if (copy && page_of(p.tables_in[(int64_t)c.parent * p.max_blocks + c.kept - 1], p.n_pages, p.stride, p.by_stride) < 0)
-          c = Child(), c.bad = true, copy = false;
-      }
-    }
+    Child c = child(i);
+    bool copy = c.parent >= 0 && c.kept * (int64_t)p.block_size != c.len && first_of(c.parent) != i;
+    // a copy needs a page to copy from
+    if (copy && page_of(p.tables_in[(int64_t)c.parent * p.max_blocks + c.kept - 1], p.n_pages, p.stride, p.by_stride) < 0)
+      c = Child(), c.bad = true, copy = false;
     const uint32_t need = c.parent >= 0 ? (uint32_t)(c.want - c.kept + copy) : 0;
     uint32_t total, copies;
     const uint32_t at = needed + plan_scan(need, sums, &total);
@@ -206,7 +232,7 @@ __global__ __launch_bounds__(kCopyThreads) void fork_move_kernel(const ForkParam
     return;
   }
   const uint64_t units = (uint64_t)p.header[0] * planes.slices;
-  for (uint64_t u = blockIdx.x; u < units; u += p.copiers) {
+  for (uint64_t u = xcd_grouped(blockIdx.x, p.copiers, kCopyGroup); u < units; u += p.copiers) {
     const uint32_t m = (uint32_t)(u / planes.slices), child = (uint32_t)p.copies[m];
     const int shared = p.shared[child];
     const int from = page_of(p.tables_in[(int64_t)p.parents[child] * p.max_blocks + shared], p.n_pages, p.stride, p.by_stride);
@@ -287,7 +313,7 @@ __global__ __launch_bounds__(kCopyThreads) void compact_move_kernel(const Compac
     return;
   }
   const uint64_t units = (uint64_t)p.header[0] * planes.slices;
-  for (uint64_t u = blockIdx.x; u < units; u += p.copiers) {
+  for (uint64_t u = xcd_grouped(blockIdx.x, p.copiers, kCopyGroup); u < units; u += p.copiers) {
     const uint32_t m = (uint32_t)(u / planes.slices);
     copy_slice(planes, (uint32_t)(u - (uint64_t)m * planes.slices), (uint32_t)p.sources[m], (uint32_t)p.places[m]);
   }

@@ -253,9 +253,9 @@ __device__ __forceinline__ float sum_bf16(uint32_t x, float c) {
 // Where the 16-byte chunk c of row r of a tile of K or V lies in LDS (in bytes): the
 // chunks of a row change places so that the lanes of a read hit different banks.
 template <int D>
-__device__ __forceinline__ uint32_t k_flip(uint32_t r) { return r & (D / 8 - 1); }
+__device__ __forceinline__ uint32_t k_flip(uint32_t r) { return r / (128 / D) & (D / 8 - 1); }
 template <int D>
-__device__ __forceinline__ uint32_t v_flip(uint32_t r) { return (2 * r) & (D / 8 - 1); }
+__device__ __forceinline__ uint32_t v_flip(uint32_t r) { return 4 * (r / (128 / D)) & (D / 8 - 1); }
 template <int D>
 __device__ __forceinline__ uint32_t code_flip(uint32_t r) { return (r / (256 / D)) & (D / 16 - 1); }
 template <int D>
