@@ -656,9 +656,10 @@ int pbe_qk_norm_rope_scatter(const void* q, int64_t q_stride, const void* k, int
  * sqrt(head_dim)) v for many query tokens a sequence, causal. Query i of a
  * sequence's n queries, which has `len` keys, sees keys 0 .. len - n + i; one that
  * sees none gets zeros. BF16 queries and outputs, FP32 scores, softmax and sums;
- * a softmax weight goes into its product with v as one BF16 number (within 2^-8).
- * The sum that the outputs are divided by is that of the weights before the
- * rounding. head_dim 64 or 128, q_heads any multiple of kv_heads.
+ * a softmax weight goes into its product with v as one BF16 number (within 2^-8), and
+ * the outputs are divided by the sum of those numbers (over FP8 pages, where a value's
+ * scale goes into its weight first, by that of the weights themselves). head_dim 64 or
+ * 128, q_heads any multiple of kv_heads.
  *
  * An infinity or a NaN in a key or value reaches the queries that see it, and no
  * other. A score beyond FP32's range, or NaN: -infinity takes a key's weight to
@@ -687,7 +688,7 @@ uint64_t pbe_prompt_workspace_bytes(int32_t n_rows, int32_t batch, int32_t q_hea
  *     to k_starts[b + 1]. k_starts NULL: the same, and n_keys = n_queries.
  * A sequence whose queries begin below 0, end before they begin or beyond
  * n_queries, or whose keys do so beyond n_keys, gets NaN in those of its rows that
- * there are. No counterpart in the reference's paged-KV runtime. */
+ * there are. Rows that two sequences claim hold the result of either, or are left. No counterpart in the reference's paged-KV runtime. */
 int pbe_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride,
                          const void* v, int64_t v_stride, int32_t n_queries, int32_t n_keys,
                          const int32_t* q_starts, const int32_t* k_starts, int32_t batch,
@@ -705,7 +706,8 @@ int pbe_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t
  *     token_starts[b+1] - 1, the last of its seq_lens[b] tokens.
  * A sequence whose rows begin below 0, end before they begin or beyond n_rows,
  * whose length is negative, beyond 2^31 - 256 or needs more than
- * max_blocks_per_seq blocks gets NaN in those of its rows that there are. A block
+ * max_blocks_per_seq blocks gets NaN in those of its rows that there are. Rows that
+ * two sequences claim hold the result of either, or are left. A block
  * id outside the pools gives NaN to the rows that see its tokens. What lies behind
  * a sequence's last token, in its page or in its table, is not used. Takes the
  * place of the reference's prefill attention (paged_kv_runtime.cpp) over pages. */

@@ -1,4 +1,4 @@
-"""Attention of prompts in 64 bits: what pbe_prompt_attention and
+"""TEST INFRASTRUCTURE ONLY: attention of prompts in 64 bits: what pbe_prompt_attention and
 pbe_paged_prompt_attention compute, from its definition.
 
 Query i of a sequence's n queries, of `length` keys, sees keys 0 .. length - n + i.

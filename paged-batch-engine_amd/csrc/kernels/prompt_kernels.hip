@@ -1,4 +1,36 @@
 // Prompt reader: causal attention of many query tokens a sequence over its keys.
+//
+// o = sum_j w_j v_j / sum_j w_j, w_j = 2^((q . k_j - m) * scale), scale = log2(e) /
+// sqrt(D), over the keys that a query sees; one pass over the keys, m and the sums
+// held in FP32. The query heads that share a KV head are stacked: row r of a sequence
+// is token r / group, head r % group, so K and V are read once for all of them, and a
+// single query of a large group still fills a wave's 32 columns.
+//
+// A wave has 32 rows and computes S^T = K Q^T and O^T += V^T W^T with the 32x32x16
+// BF16 MFMA. Transposed, because a lane then holds one row's scores (32 of a tile's 64,
+// its other half in lane + 32): maximum and sum need no exchange but one swap of
+// halves, and the scores' registers are the weights' operand as they are, without LDS.
+// V comes as the A operand by LDS reads that transpose; Q stays in registers.
+//
+// Bound: MFMA, 4 * D FLOP a row and seen key. 4 * 128 dims take 32 products of 8
+// passes each a wave and tile, beside about 400 instructions for 64 weights a lane pair.
+// Over 8,192 tokens of 28 heads of 128 dims: 462 us, 1,040 TFLOP/s, of the 1,387 that a
+// large matrix product reaches here; MFMA busy 49% at 2.05 GHz (the clock falls as the
+// kernel gets faster). Leaving out the exponentials, or the maxima, or the sums, takes 6
+// to 9% off (on the way there, of 526 us): no single part is the bound.
+// What that took, in us, each measured against the one before: 128 rows a workgroup 526;
+// special values (see there) looked for in masked tiles only, in place 507; reads some
+// products ahead and one multiply-add before each exponential 485; 256 rows 469; no bank
+// conflicts 462.
+// Tried and slower: the next tile's scores among this one's weights in one wave (510 for
+// 469), the workgroup's halves taking turns (507 for 462), three tiles in LDS (503 for
+// 469), V's loads after all of K's (500 for 467). Waves' priorities changed nothing.
+//
+// A weight goes into its product as one BF16 number, off by at most 2^-8 of itself (two
+// numbers each would double the second product's MFMA). Over rows, BF16 and MXFP4 pages
+// the sum is that of the rounded weights, so a row's outputs are a mean of its values
+// all the same, and constant values come back exactly. Over FP8 pages the value's scale
+// goes into the weight before the rounding, and the sum is of those before.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -20,11 +52,19 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 #define PBE_LDS __attribute__((address_space(3)))
 
 constexpr int kKeys = 64;         // keys of a tile
-constexpr int kPiece = 4;          // key tiles that a part has at least, on the average
-constexpr int kEdge = 4;           // key tiles of a tile that is cut before and behind the cuts
-constexpr int kMaxCuts = 4096;    // of a tile
-constexpr float kLazy = 8.f;      // how far (in base 2) scores may pass the maximum that weights refer to
-constexpr float kFar = 1024.f;    // maxima (in base 2) beyond which weights come from the scores' differences
+// Key tiles that a part has at least, on the average: a part's start, end and share of
+// the join cost about as much as four of its tiles. 64 x 4 drafted tokens over FP8
+// pages: 44.0 us with 4, 46.3 with 8.
+constexpr int kPiece = 4;
+constexpr int kEdge = 4;          // key tiles of a tile that is cut before and behind the cuts
+constexpr int kMaxCuts = 4096;    // parts at most, so also cuts of a tile
+// How far (in base 2) scores may pass the maximum that weights refer to. Weights of up
+// to 2^8 lose nothing in BF16 or FP32, and after a row's first tiles sums are scaled
+// hardly ever.
+constexpr float kLazy = 8.f;
+// Maxima (in base 2) beyond which weights come from the scores' differences: below, the
+// rounding of maximum * scale is at most 2^-14 and the same for all of a row's weights.
+constexpr float kFar = 1024.f;
 constexpr int kXcds = 8;
 static_assert(kBlockTokens == 16, "a key tile is four blocks");
 
@@ -110,6 +150,18 @@ __device__ __forceinline__ Found find_seq(int batch, int64_t x, int lane, Of of)
   return {batch, before};
 }
 
+// Parts. Tiles of a causal batch cost from one key tile to hundreds, and there may be
+// a few of them for 256 compute units. So the work (the sum of the tiles' costs, a model
+// linear in the tile's number, so that a place is found by a prefix sum over the
+// sequences and the root of a quadratic) is cut into equal parts, one a workgroup that
+// the GPU holds at once; a part is the end of a tile, whole tiles, the start of another.
+// A cut tile's partial results go to the workspace and prompt_join_kernel joins them.
+// The device does all of it from the starts and lengths, so captured calls follow them.
+// 2,041 tokens behind 5,040 others, 12 heads: 109 us. What it costs: 2.5 to 3.3 us to
+// find a part, about 3 to write partials, 12 to 15 the join.
+// Where there are two tiles a slot or more, a workgroup takes one whole tile and those
+// that cost the most go first (16 mixed prompts: 96 us; cut into parts 126).
+//
 // The batch's work, cut into `parts` of `each`: as many as there are workgroups for,
 // but none that is less than a tile or kPiece key tiles on the average.
 struct Work {
@@ -149,6 +201,7 @@ template <KeyKind kKind, int kRows>
 __device__ __forceinline__ Place place_at(const PromptParams& p, const Found& f, int64_t x) {
   if (f.b >= p.batch) return {p.batch, 0, 0, f.before};
   const Seq u = seq_of<kKind, kRows>(p, f.b);
+  if (u.tiles <= 0) return {p.batch, 0, 0, f.before};  // only where overlapping rows' work passes 63 bits
   const int64_t y = x - f.before;
   // before(t) <= y < before(t + 1), from the root of its quadratic
   const float half = (float)u.base + 0.5f * (float)u.step, root = __builtin_amdgcn_sqrtf(half * half + 2.f * (float)u.step * (float)y);
@@ -299,6 +352,7 @@ struct Stage {
   static constexpr int kTile = kKeys * D * (kFp8 ? 1 : 2);                 // bytes of K (or V) as they are read
   static constexpr int kRaw = kMx ? kKeys * D / 2 : kTile;                 // as they are loaded
   static constexpr int kTurns = 2;
+  static constexpr int kAhead = kMx ? 2 : 1;                               // tiles asked for before one is used
   static constexpr int kInstr = kRaw / 1024;                               // loads for K (or V)
   static constexpr int kLoads = (2 * kInstr + kWaves - 1) / kWaves;        // of a wave
   static constexpr int kScaleBytes = kScaled ? 512 : 0;                    // K's and V's of a tile
@@ -407,9 +461,9 @@ struct Stage {
     return wrong;
   }
 
-  // What this wave asked for of a tile is there; `after`: tiles asked for since.
-  __device__ __forceinline__ void wait(int after) const {
-    if (kMx ? after >= 1 : after >= kTurns - 2) arrived<(kMx ? 1 : kTurns - 2) * kPerTile>();
+  // What this wave asked for of a tile is there; `more`: a later one was asked for, too.
+  __device__ __forceinline__ void wait(bool more) const {
+    if (more) arrived<(kAhead - 1) * kPerTile>();
     else arrived<0>();
   }
 
@@ -474,8 +528,11 @@ __device__ __forceinline__ uint32_t without_special(uint32_t x) {
   return kFp8 ? x & ~(s | (s - (s >> 7))) : x & ~(s | (s - (s >> 15)));
 }
 
-// Which part (or tile) and head a workgroup has. Pages whose lines several heads
-// share have their heads on one XCD, others (nearly) each head on its own.
+// Which part (or tile) and head a workgroup has. Workgroups go to the eight XCDs in
+// turn, each with an L2 of its own. FP8 and MXFP4 pages' lines hold several heads' bytes
+// (scales all of them): all heads of a part on one XCD. Of BF16 every head has lines of
+// its own: neighbouring workgroups take neighbouring heads, so that with 4 or 8 KV heads
+// an XCD's L2 holds one or two heads' K and V instead of all.
 template <KeyKind kKind>
 __device__ __forceinline__ void workgroup_of(const PromptParams& p, int* w, int* head) {
   const int x = blockIdx.x;
@@ -489,6 +546,14 @@ __device__ __forceinline__ void workgroup_of(const PromptParams& p, int* w, int*
   }
 }
 
+// One part (or tile) a workgroup: kWaves waves of 32 rows that share the key tiles in
+// LDS. A tile's 64 keys are asked for a tile (MXFP4: two) ahead, straight into LDS; one
+// barrier a tile (MXFP4: two), behind which the tile read before is overwritten.
+// Registers: O 4 x 16, scores 32, Q 32, weights 16; two waves a SIMD.
+// FP8 codes become BF16 operands at the LDS reads: once a tile instead, into BF16 tiles,
+// took the same time (130.8 and 130.4 us, 128 new tokens in each of 10 sequences) and
+// more LDS. The matrix product of 8-bit operands is no faster at this shape and would
+// round the queries.
 template <int D, KeyKind kKind, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, kWaves > 2 ? 2 : 1) void prompt_attention_kernel(const PromptParams p) {
   using S = Stage<D, kKind, kWaves>;
@@ -536,7 +601,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 2 ? 2 : 1) void prompt_attent
       if (opened) __syncthreads();  // the tile before has been read
       opened = true;
       // Blocks not in the pools: of this key tile and those asked for.
-      constexpr int kAhead = S::kMx ? 2 : S::kTurns - 1;  // tiles asked for before one is used
+      constexpr int kAhead = S::kAhead;
       uint32_t wrong = 0, wrongs[kAhead] = {};
       if (kt0 < kt1) wrongs[0] = stage.load(kt0, 0);
       bf16x8 q[D / 16];
@@ -551,7 +616,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 2 ? 2 : 1) void prompt_attent
         if (kt0 + i < kt1) wrongs[i] = stage.load(kt0 + i, i);
       for (int kt = kt0; kt < kt1; ++kt) {
         const int turn = kt - kt0, first = kt * kKeys;
-        stage.wait(kt1 - 1 - kt);
+        stage.wait(kt + 1 < kt1);
         __syncthreads();
         if constexpr (S::kMx) {
           stage.convert(turn);
@@ -805,8 +870,11 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 2 ? 2 : 1) void prompt_attent
   }
 }
 
-// Joins the tiles that were cut. Of a tile's n + 1 parts, each of the n that do not
-// begin it has a workgroup here, which takes its share of the tile's rows.
+// Joins the tiles that were cut: o = sum 2^((m_i - m) scale) o_i / sum 2^((m_i - m)
+// scale) l_i, in the parts' order. Of a tile's n + 1 parts, each of the n that do not
+// begin it has a workgroup here, which takes its share of the tile's rows. A launch of
+// its own: the last part to end a tile joining it instead would need flags that every
+// call clears, and would leave the join's order of sums to chance or wait for it.
 constexpr int kJoinRows = 4;  // of a thread at once, so that their loads are on their way together
 template <int D, int kRows>
 constexpr int join_threads() {
@@ -839,7 +907,7 @@ __global__ __launch_bounds__((join_threads<D, kRows>())) void prompt_join_kernel
     w0 -= n;
     if (n < 64) break;
   }
-  --w0;  // w0 + 1 is the first that begins inside; part 0 begins at no tile's inside
+  w0 = max(w0 - 1, 0);  // w0 + 1 is the first that begins inside; part 0 begins at no tile's inside
   int n = 0;  // parts that begin inside
   for (int i = w0;; i += 64) {
     const int c = i + lane <= work.parts ? cut_of(i + lane) : all;
@@ -850,6 +918,7 @@ __global__ __launch_bounds__((join_threads<D, kRows>())) void prompt_join_kernel
     if (past) break;
   }
   __syncthreads();
+  if (w <= w0 || w > w0 + n) return;  // never, but where overlapping rows' work passes 63 bits
   const int share = w - w0 - 1, rows = min(kRows, u.rows * p.group - at.t * kRows);
   const int from = (int)((int64_t)rows * share / n), to = (int)((int64_t)rows * (share + 1) / n);
   const int q_heads = p.kv_heads * p.group;
@@ -941,14 +1010,18 @@ PromptPlan plan_prompt(int64_t n_q, int64_t batch, int32_t group, int32_t kv_hea
                        int32_t head_dim) {
   PromptPlan r;
   const int64_t rows = n_q * group;
+  // The fewest rows that hold an average sequence's: more rows read K and V from LDS and
+  // cache less often (128 instead of 256 over 8,192 tokens: 509 for 483 us; over 2,041
+  // behind 5,040: 122 for 109), rows that no token fills cost as much as others.
   r.rows = rows <= 32 * batch ? 32 : rows <= 64 * batch ? 64 : rows <= 128 * batch ? 128 : 256;
   r.tiles = rows / r.rows + std::min(batch, n_q);
   // workgroups that a compute unit holds: eight waves' registers, 160 KiB of LDS
   const int64_t held = std::min<int64_t>(256 / r.rows, 160 * 1024 / (lds_bytes(kind, head_dim) + 64));
   const int64_t slots = std::max<int64_t>(1, held * units / kv_heads);
   r.each = 2ull * (uint64_t)kv_heads * (uint64_t)r.rows * (uint64_t)(head_dim + 2) * 4;
-  const int64_t parts = std::min<int64_t>(slots, (int64_t)std::min<uint64_t>(workspace / r.each, 1 << 20));
-  // below, no tile can be cut
+  const int64_t parts = std::min<int64_t>(slots, (int64_t)std::min<uint64_t>(workspace / r.each, kMaxCuts));
+  // Parts where there are fewer than two tiles a slot, tiles long enough to be cut, and a
+  // workspace for nearly all slots (or more parts than tiles).
   const bool cut = parts > 1 && most_keys >= 2 * kEdge * kKeys && r.tiles < 2 * slots && (8 * parts >= 7 * slots || parts >= r.tiles);
   r.parts = cut ? (int32_t)parts : 0;
   return r;

@@ -85,6 +85,31 @@ bool HipPagedKVRuntime::decode_append(const base::KVPoolView& pool, const PagedK
   return read(pool, args, new_keys, new_values);
 }
 
+bool HipPagedKVRuntime::prefill(const base::KVPoolView& pool, const PagedKVPrefillRuntimeArgs& args) const {
+  if (!pool.valid() || !pool.key_pool_bytes() || !pool.value_pool_bytes())
+    throw std::invalid_argument("KV pool view is not bound or carries no pool sizes");
+  if (!args.queries || !args.outputs || !args.token_starts || !args.block_tables || !args.seq_lens)
+    throw std::invalid_argument("prefill arguments hold a null tensor");
+  if (args.num_kv_heads <= 0 || args.kv_mul <= 0 ||
+      args.head_num != (int64_t)args.kv_mul * (int64_t)args.num_kv_heads)
+    throw std::invalid_argument("head_num must equal kv_mul * num_kv_heads");
+  if (args.block_size != 16) return false;
+  const bool fp8 = pool.uses_fp8_storage();
+  if (!fp8 && pool.storage_spec().storage_dtype != base::DataType::kDataTypeBf16) return false;
+  if (fp8 && (!pool.key_scale_pool() || !pool.value_scale_pool() || !pool.scale_pool_bytes()))
+    throw std::invalid_argument("FP8 KV pool view has no scale pools");
+  const int rc = pbe_paged_prompt_attention(
+      pool.key_pool(), pool.value_pool(), std::min(pool.key_pool_bytes(), pool.value_pool_bytes()),
+      fp8 ? pool.key_scale_pool() : nullptr, fp8 ? pool.value_scale_pool() : nullptr, fp8 ? pool.scale_pool_bytes() : 0,
+      fp8 ? PBE_KV_FP8_E4M3 : PBE_KV_BF16, args.num_kv_heads, args.head_size, args.queries, args.outputs, args.n_rows,
+      args.token_starts, args.batch_size, args.head_num, args.block_tables, args.seq_lens, args.max_blocks_per_seq,
+      args.workspace, args.workspace_bytes, device_, stream_);
+  if (rc == PBE_ERR_UNSUPPORTED) return false;
+  if (rc == PBE_ERR_INVALID) throw std::invalid_argument(std::string("prefill rejected: ") + pbe_last_error());
+  raise_if_failed(rc);
+  return true;
+}
+
 bool HipPagedKVRuntime::read(const base::KVPoolView& pool, const PagedKVDecodeRuntimeArgs& args,
                              const void* new_keys, const void* new_values) const {
   if (!pool.valid() || !pool.key_pool_bytes() || !pool.value_pool_bytes())

@@ -11,7 +11,8 @@
 // sizes the view carries; negative slots are skipped. Launches are asynchronous
 // on the runtime's stream. decode() reads any KVPoolView through
 // pbe_paged_decode_pools, and decode_append() writes the step's new tokens in
-// the same launch; prefill attention is outside this build.
+// the same launch. prefill() lets a chunk's many query tokens a sequence see its
+// pages, through pbe_paged_prompt_attention.
 #ifndef PBE_INCLUDE_MODEL_PAGED_KV_RUNTIME_H_
 #define PBE_INCLUDE_MODEL_PAGED_KV_RUNTIME_H_
 
@@ -41,6 +42,29 @@ struct PagedKVDecodeRuntimeArgs {
   void* workspace = nullptr;
   uint64_t workspace_bytes = 0;
   int32_t splits = 0;
+};
+
+// A prefill chunk's operands (or drafted tokens to check): what
+// pbe_build_step_tables makes of a step, and queries as pbe_qk_norm_rope_scatter
+// writes them. The chunk's own K and V are in the pages already (scatter()).
+struct PagedKVPrefillRuntimeArgs {
+  int32_t n_rows = 0;         // of queries and outputs
+  int32_t batch_size = 0;
+  int32_t head_num = 0;       // query heads
+  int32_t head_size = 0;
+  int32_t kv_mul = 0;         // head_num / num_kv_heads
+  int32_t max_blocks_per_seq = 0;
+  int32_t block_size = 0;     // 16
+  int32_t num_kv_heads = 0;
+  const void* queries = nullptr;          // bf16 [n_rows][head_num][head_size]
+  void* outputs = nullptr;                // the same; may be the queries
+  const int32_t* token_starts = nullptr;  // [batch + 1]
+  const int32_t* block_tables = nullptr;  // [batch][max_blocks_per_seq]
+  const int32_t* seq_lens = nullptr;      // [batch], the new tokens among them
+  // pbe_prompt_workspace_bytes(n_rows, batch_size, head_num, num_kv_heads, head_size);
+  // with less, or none, few rows over many keys take longer.
+  void* workspace = nullptr;
+  uint64_t workspace_bytes = 0;
 };
 
 class HipPagedKVRuntime {
@@ -77,6 +101,11 @@ class HipPagedKVRuntime {
   // rules as decode().
   bool decode_append(const base::KVPoolView& pool, const PagedKVDecodeRuntimeArgs& args, const void* new_keys,
                      const void* new_values) const;
+
+  // Causal attention of a chunk's query tokens over the pool, in place of the
+  // reference's prefill attention. Any number of query heads per KV head;
+  // otherwise the same return and throw rules as decode().
+  bool prefill(const base::KVPoolView& pool, const PagedKVPrefillRuntimeArgs& args) const;
 
   int device() const { return device_; }
   void* stream() const { return stream_; }

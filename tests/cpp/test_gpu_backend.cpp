@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <thread>
 #include <chrono>
+#include <cmath>
 #include <atomic>
 #include <memory>
 #include <string>
@@ -1279,6 +1280,135 @@ TEST_CASE("model runtime: prompt K/V written through KVCacheManager slots, then 
                     static_cast<void*>(ws)})
       HIP_OK(hipFree(d));
   }
+  REQUIRE(pbe_stream_destroy(0, stream) == PBE_OK);
+}
+
+TEST_CASE("model runtime: a chunk's query tokens attend to its pages") {
+  const int H = 2, D = 128, B = 16, nblk = 12, kvm = 6, batch = 3, max_blocks = 4, spare = 2;
+  void* stream = nullptr;
+  REQUIRE(pbe_stream_create(0, &stream) == PBE_OK);
+  const model::HipPagedKVRuntime runtime(0, stream);
+  const std::vector<int32_t> table{3, 7, 1, 10, 0, 6, -1, -1, 5, 9, 2, -1}, lens{64, 20, 33}, starts{0, 30, 31, 64};
+  const int rows = starts[batch] + spare;
+  const auto q = random_bf16(rows * kvm * H * D, 91);
+  int32_t* dt = to_device(table);
+  int32_t* dl = to_device(lens);
+  int32_t* ds = to_device(starts);
+  uint8_t* dq = to_device(q);
+  const uint64_t ws_bytes = pbe_prompt_workspace_bytes(rows, batch, kvm * H, H, D);
+  const int32_t splits = 2;
+  const uint64_t decode_bytes = pbe_paged_decode_workspace_bytes(batch, kvm * H, D, splits);
+  uint8_t *o1 = nullptr, *o2 = nullptr, *ws = nullptr;
+  HIP_OK(hipMalloc(&o1, q.size()));
+  HIP_OK(hipMalloc(&o2, q.size()));
+  HIP_OK(hipMalloc(&ws, std::max(ws_bytes, decode_bytes)));
+  REQUIRE(dt && dl && ds && dq);
+  for (const bool fp8 : {false, true}) {
+    base::BlockAllocator blocks(nblk, B, H, D, base::DataType::kDataTypeBf16, base::DeviceType::kDeviceHIP,
+                                fp8 ? base::BlockStorageMode::kFp8E4M3PerTokenHead : base::BlockStorageMode::kPlain);
+    const base::KVPoolView pool = blocks.pool_view();
+    // every token's K and V, written by the runtime itself
+    const auto K = random_bf16(nblk * B * H * D, 92), V = random_bf16(nblk * B * H * D, 93);
+    std::vector<int32_t> slots(nblk * B);
+    for (int i = 0; i < nblk * B; ++i) slots[i] = i;
+    uint8_t* dK = to_device(K);
+    uint8_t* dV = to_device(V);
+    int32_t* dS = to_device(slots);
+    REQUIRE(dK && dV && dS);
+    runtime.scatter(dK, dV, base::DataType::kDataTypeBf16, pool, dS, B, H, D, nblk * B);
+    HIP_OK(hipMemset(o1, 0x3f, q.size()));
+    HIP_OK(hipMemset(o2, 0x3f, q.size()));
+    model::PagedKVPrefillRuntimeArgs a;
+    a.n_rows = rows;
+    a.batch_size = batch;
+    a.head_num = kvm * H;
+    a.head_size = D;
+    a.kv_mul = kvm;
+    a.max_blocks_per_seq = max_blocks;
+    a.block_size = B;
+    a.num_kv_heads = H;
+    a.queries = dq;
+    a.outputs = o1;
+    a.token_starts = ds;
+    a.block_tables = dt;
+    a.seq_lens = dl;
+    a.workspace = ws;
+    a.workspace_bytes = ws_bytes;
+    CHECK(runtime.prefill(pool, a));
+    REQUIRE(pbe_stream_synchronize(0, stream) == PBE_OK);
+    const auto got = to_host(o1, q.size());
+    const size_t row = static_cast<size_t>(kvm) * H * D * 2;
+    for (size_t i = starts[batch] * row; i < got.size(); ++i) REQUIRE(got[i] == 0x3f);  // rows of no sequence
+    REQUIRE(pbe_paged_prompt_attention(pool.key_pool(), pool.value_pool(), pool.key_pool_bytes(),
+                                       fp8 ? pool.key_scale_pool() : nullptr, fp8 ? pool.value_scale_pool() : nullptr,
+                                       fp8 ? pool.scale_pool_bytes() : 0, fp8 ? PBE_KV_FP8_E4M3 : PBE_KV_BF16, H, D, dq,
+                                       o2, rows, ds, batch, kvm * H, dt, dl, max_blocks, ws, ws_bytes, 0,
+                                       stream) == PBE_OK);
+    REQUIRE(pbe_stream_synchronize(0, stream) == PBE_OK);
+    CHECK(got == to_host(o2, q.size()));
+    // A sequence's last row sees what a decode step sees. Of values below M each reader
+    // is off by less than 2^-8 (its output's rounding) + 2^-8 (its weights') and a
+    // little of M.
+    std::vector<uint8_t> last;
+    for (int b = 0; b < batch; ++b) last.insert(last.end(), q.begin() + (starts[b + 1] - 1) * row, q.begin() + starts[b + 1] * row);
+    uint8_t* dlast = to_device(last);
+    REQUIRE(dlast);
+    model::PagedKVDecodeRuntimeArgs d;
+    d.batch_size = batch;
+    d.head_num = kvm * H;
+    d.head_size = D;
+    d.kv_mul = kvm;
+    d.max_blocks_per_seq = max_blocks;
+    d.block_size = B;
+    d.num_kv_heads = H;
+    d.queries = dlast;
+    d.outputs = o2;
+    d.block_tables = dt;
+    d.seq_lens = dl;
+    d.workspace = ws;
+    d.workspace_bytes = decode_bytes;
+    d.splits = splits;
+    CHECK(runtime.decode(pool, d));
+    REQUIRE(pbe_stream_synchronize(0, stream) == PBE_OK);
+    const auto one = to_host(o2, batch * row);
+    auto value = [](const std::vector<uint8_t>& x, size_t i) {
+      const uint32_t bits = (static_cast<uint32_t>(x[2 * i]) | static_cast<uint32_t>(x[2 * i + 1]) << 8) << 16;
+      float f;
+      std::memcpy(&f, &bits, 4);
+      return f;
+    };
+    float most = 0.f, apart = 0.f;
+    for (size_t i = 0; i < V.size() / 2; ++i) most = std::max(most, std::fabs(value(V, i)));
+    for (int b = 0; b < batch; ++b)
+      for (size_t i = 0; i < row / 2; ++i)
+        apart = std::max(apart, std::fabs(value(one, b * row / 2 + i) - value(got, (starts[b + 1] - 1) * row / 2 + i)));
+    CHECK(apart <= 2.f * (1.f / 128.f + 1.f / 4096.f) * most * (fp8 ? 1.0625f : 1.f));  // E4M3 values: 2^-4 more
+    // no workspace: the same to within the order of sums, and in place
+    a.workspace = nullptr;
+    a.workspace_bytes = 0;
+    a.queries = a.outputs = o1;
+    HIP_OK(hipMemcpy(o1, q.data(), q.size(), hipMemcpyHostToDevice));
+    CHECK(runtime.prefill(pool, a));
+    REQUIRE(pbe_stream_synchronize(0, stream) == PBE_OK);
+    a.queries = dq;
+    a.block_size = 32;
+    CHECK(!runtime.prefill(pool, a));
+    a.block_size = B;
+    a.head_size = 96;
+    CHECK(!runtime.prefill(pool, a));
+    a.head_size = D;
+    a.kv_mul = 5;
+    CHECK_THROWS_AS(runtime.prefill(pool, a), std::invalid_argument);
+    a.kv_mul = kvm;
+    a.outputs = dq + 16;
+    CHECK_THROWS_AS(runtime.prefill(pool, a), std::invalid_argument);
+    a.outputs = nullptr;
+    CHECK_THROWS_AS(runtime.prefill(pool, a), std::invalid_argument);
+    for (void* x : {static_cast<void*>(dK), static_cast<void*>(dV), static_cast<void*>(dS), static_cast<void*>(dlast)}) HIP_OK(hipFree(x));
+  }
+  for (void* x : {static_cast<void*>(dt), static_cast<void*>(dl), static_cast<void*>(ds), static_cast<void*>(dq), static_cast<void*>(o1),
+                  static_cast<void*>(o2), static_cast<void*>(ws)})
+    HIP_OK(hipFree(x));
   REQUIRE(pbe_stream_destroy(0, stream) == PBE_OK);
 }
 

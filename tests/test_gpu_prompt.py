@@ -223,3 +223,227 @@ def test_pages_of_one_sequence_in_pieces(torch_cuda, kind, dim, new, length):
         c.out.fill_(5.0)
         c.call(torch.full((n,), 0xff, dtype=torch.uint8, device="cuda"))
         c.check()
+
+
+def test_many_sequences(torch_cuda):
+    torch = torch_cuda
+    say("prompt: 150 sequences")
+    rng = np.random.default_rng(5)
+    news, cached = [int(x) for x in rng.integers(0, 12, 150)], [int(x) for x in rng.integers(0, 90, 150)]
+    news[70], cached[70] = 90, 700
+    c = Rows(torch, news, cached, 2, 3, 64, seed=8)
+    for n in (None, torch.empty(0, dtype=torch.uint8, device="cuda")):
+        c.out.fill_(5.0)
+        c.call(n)
+        c.check()
+    p = Pages(torch, [(a + b, a) for a, b in zip(news, cached)], 1, 2, 128, "mxfp4", seed=8)
+    p.call()
+    p.check()
+
+
+@pytest.mark.parametrize("kind", ["rows", "bf16", "fp8"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("news,lens,group", [([1, 40, 3], [1, 40, 700], 3), ([300], [520], 7), ([70, 1], [600, 65], 1)])
+def test_infinities_and_nans_reach_only_the_rows_that_see_them(torch_cuda, kind, dim, news, lens, group):
+    """Keys and values of infinity and NaN, one a place of its own, on both sides of
+    tiles' ends."""
+    torch = torch_cuda
+    say(f"prompt {kind} D={dim}: infinities and NaN, {news} of {lens}")
+    heads = 2
+    if kind == "rows":
+        c = Rows(torch, news, [a - b for a, b in zip(lens, news)], heads, group, dim, seed=dim)
+        at, k, v = c.ks, c.k.view(-1, heads, dim), c.v.view(-1, heads, dim)
+    else:
+        c = Pages(torch, list(zip(lens, news)), heads, group, dim, kind, seed=dim)
+        k, v = (x[0].view(-1, heads, dim) for x in c.pools)
+    inf, nan = float("inf"), float("nan")
+    for b, n in enumerate(lens):
+        for j, (what, value) in enumerate([("v", inf), ("v", -inf), ("v", nan), ("k", -inf), ("k", nan), ("v", inf), ("v", -inf)]):
+            # places a row or two from the end, the last two on one dim; keys of one head
+            t = n - 1 - (3 * j + 1) % max(1, min(n, 60))
+            if t < 0 or (n == 1 and j):
+                continue
+            if kind == "fp8" and value != nan:
+                continue                            # E4M3 has no infinities
+            slot = int(at[b]) + t if kind == "rows" else int(c.slots[b][t])
+            d, h = (5 if j >= 5 else (11 * j) % dim), (1 if what == "v" else 0)
+            store = 0x7f if kind == "fp8" else value
+            (v if what == "v" else k)[slot, h, d] = store
+            if kind != "rows":
+                c.host[1 if what == "v" else 0][slot, h, d] = value
+    c.call()
+    c.check()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("size", [1.0, 64.0, 2.0 ** 40, 2.0 ** 100])
+def test_equal_scores_of_any_size_weigh_alike(torch_cuda, dim, size):
+    """Keys that are all the same: whatever the scores, outputs are means, off by
+    their own rounding and that of sums of n / 16 + 600 products."""
+    torch = torch_cuda
+    say(f"prompt: equal scores of size {size}")
+    c = Rows(torch, [5, 300], [700, 0], 1, 2, dim, seed=dim, size=size)
+    c.k[:] = c.k[:1].clone()
+    c.call()
+    v = c.v.double().cpu().numpy()
+    got = c.out.double().cpu().numpy()
+    for b in range(2):
+        n, m = c.news[b], c.lens[b]
+        for i in range(n):
+            seen = v[c.ks[b]:c.ks[b] + m - n + i + 1]
+            bound = 2.0 ** -8 * np.abs(seen.mean(0)) + (m / 16 + 600) * 2.0 ** -23 * np.abs(seen).mean(0)
+            assert (np.abs(got[c.qs[b] + i] - seen.mean(0)) <= bound).all()
+
+
+def test_constant_values_come_back_as_they_are(torch_cuda):
+    say("prompt: constant values")
+    for kind in ("bf16", "mxfp4"):
+        c = Pages(torch_cuda, [(900, 200), (33, 33)], 2, 4, 128, kind, seed=3)
+        pool = c.pools[1]
+        if kind == "bf16":
+            pool[0].fill_(1.5)
+        else:
+            pool[0].fill_(0x33)      # codes of 1.5
+            pool[1].fill_(127)
+        c.call()
+        c.torch.cuda.synchronize()
+        assert (c.out[: c.starts[-1]] == 1.5).all()
+
+
+def test_rows_and_sequences_that_make_no_sense(torch_cuda):
+    torch = torch_cuda
+    say("prompt: bad starts, lengths and ids")
+    # starts: rows before 0, behind the last, in the wrong order; keys beyond theirs
+    c = Rows(torch, [20, 30, 10, 25], [0, 40, 5, 6], 2, 2, 64, seed=1)
+    n_q, n_k = len(c.q), len(c.k)
+    for qs, ks, nan, good in (([-4, 20, 50, 60, 85], c.ks, (0, 20), (1, 2, 3)), ([0, 20, 50, 60, n_q + 1], c.ks, (60, n_q), (0, 1, 2)),
+                              (c.qs, [0, 20, 90, 105, n_k + 1], (60, 85), (0, 1, 2)), (c.qs, [0, 20, 90, 80, 111], (50, 60), (0, 1))):
+        c.out.fill_(5.0)
+        c.call(starts=(np.array(qs, np.int32), np.array(ks, np.int32)))
+        got = c.out.double().cpu().numpy()
+        assert np.isnan(got[nan[0]:nan[1]]).all()
+        q, k, v = (x.double().cpu().numpy().reshape(len(x), -1, 64) for x in (c.q, c.k, c.v))
+        for b in good:
+            within(got[qs[b]:qs[b + 1]], q[qs[b]:qs[b + 1]], k[ks[b]:ks[b + 1]], v[ks[b]:ks[b + 1]])
+    c.out.fill_(5.0)
+    c.call(starts=(np.array([0, 20, 10, 60, 85], np.int32), c.ks))   # the second ends before it begins: it has no rows
+    assert not (c.out[60:85] == 5.0).any() and (c.out[85:] == 5.0).all()
+    # a length of more queries than keys: the first see nothing
+    c = Rows(torch, [20], [0], 1, 3, 64, seed=2, spare=0)
+    c.lens, c.ks = [8], np.array([0, 8], np.int32)
+    c.call()
+    got = c.out.double().cpu().numpy()
+    assert (got[:12] == 0).all()
+    q, k, v = (x.double().cpu().numpy().reshape(20, -1, 64) for x in (c.q, c.k, c.v))
+    within(got[12:], q[12:], k[:8], v[:8])
+    for kind in ("bf16", "fp8", "mxfp4"):
+        reqs = [(100, 40), (50, 50), (70, 3), (1500, 20), (33, 2)]
+        p = Pages(torch, reqs, 2, 3, 128, kind, seed=5)
+        lens, tables = p.lens.copy(), p.tables.copy()
+        lens[0], lens[4] = -1, (p.max_blocks + 1) * T
+        tables[1, 2], tables[3, 70] = p.blocks, -1      # keys 32..47 and 1120..1135
+        p.dev[1:] = [torch.from_numpy(tables).cuda(), torch.from_numpy(lens).cuda()]
+        p.call()
+        got = p.check(skip=(0, 1, 3, 4))
+        s = p.starts
+        assert np.isnan(got[s[0]:s[1]]).all() and np.isnan(got[s[4]:s[5]]).all() and np.isnan(got[s[3]:s[4]]).all()
+        assert np.isnan(got[s[1] + 32:s[2]]).all()
+        slots = p.slots[1]
+        within(got[s[1]:s[1] + 32], p.q_host[s[1]:s[1] + 32], p.host[0][slots[:32]], p.host[1][slots[:32]], kind == "fp8")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "mxfp4"])
+def test_captured_calls_follow_what_changes_between_replays(torch_cuda, kind):
+    """Two graphs that share a workspace, replayed in turn on a stream of their own
+    while lengths and queries change, against eager calls."""
+    torch = torch_cuda
+    say(f"prompt {kind}: captured")
+    cases = [Pages(torch, [(1500, 30), (200, 64), (17, 1)], 2, 3, 128, kind, seed=s) for s in (1, 2)]
+    need = max(P.prompt_workspace_bytes(len(c.q), 3, 6, 2, 128) for c in cases)
+    ws = torch.full((need,), 0xff, dtype=torch.uint8, device="cuda")
+    side, graphs = torch.cuda.Stream(), []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side):
+            with torch.cuda.graph(g, stream=side):
+                c.call(ws, stream=side.cuda_stream)
+        graphs.append(g)
+    for rep in range(4):
+        for c, g in zip(cases, graphs):
+            lens = torch.tensor([1500 - 64 * rep, 200 - rep, 17], dtype=torch.int32, device="cuda")
+            c.dev[2].copy_(lens)
+            c.q.copy_(c.q.roll(1, 0))
+            want = torch.full_like(c.out, 5.0)
+            c.call(out=want)
+            c.out.fill_(5.0)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(c.out.view(torch.int16), want.view(torch.int16)), rep
+
+
+def test_calls_beside_each_other_and_in_place(torch_cuda):
+    torch = torch_cuda
+    say("prompt: two streams, outputs over queries")
+    cases = [Pages(torch, [(2500, 200), (300, 7)], 2, 6, 128, k, seed=i) for i, k in enumerate(("bf16", "fp8", "mxfp4", "bf16"))]
+    for c in cases:
+        c.call()
+    torch.cuda.synchronize()
+    want = [c.out.clone() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    kept = []
+    for c in cases:
+        c.out.fill_(5.0)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                kept.append(c.call(stream=s.cuda_stream))
+    torch.cuda.synchronize()
+    for c, w in zip(cases, want):
+        assert torch.equal(c.out.view(torch.int16), w.view(torch.int16))
+        n = int(c.starts[-1])
+        q = c.q.clone()
+        c.call(out=q, q=q)
+        torch.cuda.synchronize()
+        assert torch.equal(q[:n].view(torch.int16), w[:n].view(torch.int16)) and torch.equal(q[n:], c.q[n:])
+    r = Rows(torch, [300, 20], [50, 900], 2, 3, 64, seed=4)
+    r.call()
+    w = r.out.clone()
+    q = r.q
+    r.call(out=q.view(len(q), 6, 64))
+    assert torch.equal(q.view(len(q), 6, 64)[:320].view(torch.int16), w[:320].view(torch.int16))
+
+
+def test_pages_beyond_four_gigabytes(torch_cuda):
+    torch = torch_cuda
+    say("prompt: pools of 5 GiB")
+    heads, dim, group = 2, 128, 3
+    half = T * heads * dim * 2
+    blocks = 5 * 2 ** 30 // half
+    c = Pages(torch, [(150, 40), (70, 2)], heads, group, dim, "bf16", seed=6, spare=0)
+    big = [torch.zeros((blocks * T, heads, dim), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    far = blocks - c.blocks
+    for x, (small, _) in zip(big, c.pools):
+        x[far * T:] = small
+    tables = c.tables.copy()
+    for b, (n, _) in enumerate(c.reqs):
+        tables[b, : -(-n // T)] += far
+    c.dev[1] = torch.from_numpy(tables).cuda()
+    c.pools = [[x, None] for x in big]
+    c.blocks = blocks
+    c.call()
+    c.check()
+
+
+def test_long_sequences_and_each_tile_size(torch_cuda):
+    """Rows per sequence of 32, 64, 128, 256 and more, a query head or two each, over a
+    few thousand keys; the last rows against the oracle."""
+    torch = torch_cuda
+    for kind, dim in (("bf16", 128), ("fp8", 128), ("fp8", 64), ("mxfp4", 64), ("mxfp4", 128), ("bf16", 64)):
+        for new in (20, 33, 100, 200, 700):
+            say(f"prompt pages {kind} D={dim}: {new} rows over 3000 keys")
+            c = Pages(torch, [(3001, new), (2999, new)], 1, 1, dim, kind, seed=new)
+            c.call()
+            c.check()
