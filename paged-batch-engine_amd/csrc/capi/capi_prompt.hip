@@ -71,8 +71,10 @@ uint64_t pbe_prompt_workspace_bytes(int32_t n_rows, int32_t batch, int32_t q_hea
   if (n_rows <= 0 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_heads % kv_heads) return 0;
   uint64_t most = 0;  // over the kinds of keys and values
   for (const pbe::KeyKind kind : {pbe::KeyKind::kRows, pbe::KeyKind::kBf16, pbe::KeyKind::kFp8, pbe::KeyKind::kMxfp4}) {
-    const pbe::PromptPlan r = pbe::plan_prompt(n_rows, batch, q_heads / kv_heads, kv_heads, kind, INT32_MAX, compute_units(), ~0ull, head_dim);
-    most = std::max(most, (uint64_t)r.parts * r.each);
+    for (const int64_t keys : {(int64_t)INT32_MAX, (int64_t)512 * batch - 1}) {  // over sequences, long and short
+      const pbe::PromptPlan r = pbe::plan_prompt(n_rows, batch, q_heads / kv_heads, kv_heads, kind, keys, compute_units(), ~0ull, head_dim);
+      most = std::max(most, (uint64_t)r.parts * r.each);
+    }
   }
   return most;
 }

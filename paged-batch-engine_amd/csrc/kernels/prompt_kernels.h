@@ -42,7 +42,7 @@ struct PromptPlan {
   int32_t parts = 0;
   uint64_t each = 0;
 };
-// most_keys: that a sequence may have; units: compute units.
+// most_keys: that a sequence may have (rows: that there are); units: compute units.
 PromptPlan plan_prompt(int64_t n_q, int64_t batch, int32_t group, int32_t kv_heads, KeyKind kind, int64_t most_keys, int64_t units, uint64_t workspace,
                        int32_t head_dim);
 

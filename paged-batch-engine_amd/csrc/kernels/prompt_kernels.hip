@@ -22,7 +22,9 @@
 // special values (see there) looked for in masked tiles only, in place 507; reads some
 // products ahead and one multiply-add before each exponential 485; 256 rows 469; no bank
 // conflicts 462.
-// Tried and slower: the next tile's scores among this one's weights in one wave (510 for
+// Tried and slower: 64 rows a wave, operands from LDS used twice, one half's softmax
+// beside the other's products (554 for 469: with 478 registers the compiler moves operands
+// between the files before most products), the next tile's scores among this one's weights in one wave (510 for
 // 469), the workgroup's halves taking turns (507 for 462), three tiles in LDS (503 for
 // 469), V's loads after all of K's (500 for 467). Waves' priorities changed nothing.
 //
@@ -551,8 +553,7 @@ __device__ __forceinline__ void workgroup_of(const PromptParams& p, int* w, int*
 // barrier a tile (MXFP4: two), behind which the tile read before is overwritten.
 // Registers: O 4 x 16, scores 32, Q 32, weights 16; two waves a SIMD.
 // FP8 codes become BF16 operands at the LDS reads: once a tile instead, into BF16 tiles,
-// took the same time (130.8 and 130.4 us, 128 new tokens in each of 10 sequences) and
-// more LDS. The matrix product of 8-bit operands is no faster at this shape and would
+// took the same time (130.8 and 130.4 us, 128 tokens at the end of 32,768) and more LDS. The matrix product of 8-bit operands is no faster at this shape and would
 // round the queries.
 template <int D, KeyKind kKind, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, kWaves > 2 ? 2 : 1) void prompt_attention_kernel(const PromptParams p) {
@@ -976,7 +977,9 @@ hipError_t launch(const PromptParams& p, int64_t workgroups, hipStream_t stream)
 template <int D, KeyKind kKind>
 hipError_t launch_rows(const PromptParams& p, int rows, int64_t workgroups, hipStream_t stream) {
   switch (rows) {
-    case 32: return launch<D, kKind, 1>(p, workgroups, stream);
+    case 32:
+      if constexpr (kKind == KeyKind::kFp8 && D == 128) return launch<D, kKind, 1>(p, workgroups, stream);
+      return hipErrorInvalidValue;
     case 64: return launch<D, kKind, 2>(p, workgroups, stream);
     case 128: return launch<D, kKind, 4>(p, workgroups, stream);
     default: return launch<D, kKind, 8>(p, workgroups, stream);
@@ -1011,9 +1014,20 @@ PromptPlan plan_prompt(int64_t n_q, int64_t batch, int32_t group, int32_t kv_hea
   PromptPlan r;
   const int64_t rows = n_q * group;
   // The fewest rows that hold an average sequence's: more rows read K and V from LDS and
-  // cache less often (128 instead of 256 over 8,192 tokens: 509 for 483 us; over 2,041
-  // behind 5,040: 122 for 109), rows that no token fills cost as much as others.
-  r.rows = rows <= 32 * batch ? 32 : rows <= 64 * batch ? 64 : rows <= 128 * batch ? 128 : 256;
+  // cache less often (256 and 128 rows a tile over 8,192 tokens: 469 and 495 us; over
+  // 2,041 behind 5,040: 109 and 122), rows that no token fills cost as much as others.
+  r.rows = rows <= 64 * batch ? 64 : rows <= 128 * batch ? 128 : 256;
+  // A wave alone loads and waits by itself, and is slower (64 x 4 tokens over MXFP4 pages
+  // of 128 dims: 66 us, two waves with one at work 54; over BF16 pages 80 and 81; 4 x 4
+  // over FP8 pages 40 and 34), but for FP8 pages of 128 dims and heads enough for a
+  // quarter of the GPU: 64 x 4 tokens 57 and 70, 16 x 4 of four KV heads 45 and 48, 16 x
+  // 4 of two 46 and 42.
+  if (rows <= 32 * batch && kind == KeyKind::kFp8 && head_dim == 128 && 4 * batch * kv_heads >= units) r.rows = 32;
+  // Few short prompts, whose tiles are not cut: smaller tiles, so that more compute units
+  // have one (41 tokens of 14 heads of 64 dims: 256 rows a tile 7.2 us, 128 5.9, 64 5.6;
+  // eight of 128 tokens 14.5, 12.7, 13.2).
+  const int64_t keys = kind == KeyKind::kRows ? most_keys / batch : most_keys;  // of a sequence, on the average or at most
+  while (r.rows > 64 && keys < 2 * kEdge * kKeys && 2 * (rows / r.rows + std::min(batch, n_q)) * kv_heads < units) r.rows /= 2;
   r.tiles = rows / r.rows + std::min(batch, n_q);
   // workgroups that a compute unit holds: eight waves' registers, 160 KiB of LDS
   const int64_t held = std::min<int64_t>(256 / r.rows, 160 * 1024 / (lds_bytes(kind, head_dim) + 64));
