@@ -876,10 +876,10 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 2 ? 2 : 1) void prompt_attent
 // begin it has a workgroup here, which takes its share of the tile's rows. A launch of
 // its own: the last part to end a tile joining it instead would need flags that every
 // call clears, and would leave the join's order of sums to chance or wait for it.
-constexpr int kJoinRows = 4;  // of a thread at once, so that their loads are on their way together
+constexpr int kTogether = 4;  // loads of a thread that are on their way together
 template <int D, int kRows>
 constexpr int join_threads() {
-  return D / 4 * kRows / kJoinRows < 1024 ? D / 4 * kRows / kJoinRows : 1024;
+  return D / 4 * kRows / kTogether < 1024 ? D / 4 * kRows / kTogether : 1024;
 }
 template <int D, KeyKind kKind, int kRows>
 __global__ __launch_bounds__((join_threads<D, kRows>())) void prompt_join_kernel(const PromptParams p) {
@@ -924,39 +924,52 @@ __global__ __launch_bounds__((join_threads<D, kRows>())) void prompt_join_kernel
   const int from = (int)((int64_t)rows * share / n), to = (int)((int64_t)rows * (share + 1) / n);
   const int q_heads = p.kv_heads * p.group;
   const bool begins = cuts[0] == 0;  // else its first tile was another one
-  constexpr int kStep = join_threads<D, kRows>() / kLanes, kTogether = kJoinRows;
+  constexpr int kStep = join_threads<D, kRows>() / kLanes;
   const int d = 4 * ((int)threadIdx.x % kLanes);
+  // A thread has kTogether rows and a part at a time, or, where the share has no more
+  // rows than are under way at once, a row and kTogether parts (128 tokens at the end of
+  // 32,768: 129 to 119 us; 4 x 4 tokens over 5,040: 35 to 30). Eight parts take registers
+  // that cost more workgroups at once than they save: 64 x 4 over MXFP4 pages 81 to 90.
+  const bool few = to - from <= kStep;
+  const int next_row = few ? 0 : kStep, next_part = few ? 1 : 0;
+  auto add_to = [&](float& m, float& l, f32x4& acc, float pm, float pl, f32x4 x) {
+    const float now = fmaxf(m, pm), base = now == -INFINITY ? 0.f : now;
+    const float old = m == now ? 1.f : __builtin_amdgcn_exp2f((m - base) * p.scale);
+    const float add = pm == now ? 1.f : __builtin_amdgcn_exp2f((pm - base) * p.scale);
+    m = now;
+    l = l * old + pl * add;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] = acc[c] * old + x[c] * add;
+  };
   for (int r0 = from + (int)threadIdx.x / kLanes; r0 < to; r0 += kTogether * kStep) {
     float m[kTogether], l[kTogether];
     f32x4 acc[kTogether];
 #pragma unroll
     for (int e = 0; e < kTogether; ++e) m[e] = -INFINITY, l[e] = 0.f, acc[e] = f32x4{};
-    for (int i = 0; i <= n; ++i) {
-      if (max(cuts[i], 0) == cuts[i + 1]) continue;  // nothing between two cuts
-      const uint64_t place = (((uint64_t)(w0 + i) * 2 + (i == 0 && !begins)) * (uint64_t)p.kv_heads + (uint64_t)head) * kRows;
+    for (int i0 = 0; i0 <= n; i0 += few ? kTogether : 1) {
       f32x2 ml[kTogether];
       f32x4 x[kTogether];
 #pragma unroll
       for (int e = 0; e < kTogether; ++e) {
-        const uint64_t at_row = place + (uint64_t)min(r0 + e * kStep, to - 1);
+        const int i = i0 + e * next_part;
+        ml[e] = f32x2{-INFINITY, 0.f}, x[e] = f32x4{};
+        if (i > n || max(cuts[i], 0) == cuts[i + 1]) continue;  // nothing between two cuts
+        const uint64_t place = (((uint64_t)(w0 + i) * 2 + (i == 0 && !begins)) * (uint64_t)p.kv_heads + (uint64_t)head) * kRows;
+        const uint64_t at_row = place + (uint64_t)min(r0 + e * next_row, to - 1);
         ml[e] = *(PBE_GLOBAL const f32x2*)(uintptr_t)(p.part_ml + at_row * 2);
         x[e] = *(PBE_GLOBAL const f32x4*)(uintptr_t)(p.part_acc + at_row * D + d);
       }
 #pragma unroll
-      for (int e = 0; e < kTogether; ++e) {
-        const float now = fmaxf(m[e], ml[e].x), base = now == -INFINITY ? 0.f : now;
-        const float old = m[e] == now ? 1.f : __builtin_amdgcn_exp2f((m[e] - base) * p.scale);
-        const float add = ml[e].x == now ? 1.f : __builtin_amdgcn_exp2f((ml[e].x - base) * p.scale);
-        m[e] = now;
-        l[e] = l[e] * old + ml[e].y * add;
+      for (int e = 0; e < kTogether; ++e) add_to(m[e], l[e], acc[e], ml[e].x, ml[e].y, x[e]);
+    }
+    if (few) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[e][c] = acc[e][c] * old + x[e][c] * add;
-      }
+      for (int e = 1; e < kTogether; ++e) add_to(m[0], l[0], acc[0], m[e], l[e], acc[e]);
     }
 #pragma unroll
     for (int e = 0; e < kTogether; ++e) {
+      if (e > 0 && (few || r0 + e * kStep >= to)) break;
       const int row = at.t * kRows + r0 + e * kStep;
-      if (r0 + e * kStep >= to) break;
       const int token = (int)fast_div((uint32_t)row, p.by_group), g = row - token * p.group;
       const float over = seen_by(u, token) > 0 ? 1.f / l[e] : 0.f;
       *(PBE_GLOBAL u32x2*)(uintptr_t)(p.out + (((uint64_t)u.begin + token) * (uint64_t)q_heads + (uint64_t)(head * p.group + g)) * (2 * D) + 2 * d) =
