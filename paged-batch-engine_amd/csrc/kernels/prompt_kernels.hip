@@ -14,19 +14,22 @@
 //
 // Bound: MFMA, 4 * D FLOP a row and seen key. 4 * 128 dims take 32 products of 8
 // passes each a wave and tile, beside about 400 instructions for 64 weights a lane pair.
-// Over 8,192 tokens of 28 heads of 128 dims: 462 us, 1,040 TFLOP/s, of the 1,387 that a
-// large matrix product reaches here; MFMA busy 49% at 2.05 GHz (the clock falls as the
-// kernel gets faster). Leaving out the exponentials, or the maxima, or the sums, takes 6
-// to 9% off (on the way there, of 526 us): no single part is the bound.
+// Over 8,192 tokens of 28 heads of 128 dims: 455 to 477 us by run, 1,010 to 1,058
+// TFLOP/s, of the 1,387 that a large matrix product reaches here; MFMA busy 49% at 2.05
+// GHz (the clock falls as the kernel gets faster). A SIMD's two waves share a barrier a
+// tile and mostly multiply, and mostly weigh, at the same time. Leaving out the
+// exponentials, or the maxima, or the sums, takes 6 to 9% off (on the way there, of 526
+// us): no single part is the bound.
 // What that took, in us, each measured against the one before: 128 rows a workgroup 526;
 // special values (see there) looked for in masked tiles only, in place 507; reads some
 // products ahead and one multiply-add before each exponential 485; 256 rows 469; no bank
 // conflicts 462.
 // Tried and slower: 64 rows a wave, operands from LDS used twice, one half's softmax
 // beside the other's products (554 for 469: with 478 registers the compiler moves operands
-// between the files before most products), the next tile's scores among this one's weights in one wave (510 for
-// 469), the workgroup's halves taking turns (507 for 462), three tiles in LDS (503 for
-// 469), V's loads after all of K's (500 for 467). Waves' priorities changed nothing.
+// between the files before most products), the next tile's scores among this one's
+// weights in one wave (510 for 469), the workgroup's halves taking turns (507 for 462),
+// three tiles in LDS (503 for 469), V's loads after all of K's (500 for 467). Waves'
+// priorities changed nothing.
 //
 // A weight goes into its product as one BF16 number, off by at most 2^-8 of itself (two
 // numbers each would double the second product's MFMA). Over rows, BF16 and MXFP4 pages
@@ -160,7 +163,8 @@ __device__ __forceinline__ Found find_seq(int batch, int64_t x, int lane, Of of)
 // A cut tile's partial results go to the workspace and prompt_join_kernel joins them.
 // The device does all of it from the starts and lengths, so captured calls follow them.
 // 2,041 tokens behind 5,040 others, 12 heads: 109 us. What it costs: 2.5 to 3.3 us to
-// find a part, about 3 to write partials, 12 to 15 the join.
+// find a part, about 3 to write partials, 9 to 16 the join (of 256 rows a tile, some 40 MB
+// of partials).
 // Where there are two tiles a slot or more, a workgroup takes one whole tile and those
 // that cost the most go first (16 mixed prompts: 96 us; cut into parts 126).
 //

@@ -213,3 +213,47 @@ def test_compacted_pages_are_one_run(torch_cuda):
     rows, _ = rows_of(rng, [160, 300, 47], 200, 1, 20)
     out, _, counts, _ = check_compact(torch_cuda, pool, rows)
     assert sorted(out[out >= 0]) == list(range(counts[0]))
+
+
+def test_captured_moves_follow_what_changes_between_replays(torch_cuda):
+    """A compaction behind a fork in one graph on a stream of its own, replayed in turn
+    with another graph that shares the workspace."""
+    torch = torch_cuda
+    say("fork and compact in graphs that share a workspace")
+    n, width, rows = 70, 8, 5
+    ws = torch.full((max(P.fork_pages_workspace_bytes(n, rows, rows), P.compact_pages_workspace_bytes(n)),), 0xff, dtype=torch.uint8, device="cuda")
+    side, runs = torch.cuda.Stream(), []
+    for seed in range(2):
+        rng = np.random.default_rng(seed)
+        pool = Pool(torch, n, (4096, 528), 0, seed)
+        lens = [int(x) for x in rng.integers(1, 60, rows)]
+        tables, _ = rows_of(rng, lens, n, 3, width)
+        dev = [ints(torch, x) for x in (tables, lens, range(rows))]
+        mid, mid_lens, counts, last, moved = ints(torch, np.zeros((rows, width))), ints(torch, [0] * rows), ints(torch, [0, 0]), \
+            ints(torch, np.zeros((rows, width))), ints(torch, [0] * n)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side):
+            with torch.cuda.graph(g, stream=side):
+                P.fork_pages(pool.planes, n, 3, 16, ptr(dev[0]), ptr(dev[1]), rows, ptr(dev[2]), 0, rows, width, 0, mid.data_ptr(),
+                             mid_lens.data_ptr(), counts.data_ptr(), ws.data_ptr(), ws.numel(), stream=side.cuda_stream)
+                P.compact_pages(pool.planes, n, 3, mid.data_ptr(), rows, width, 0, last.data_ptr(), moved.data_ptr(), counts.data_ptr(), ws.data_ptr(),
+                                ws.numel(), stream=side.cuda_stream)
+        runs.append((g, pool, rng, tables, lens, dev, mid, mid_lens, last, moved, counts))
+    for rep in range(4):
+        for g, pool, rng, tables, lens, dev, mid, mid_lens, last, moved, counts in runs:
+            parents = rng.integers(-1, rows, rows)
+            dev[2].copy_(ints(torch, parents))
+            want = O.fork(tables, np.asarray(lens), parents, None, n, 3, 16)
+            packed = O.compact(want[0], n, 3)
+            pages = pool.host()
+            for moves in (want[3], packed[3]):
+                for x in pages:
+                    x[[b for _, b in moves]] = x[[a for a, _ in moves]]
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                g.replay()
+            torch.cuda.synchronize()
+            for got, x in zip((mid, mid_lens, last, moved, counts), (want[0], want[1], *packed[:3])):
+                np.testing.assert_array_equal(got.cpu().numpy(), x)
+            for got, x in zip(pool.host(), pages):
+                np.testing.assert_array_equal(got, x)
