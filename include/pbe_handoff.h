@@ -664,7 +664,9 @@ int pbe_qk_norm_rope_scatter(const void* q, int64_t q_stride, const void* k, int
  * An infinity or a NaN in a key or value reaches the queries that see it, and no
  * other. A score beyond FP32's range, or NaN: -infinity takes a key's weight to
  * zero, +infinity, NaN, or -infinity for all keys that a query sees, its head to
- * NaN. Query rows that belong to no sequence are left as they are. The order of a
+ * NaN. Weights (up to 2^8, their largest at least 1) times values are summed in FP32
+ * before they are divided, so values beyond 2^119 over a row's keys may end as
+ * infinities. Query rows that belong to no sequence are left as they are. The order of a
  * row's sums, and with it the last bits of its outputs, depends on the batch it is
  * in and on the workspace's size; for one call they are the same every time.
  *

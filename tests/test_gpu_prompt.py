@@ -447,3 +447,46 @@ def test_long_sequences_and_each_tile_size(torch_cuda):
             c = Pages(torch, [(3001, new), (2999, new)], 1, 1, dim, kind, seed=new)
             c.call()
             c.check()
+
+
+def test_no_keys_at_all_give_zeros(torch_cuda):
+    torch = torch_cuda
+    say("prompt: no keys")
+    q = torch.randn((70, 128), device="cuda").to(torch.bfloat16)
+    out = torch.full((70, 128), 5.0, dtype=torch.bfloat16, device="cuda")
+    starts = torch.tensor([0, 1, 65], dtype=torch.int32, device="cuda")
+    none = torch.zeros(3, dtype=torch.int32, device="cuda")
+    P.prompt_attention(q.data_ptr(), 128, 0, 64, 0, 64, 70, 0, starts.data_ptr(), none.data_ptr(), 2, 2, 1, 64, out.data_ptr(), 0, 0,
+                       stream=stream_ptr(torch))
+    torch.cuda.synchronize()
+    assert (out[:65] == 0).all() and (out[65:] == 5.0).all()
+
+
+def test_values_up_to_the_sums_range(torch_cuda):
+    """Values of 2^100 and queries whose scores climb from key to key, so that the
+    maximum moves all the time."""
+    torch = torch_cuda
+    say("prompt: large values, climbing scores")
+    for kind in ("bf16", "fp8"):
+        c = Pages(torch, [(700, 90), (64, 64)], 1, 2, 64, kind, seed=12)
+        slots = np.concatenate(c.slots)
+        climb = np.concatenate([np.arange(n) / 64.0 for n, _ in c.reqs])
+        c.q.fill_(1.0)
+        c.q_host[:] = 1.0
+        at = torch.from_numpy(slots).cuda()
+        if kind == "bf16":
+            k = torch.from_numpy(climb).to(torch.bfloat16)
+            c.pools[0][0][at] = k.cuda()[:, None, None]
+            c.host[0][slots] = k.double().numpy()[:, None, None]
+            big = (c.pools[1][0][at].float() * 2.0 ** 100).to(torch.bfloat16)
+            c.pools[1][0][at] = big
+            c.host[1][slots] = big.double().cpu().numpy()
+        else:
+            scale = torch.from_numpy(climb).float()
+            c.pools[0][0][at] = 0x38                                   # 1.0
+            c.pools[0][1].view(-1, 1)[at] = scale.cuda()[:, None]
+            c.host[0][slots] = scale.double().numpy()[:, None, None]
+            c.pools[1][1].view(-1, 1)[at] *= 2.0 ** 100
+            c.host[1][slots] *= 2.0 ** 100
+        c.call()
+        c.check()
