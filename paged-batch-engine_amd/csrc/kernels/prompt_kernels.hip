@@ -45,6 +45,7 @@
 #include "decode_device.h"
 #include "mxfp4_device.h"
 #include "prompt_kernels.h"
+#include "prompt_order.h"
 
 namespace pbe {
 namespace {
@@ -266,24 +267,11 @@ __device__ __forceinline__ bool find_tile(const PromptParams& p, int w, int lane
   }
   const Seq u = lane < p.batch ? seq_of<kKind, kRows>(p, lane) : Seq{};
   if (w >= __builtin_amdgcn_readlane(wave_scan(u.tiles), 63)) return false;
-  // Tiles of this lane's sequence that cost more than c: those from t on with base +
-  // step * (t + 1) > c.
-  const float base = (float)u.base, step = (float)u.step, a_step = u.step ? 1.f / step : 0.f;
-  auto above = [&](float c) {
-    const int below = u.step ? min(u.tiles, max(0, (int)floorf((c - base) * a_step))) : base > c ? 0 : u.tiles;
-    return u.tiles - below;
-  };
-  // The largest cost (of some float grid) that at most w tiles pass: then those that
-  // pass it are before tile w, and what is left is taken in the sequences' order.
-  float low = 0.f, high = (float)wave_max_int((int)min((int64_t)0x7fffff00, u.cost(u.tiles) / 16 + 1)) * 16.f;
-  for (int i = 0; i < 14; ++i) {
-    const float mid = 0.5f * (low + high);
-    const bool few = __builtin_amdgcn_readlane(wave_scan(above(mid)), 63) <= w;
-    high = few ? mid : high;
-    low = few ? low : mid;
-  }
-  // `high` is passed by at most w tiles, `low` by more: tile w is among those between.
-  const int over = above(high), between = above(low) - over;
+  const TileRun run = tile_run(u.tiles, u.base, u.step);
+  const uint32_t costs_end = cost_end(wave_max_int(u.tiles ? (int)(u.cost(u.tiles - 1) / 32) : 0));
+  const CostRange costs = costs_of(costs_end, w, [&](uint32_t c) { return __builtin_amdgcn_readlane(wave_scan(tiles_above(run, c)), 63); });
+  // what is left between them is taken in the sequences' order
+  const int over = tiles_above(run, costs.high), between = tiles_above(run, costs.low) - over;
   const int rank = w - __builtin_amdgcn_readlane(wave_scan(over), 63);
   const int upto = wave_scan(between);
   const int b = __builtin_ctzll(__ballot(upto > rank));

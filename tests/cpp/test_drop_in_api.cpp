@@ -9,7 +9,9 @@
 #include <memory>
 #include <numeric>
 #include <random>
+#include <set>
 #include <stdexcept>
+#include <utility>
 #include <vector>
 
 #include "base/global_chunk_allocator.h"
@@ -28,6 +30,7 @@
 #include "base/block_allocator.h"
 #include "base/kv_cache_manager.h"
 #include "base/page_index.h"
+#include "kernels/prompt_order.h"
 #include "kernels/xcd_order.h"
 
 using namespace cache;
@@ -1519,6 +1522,108 @@ TEST_CASE("page index: multiply-shift quotient equals id / stride, -1 off the pa
     CHECK_EQ(pi.of(INT32_MAX - INT32_MAX % stride), INT32_MAX / stride);
   }
   CHECK_EQ(base::PageIndex(1).of(12345), 12345);
+}
+
+namespace {
+// A prompt batch's tiles in the order of the prompt reader's workgroups: sequences of
+// `news` query tokens and `lens` keys, `group` query heads a KV head, `rows` a tile.
+// costs: of a sequence's tiles, base and step.
+std::vector<std::pair<int, int>> prompt_tile_order(const std::vector<int64_t>& news, const std::vector<int64_t>& lens, int64_t group,
+                                                   int64_t rows, std::vector<std::pair<int64_t, int64_t>>* costs, std::vector<pbe::TileRun>* runs) {
+  runs->clear(), costs->clear();
+  int64_t total = 0, most = 0;
+  for (size_t b = 0; b < news.size(); ++b) {
+    const int64_t tiles = (news[b] * group + rows - 1) / rows, base = 2048 + 16 * std::max<int64_t>(0, lens[b] - news[b]);
+    const int64_t step = lens[b] ? 16 * rows / group : 0;
+    costs->push_back({base, step});
+    runs->push_back(pbe::tile_run((int32_t)tiles, base, step));
+    total += tiles;
+    if (tiles) most = std::max(most, base + step * tiles);
+  }
+  const uint32_t end = pbe::cost_end((int32_t)(most / 32));
+  std::vector<std::pair<int, int>> order;
+  for (int64_t w = 0; w < total; ++w) {
+    auto above = [&](uint32_t c) {
+      int64_t n = 0;
+      for (const pbe::TileRun& r : *runs) n += pbe::tiles_above(r, c);
+      return n;
+    };
+    const pbe::CostRange range = pbe::costs_of(end, w, above);
+    int64_t rank = w - above(range.high);
+    std::pair<int, int> at{-1, -1};
+    for (size_t b = 0; b < runs->size(); ++b) {
+      const int32_t over = pbe::tiles_above((*runs)[b], range.high), between = pbe::tiles_above((*runs)[b], range.low) - over;
+      if (rank < between) {
+        at = {(int)b, (int)((*runs)[b].tiles - 1 - over - rank)};
+        break;
+      }
+      rank -= between;
+    }
+    order.push_back(at);
+  }
+  return order;
+}
+}  // namespace
+
+TEST_CASE("prompt tiles: every tile of a batch is taken once, the costly ones first") {
+  std::mt19937_64 rng(11);
+  const int64_t most_len = 0x7fffff00;
+  // where counts that were not pinned at the search's end lost tiles
+  const std::vector<std::vector<int64_t>> fixed_news{{17, 14}, {1, 5}, {5, 5}};
+  const std::vector<std::vector<int64_t>> fixed_lens{{134323040, 134323112}, {16777287, 16777344}, {33554515, 33554555}};
+  for (int i = 0; i < 3000; ++i) {
+    std::vector<int64_t> news, lens;
+    int64_t rows = 32 << rng() % 4, group = std::vector<int64_t>{1, 2, 3, 6, 7, 14, 64, 128, 256, 4096, 5000}[rng() % 11];
+    if (i < 3) {
+      news = fixed_news[i], lens = fixed_lens[i], rows = 64;
+      group = i ? 256 : 7;
+    } else {
+      const int batch = 1 + rng() % (i % 5 ? 4 : 64);
+      const int64_t tokens = 1 + (int64_t)(rng() % 400) * rows / group / batch;
+      const int64_t far = 1ll << rng() % 31;
+      for (int b = 0; b < batch; ++b) {
+        news.push_back((int64_t)(rng() % (2 * tokens + 1)));
+        const int64_t near = rng() % 3 ? far + (int64_t)(rng() % 300) : (int64_t)(rng() % (uint64_t)(far + 1));
+        lens.push_back(rng() % 9 ? std::min(most_len - (int64_t)(rng() % 2), near) : 0);
+      }
+    }
+    std::vector<pbe::TileRun> runs;
+    std::vector<std::pair<int64_t, int64_t>> costs;
+    const auto order = prompt_tile_order(news, lens, group, rows, &costs, &runs);
+    std::set<std::pair<int, int>> seen;
+    int64_t least = INT64_MAX, most = 0;
+    for (size_t b = 0; b < runs.size(); ++b)
+      if (runs[b].tiles) most = std::max(most, costs[b].first + costs[b].second * runs[b].tiles);
+    for (const auto& at : order) {
+      REQUIRE(at.first >= 0);
+      REQUIRE(at.second >= 0 && at.second < runs[at.first].tiles);
+      REQUIRE(seen.insert(at).second);
+      const int64_t cost = costs[at.first].first + costs[at.first].second * (at.second + 1);
+      // the range that 14 halvings leave, and what a count may be off
+      REQUIRE(cost <= least || cost - least <= most / 8192 + 2 * costs[at.first].second + 64);
+      least = std::min(least, cost);
+    }
+  }
+  // as many tiles as a call can have: all at 0, none at the end, never more at a higher cost
+  for (const int64_t len : {(int64_t)1, (int64_t)1 << 24, most_len})
+    for (const int64_t rows : {64, 128, 256})
+      for (const int64_t group : {(int64_t)1, (int64_t)7, (int64_t)300, (int64_t)1 << 20, most_len}) {
+        for (const int64_t tokens : {(int64_t)1, most_len / group / 2, most_len / group}) {
+          const int64_t tiles = (tokens * group + rows - 1) / rows, base = 2048 + 16 * std::max<int64_t>(0, len - tokens), step = 16 * rows / group;
+          const pbe::TileRun r = pbe::tile_run((int32_t)tiles, base, step);
+          const int64_t most = base + step * tiles;
+          REQUIRE(most / 32 <= INT32_MAX);
+          const uint32_t end = pbe::cost_end((int32_t)(most / 32));
+          REQUIRE((int64_t)end * 16 > most);
+          REQUIRE(pbe::tiles_above(r, 0) == tiles && pbe::tiles_above(r, end) == 0);
+          int32_t last = (int32_t)tiles;
+          for (int64_t i = 0; i <= 20000; ++i) {
+            const int32_t n = pbe::tiles_above(r, (uint32_t)((int64_t)end * i / 20000));
+            REQUIRE(n >= 0 && n <= last);
+            last = n;
+          }
+        }
+      }
 }
 
 TEST_CASE("xcd grouping: the copy kernels' workgroup renumbering is a bijection") {
