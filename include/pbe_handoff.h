@@ -675,8 +675,8 @@ int pbe_qk_norm_rope_scatter(const void* q, int64_t q_stride, const void* k, int
  * current GPU) few rows over many keys are read in pieces that fill the GPU; with
  * less, or NULL, in fewer or none. outputs may be the queries themselves (rows that
  * lie one after another); but for that, outputs and workspace may overlap neither
- * each other nor anything read. rows * q_heads at most INT32_MAX - 255. All
- * arrays in memory of `device`; no rows are no work. Asynchronous on `stream`, one
+ * each other nor anything read. rows * q_heads and batch at most INT32_MAX - 255.
+ * All arrays in memory of `device`; no rows are no work. Asynchronous on `stream`, one
  * launch, or two where rows are read in pieces; the calls can be captured. */
 uint64_t pbe_prompt_workspace_bytes(int32_t n_rows, int32_t batch, int32_t q_heads,
                                     int32_t kv_heads, int32_t head_dim);

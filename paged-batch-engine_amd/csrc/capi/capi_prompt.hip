@@ -14,7 +14,7 @@ using namespace pbe_capi;
 namespace {
 
 constexpr uint64_t kTokens = 16;
-constexpr int32_t kMostTokens = INT32_MAX - 255;  // so that a tile's end fits 31 bits
+constexpr int32_t kMostTokens = INT32_MAX - 255;  // so that a tile's end fits 31 bits, and 64 sequences behind the last
 
 struct Call {
   const void* queries;
@@ -30,6 +30,7 @@ struct Call {
 int check(const Call& c, int device) {
   if (c.n_rows < 0 || c.batch <= 0 || c.q_heads <= 0 || c.kv_heads <= 0 || device < 0)
     return fail(PBE_ERR_INVALID, "query rows >= 0, batch, q_heads, kv_heads > 0 and a device");
+  if (c.batch > kMostTokens) return fail(PBE_ERR_INVALID, "batch must be at most %d", (int)kMostTokens);
   if (c.head_dim != 64 && c.head_dim != 128) return fail(PBE_ERR_UNSUPPORTED, "heads of 64 or 128 dims");
   if (c.q_heads % c.kv_heads) return fail(PBE_ERR_UNSUPPORTED, "q_heads must be a multiple of kv_heads");
   if ((int64_t)c.n_rows * c.q_heads > kMostTokens) return fail(PBE_ERR_INVALID, "rows * q_heads must be at most %d", (int)kMostTokens);
