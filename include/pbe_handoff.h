@@ -742,8 +742,8 @@ int pbe_paged_prompt_attention(const void* key_pool, const void* value_pool, uin
  *     completes and holding anything when it starts.
  * Arrays 4-byte aligned and in memory of `device`; outputs and workspace may
  * overlap nothing else of a call, nor any array the planes. Rows *
- * max_blocks_per_seq and n_pages * id_stride at most INT32_MAX. Asynchronous on
- * `stream`, two launches; the calls can be captured. */
+ * max_blocks_per_seq and n_pages * id_stride at most INT32_MAX, rows of a fork at most
+ * INT32_MAX - 1023. Asynchronous on `stream`, two launches; the calls can be captured. */
 typedef struct pbe_page_plane {
   pbe_arena_view memory;
   uint64_t page_bytes;

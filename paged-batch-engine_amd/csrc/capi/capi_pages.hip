@@ -100,6 +100,7 @@ int pbe_fork_pages(const pbe_page_plane* planes, int32_t n_planes, int32_t n_pag
     return fail(PBE_ERR_INVALID, "block_size, rows and max_blocks_per_seq > 0 and a device");
   int rc = check_pool(n_pages, id_stride);
   if (rc != PBE_OK) return rc;
+  if (std::max(rows_in, rows_out) > pbe::kMostRows) return fail(PBE_ERR_INVALID, "at most %d rows", (int)pbe::kMostRows);
   if ((int64_t)std::max(rows_in, rows_out) * max_blocks_per_seq > INT32_MAX)
     return fail(PBE_ERR_INVALID, "rows * max_blocks_per_seq must be at most INT32_MAX");
   if (!tables_in || !lens_in || !parents || !tables_out || !lens_out || !counts || !workspace) return fail(PBE_ERR_INVALID, "null page mover operand");

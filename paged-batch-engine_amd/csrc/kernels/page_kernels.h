@@ -11,6 +11,7 @@ namespace pbe {
 constexpr int kPagePlanes = 112;         // pools of a call
 constexpr int kPageBases = 224;          // their allocations
 constexpr int32_t kMostPages = 1 << 20;  // bits of the plan's map, in LDS
+constexpr int32_t kMostRows = 0x7fffffff - 1023;  // the plan counts 1,024 rows at a time
 constexpr uint32_t kPageSlice = 16384;   // bytes that a workgroup copies at a time
 constexpr uint32_t kPageEntries = 1024;  // table entries of a workgroup
 constexpr int kPageHeader = 16;          // first words of a workspace

@@ -26,6 +26,7 @@ namespace pbe {
 namespace {
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+static_assert(kMostRows <= 0x7fffffff - (kPlanThreads - 1), "a row's number and the next turn's fit 31 bits");
 constexpr int kWords = kMostPages / 32;
 constexpr int kForkRows = 3584;  // whose first children fit LDS beside the map; more take the workspace
 constexpr uint32_t kCopyGroup = 192 * 1024 / kPageSlice;  // slices that an XCD takes one after another
