@@ -345,15 +345,15 @@ __device__ __forceinline__ uint32_t code_at(uint32_t r, uint32_t c) { return r *
 // A lane's 16 (or 4) bytes to LDS, lane after lane from `to` on, past the registers.
 // Written as instructions because the compiler would wait for the builtin's result
 // before any read of LDS; here arrived() says when it is there. They write no
-// register but m0, which nothing else here uses.
+// register but m0.
 __device__ __forceinline__ void load_to_lds(const uint8_t* from, PBE_LDS uint8_t* to) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"((uint32_t)(uintptr_t)to) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"((uint32_t)(uintptr_t)to) : "memory", "m0");
 }
 __device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t lane_at, PBE_LDS uint8_t* to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_at), "s"(base), "s"((uint32_t)(uintptr_t)to) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_at), "s"(base), "s"((uint32_t)(uintptr_t)to) : "memory", "m0");
 }
 __device__ __forceinline__ void load_word_to_lds(const uint8_t* from, PBE_LDS uint8_t* to) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"((uint32_t)(uintptr_t)to) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"((uint32_t)(uintptr_t)to) : "memory", "m0");
 }
 // Waits until at most kLeft of what this wave has asked global memory for is on its way.
 template <int kLeft>
