@@ -345,7 +345,10 @@ __device__ __forceinline__ uint32_t code_at(uint32_t r, uint32_t c) { return r *
 // A lane's 16 (or 4) bytes to LDS, lane after lane from `to` on, past the registers.
 // Written as instructions because the compiler would wait for the builtin's result
 // before any read of LDS; here arrived() says when it is there. They write no
-// register but m0.
+// register but m0. That one is reserved, of which the compiler warns; it still takes the
+// clobber as a write that uses of m0 of its own (here there are none) may not pass.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(const uint8_t* from, PBE_LDS uint8_t* to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"((uint32_t)(uintptr_t)to) : "memory", "m0");
 }
@@ -355,6 +358,7 @@ __device__ __forceinline__ void load_to_lds(const uint8_t* base, uint32_t lane_a
 __device__ __forceinline__ void load_word_to_lds(const uint8_t* from, PBE_LDS uint8_t* to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"((uint32_t)(uintptr_t)to) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 // Waits until at most kLeft of what this wave has asked global memory for is on its way.
 template <int kLeft>
 __device__ __forceinline__ void arrived() {
