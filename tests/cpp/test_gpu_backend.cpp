@@ -1412,4 +1412,92 @@ TEST_CASE("model runtime: a chunk's query tokens attend to its pages") {
   REQUIRE(pbe_stream_destroy(0, stream) == PBE_OK);
 }
 
+TEST_CASE("model runtime: a long chunk without a workspace, over its queries") {
+  const int H = 2, D = 128, B = 16, nblk = 70, kvm = 6, max_blocks = 66;
+  void* stream = nullptr;
+  REQUIRE(pbe_stream_create(0, &stream) == PBE_OK);
+  const model::HipPagedKVRuntime runtime(0, stream);
+  std::vector<int32_t> table(2 * max_blocks, -1);
+  for (int i = 0; i < 63; ++i) table[i] = (i * 11) % nblk;  // 11 and 70 have no factor in common: blocks of their own
+  for (int i = 0; i < 3; ++i) table[max_blocks + i] = ((63 + i) * 11) % nblk;
+  const std::vector<int32_t> lens{1000, 40}, starts{0, 45, 85};
+  const int rows = starts[2] + 1;
+  const size_t row = static_cast<size_t>(kvm) * H * D * 2;
+  const auto q = random_bf16(rows * kvm * H * D, 95);
+  int32_t* dt = to_device(table);
+  int32_t* dl = to_device(lens);
+  int32_t* ds = to_device(starts);
+  uint8_t* dq = to_device(q);
+  const uint64_t ws_bytes = pbe_prompt_workspace_bytes(rows, 2, kvm * H, H, D);
+  REQUIRE(ws_bytes > 0);
+  uint8_t *out = nullptr, *ws = nullptr;
+  HIP_OK(hipMalloc(&out, q.size()));
+  HIP_OK(hipMalloc(&ws, ws_bytes));
+  REQUIRE(dt && dl && ds && dq);
+  auto value = [](const std::vector<uint8_t>& x, size_t i) {
+    const uint32_t bits = (static_cast<uint32_t>(x[2 * i]) | static_cast<uint32_t>(x[2 * i + 1]) << 8) << 16;
+    float f;
+    std::memcpy(&f, &bits, 4);
+    return f;
+  };
+  for (const bool fp8 : {false, true}) {
+    base::BlockAllocator blocks(nblk, B, H, D, base::DataType::kDataTypeBf16, base::DeviceType::kDeviceHIP,
+                                fp8 ? base::BlockStorageMode::kFp8E4M3PerTokenHead : base::BlockStorageMode::kPlain);
+    const base::KVPoolView pool = blocks.pool_view();
+    const auto K = random_bf16(nblk * B * H * D, 96), V = random_bf16(nblk * B * H * D, 97);
+    std::vector<int32_t> slots(nblk * B);
+    for (int i = 0; i < nblk * B; ++i) slots[i] = i;
+    uint8_t* dK = to_device(K);
+    uint8_t* dV = to_device(V);
+    int32_t* dS = to_device(slots);
+    REQUIRE(dK && dV && dS);
+    runtime.scatter(dK, dV, base::DataType::kDataTypeBf16, pool, dS, B, H, D, nblk * B);
+    HIP_OK(hipMemset(out, 0x3f, q.size()));
+    model::PagedKVPrefillRuntimeArgs a;
+    a.n_rows = rows;
+    a.batch_size = 2;
+    a.head_num = kvm * H;
+    a.head_size = D;
+    a.kv_mul = kvm;
+    a.max_blocks_per_seq = max_blocks;
+    a.block_size = B;
+    a.num_kv_heads = H;
+    a.queries = dq;
+    a.outputs = out;
+    a.token_starts = ds;
+    a.block_tables = dt;
+    a.seq_lens = dl;
+    a.workspace = ws;
+    a.workspace_bytes = ws_bytes;
+    CHECK(runtime.prefill(pool, a));
+    REQUIRE(pbe_stream_synchronize(0, stream) == PBE_OK);
+    const auto in_parts = to_host(out, q.size());
+    a.workspace = nullptr;
+    a.workspace_bytes = 0;
+    a.queries = out;
+    HIP_OK(hipMemcpy(out, q.data(), q.size(), hipMemcpyHostToDevice));
+    CHECK(runtime.prefill(pool, a));
+    REQUIRE(pbe_stream_synchronize(0, stream) == PBE_OK);
+    const auto whole = to_host(out, q.size());
+    // Of values below M either is off by less than 2^-8 M by its output's rounding, 2^-8
+    // (1 + 2^-7) M by its weights', and 2^-12 M by FP32's.
+    float most = 0.f, apart = 0.f;
+    for (size_t i = 0; i < V.size() / 2; ++i) most = std::max(most, std::fabs(value(V, i)));
+    bool numbers = true;
+    for (size_t i = 0; i < starts[2] * row / 2; ++i) {
+      numbers &= std::isfinite(value(whole, i)) && std::isfinite(value(in_parts, i));
+      apart = std::max(apart, std::fabs(value(whole, i) - value(in_parts, i)));
+    }
+    CHECK(numbers);
+    CHECK(apart <= 2.f * (1.f / 128.f + 1.f / 2048.f) * most * (fp8 ? 1.0625f : 1.f));  // E4M3 values: 2^-4 more
+    bool kept = true;  // the row behind the last sequence: what was there
+    for (size_t i = starts[2] * row; i < q.size(); ++i) kept &= whole[i] == q[i] && in_parts[i] == 0x3f;
+    CHECK(kept);
+    for (void* x : {static_cast<void*>(dK), static_cast<void*>(dV), static_cast<void*>(dS)}) HIP_OK(hipFree(x));
+  }
+  for (void* x : {static_cast<void*>(dt), static_cast<void*>(dl), static_cast<void*>(ds), static_cast<void*>(dq), static_cast<void*>(out), static_cast<void*>(ws)})
+    HIP_OK(hipFree(x));
+  REQUIRE(pbe_stream_destroy(0, stream) == PBE_OK);
+}
+
 MINITEST_MAIN()
