@@ -666,9 +666,11 @@ int pbe_qk_norm_rope_scatter(const void* q, int64_t q_stride, const void* k, int
  * zero, +infinity, NaN, or -infinity for all keys that a query sees, its head to
  * NaN. Weights (up to 2^8, their largest at least 1) times values are summed in FP32
  * before they are divided, so values beyond 2^119 over a row's keys may end as
- * infinities. Query rows that belong to no sequence are left as they are. The order of a
- * row's sums, and with it the last bits of its outputs, depends on the batch it is
- * in and on the workspace's size; for one call they are the same every time.
+ * infinities, and sums over n keys may be off by 2^-23 of what they add up for every 16 of
+ * them: of tens of millions of keys fewer digits are left. Query rows that belong to
+ * no sequence are left as they are. The order of a row's sums, and with it the last bits
+ * of its outputs, depends on the batch it is in and on the workspace's size; for one
+ * call they are the same every time.
  *
  * workspace: device memory, 16-byte aligned, used until the call completes and
  * holding anything when it starts. With pbe_prompt_workspace_bytes() of it (of the

@@ -8,11 +8,13 @@
 // sum: the lowest ones, in order.
 //
 // Bound: the plan, for small pools: a chain of table reads, marks and scans in one
-// workgroup, 3 to 6 us, which several workgroups with a pass over the grid between them
-// would not shorten; then the copies, two passes over the pages' bytes at HBM's rate.
-// One page of 458,752 bytes forked four ways 10.5 us, 64 x 4 drafts forked 18.3 us, 96
-// pages compacted 8.6 us, 200 of 1,024 pages of 917,504 bytes moved 72 us (5.2 TB/s
-// read and written; a large library copy 6.6 TB/s).
+// workgroup, 6 to 9 us for a fork and 4 to 5 for a compaction (kernel trace), which several
+// workgroups with a pass over the grid between them would not shorten; then the copies, two
+// passes over the pages' bytes at HBM's rate. One page of 458,752 bytes forked four ways
+// 10.4 us, 64 x 4 drafts forked 18.9 us, 96 pages compacted 9.2 us, 200 of 1,024 pages of
+// 917,504 bytes moved 72 us (5.1 TB/s read and written; a large library copy 6.6 TB/s).
+// One workgroup's plan grows with the tables: 256 rows of 2,048 entries over 2^17 pages
+// take a fork 128 us and a compaction that moves nothing 196.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

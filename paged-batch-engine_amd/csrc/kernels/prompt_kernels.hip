@@ -14,9 +14,10 @@
 //
 // Bound: MFMA, 4 * D FLOP a row and seen key. 4 * 128 dims take 32 products of 8
 // passes each a wave and tile, beside about 400 instructions for 64 weights a lane pair.
-// Over 8,192 tokens of 28 heads of 128 dims: 455 to 477 us by run, 1,010 to 1,058
-// TFLOP/s, of the 1,387 that a large matrix product reaches here; MFMA busy 49% at 2.05
-// GHz (the clock falls as the kernel gets faster). A SIMD's two waves share a barrier a
+// Over 8,192 tokens of 28 heads of 128 dims, back to back in a graph: 455 to 497 us by GPU
+// (one GPU repeats itself within 1%), 969 to 1,058 TFLOP/s, of the 1,387 that a large
+// matrix product reaches; MFMA busy 49% at 2.05 GHz (the clock falls as the kernel gets
+// faster). A SIMD's two waves share a barrier a
 // tile and mostly multiply, and mostly weigh, at the same time. Leaving out the
 // exponentials, or the maxima, or the sums, takes 6 to 9% off (on the way there, of 526
 // us): no single part is the bound.
@@ -163,9 +164,9 @@ __device__ __forceinline__ Found find_seq(int batch, int64_t x, int lane, Of of)
 // the GPU holds at once; a part is the end of a tile, whole tiles, the start of another.
 // A cut tile's partial results go to the workspace and prompt_join_kernel joins them.
 // The device does all of it from the starts and lengths, so captured calls follow them.
-// 2,041 tokens behind 5,040 others, 12 heads: 109 us. What it costs: 2.5 to 3.3 us to
-// find a part, about 3 to write partials, 9 to 16 the join (of 256 rows a tile, some 40 MB
-// of partials).
+// 2,041 tokens behind 5,040 others, 12 heads: 105 to 110 us. What it costs: 2.5 to 3.3 us
+// to find a part, about 3 to write partials, 9 to 16 the join (15 here: of 256 rows a
+// tile, some 40 MB of partials).
 // Where there are two tiles a slot or more, a workgroup takes one whole tile and those
 // that cost the most go first (16 mixed prompts: 96 us; cut into parts 126).
 //
@@ -578,8 +579,10 @@ __device__ __forceinline__ void workgroup_of(const PromptParams& p, int* w, int*
 // barrier a tile (MXFP4: two), behind which the tile read before is overwritten.
 // Registers: O 4 x 16, scores 32, Q 32, weights 16; two waves a SIMD.
 // FP8 codes become BF16 operands at the LDS reads: once a tile instead, into BF16 tiles,
-// took the same time (130.8 and 130.4 us, 128 tokens at the end of 32,768) and more LDS. The matrix product of 8-bit operands is no faster at this shape and would
-// round the queries.
+// took the same time (130.8 and 130.4 us, 128 tokens at the end of 32,768) and more LDS.
+// A lane reads eight of a chunk's 16 codes of a key, so each half of a wave uses half of
+// the banks (37% of the kernel's LDS cycles are conflicts; over rows none). The matrix
+// product of 8-bit operands is no faster at this shape and would round the queries.
 template <int D, KeyKind kKind, int kWaves>
 __global__ __launch_bounds__(64 * kWaves, kWaves > 2 ? 2 : 1) void prompt_attention_kernel(const PromptParams p) {
   using S = Stage<D, kKind, kWaves>;
@@ -897,9 +900,10 @@ __global__ __launch_bounds__(64 * kWaves, kWaves > 2 ? 2 : 1) void prompt_attent
 
 // Joins the tiles that were cut: o = sum 2^((m_i - m) scale) o_i / sum 2^((m_i - m)
 // scale) l_i, in the parts' order. Of a tile's n + 1 parts, each of the n that do not
-// begin it has a workgroup here, which takes its share of the tile's rows. A launch of
-// its own: the last part to end a tile joining it instead would need flags that every
-// call clears, and would leave the join's order of sums to chance or wait for it.
+// begin it has a workgroup here, which takes its share of the tile's rows: a launch of its
+// own, so that as many workgroups join as there are parts. The last part to arrive at a
+// tile could join it instead, by tickets (arrival.h) and in the same order; one workgroup
+// would then read all of a tile's partials. That was not tried.
 constexpr int kTogether = 4;  // loads of a thread that are on their way together
 template <int D, int kRows>
 constexpr int join_threads() {
@@ -953,7 +957,8 @@ __global__ __launch_bounds__((join_threads<D, kRows>())) void prompt_join_kernel
   // A thread has kTogether rows and a part at a time, or, where the share has no more
   // rows than are under way at once, a row and kTogether parts (128 tokens at the end of
   // 32,768: 129 to 119 us; 4 x 4 tokens over 5,040: 35 to 30). Eight parts take registers
-  // that cost more workgroups at once than they save: 64 x 4 over MXFP4 pages 81 to 90.
+  // that cost more workgroups at once than they save: 64 x 4 tokens of 28 heads of 128 dims
+  // over MXFP4 pages 81 to 90.
   const bool few = to - from <= kStep;
   const int next_row = few ? 0 : kStep, next_part = few ? 1 : 0;
   auto add_to = [&](float& m, float& l, f32x4& acc, float pm, float pl, f32x4 x) {
@@ -1054,11 +1059,12 @@ PromptPlan plan_prompt(int64_t n_q, int64_t batch, int32_t group, int32_t kv_hea
   // cache less often (256 and 128 rows a tile over 8,192 tokens: 469 and 495 us; over
   // 2,041 behind 5,040: 109 and 122), rows that no token fills cost as much as others.
   r.rows = rows <= 64 * batch ? 64 : rows <= 128 * batch ? 128 : 256;
-  // A wave alone loads and waits by itself, and is slower (64 x 4 tokens over MXFP4 pages
-  // of 128 dims: 66 us, two waves with one at work 54; over BF16 pages 80 and 81; 4 x 4
-  // over FP8 pages 40 and 34), but for FP8 pages of 128 dims and heads enough for a
-  // quarter of the GPU: 64 x 4 tokens 57 and 70, 16 x 4 of four KV heads 45 and 48, 16 x
-  // 4 of two 46 and 42.
+  // A wave alone loads and waits by itself, and is slower (64 x 4 tokens of 12 heads of 128
+  // dims over 5,040 of MXFP4 pages: 66 us, two waves with one at work 54; of BF16 pages 80
+  // and 81; 4 x 4 over FP8 pages 40 and 34), but for FP8 pages of 128 dims and heads enough
+  // for a quarter of the GPU: 64 x 4 tokens 57 and 70, 16 x 4 of four KV heads 45 and 48,
+  // 16 x 4 of two 46 and 42 (all before the join took four parts at once; 64 x 4 is 53 with
+  // it). Three batches are few for such a border.
   if (rows <= 32 * batch && kind == KeyKind::kFp8 && head_dim == 128 && 4 * batch * kv_heads >= units) r.rows = 32;
   // Few short prompts, whose tiles are not cut: smaller tiles, so that more compute units
   // have one (41 tokens of 14 heads of 64 dims: 256 rows a tile 7.2 us, 128 5.9, 64 5.6;
